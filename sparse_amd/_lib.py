@@ -55,7 +55,19 @@ class SegList(C.Structure):
     ]
 
 
+class Fp8Matrix(C.Structure):
+    """``sparse_hip_fp8_matrix``."""
+
+    _fields_ = [
+        ("values_dev", C.c_void_p),
+        ("scales_dev", C.c_void_p),
+        ("rows", C.c_int32),
+        ("cols", C.c_int32),
+    ]
+
+
 _vp, _i, _sz = C.c_void_p, C.c_int, C.c_size_t
+_mat = C.POINTER(Fp8Matrix)
 
 # name -> (restype, argtypes); every symbol include/sparse_hip.h declares
 SIGNATURES = {
@@ -100,6 +112,15 @@ SIGNATURES = {
     "sparse_hip_combine_split": (_i, [_vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp, _vp]),
     "sparse_hip_shared_expert": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp]),
     "sparse_hip_combine": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
+    "sparse_hip_gate_select": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, C.c_float, _i, _vp, _vp, _vp]),
+    "sparse_hip_fp8_quantize": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
+    "sparse_hip_fp8_linear_ws_bytes": (_sz, [_i, _i]),
+    "sparse_hip_fp8_linear": (_i, [_vp, _vp, _vp, _i, _i, _mat, _vp, _vp, _vp]),
+    "sparse_hip_fp8_slot_bytes": (_sz, [_i, _i]),
+    "sparse_hip_fp8_moe_ffn_ws_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "sparse_hip_fp8_moe_ffn": (
+        _i, [C.POINTER(Experts), _vp, _vp, _vp, _vp, C.POINTER(SegList), _i, _i, _vp, _mat, _mat, _mat, _vp, _vp, _vp,
+             _vp]),
     "sparse_hip_expert_upload_async": (_i, [_vp, _vp, _sz, _vp, _vp]),
     "sparse_hip_event_create": (_i, [_i, C.POINTER(_vp)]),
     "sparse_hip_event_destroy": (_i, [_vp]),

@@ -30,6 +30,10 @@ SOURCES = [
     "ffn_tiled.hip",
     "ffn.hip",
     "combine.hip",
+    "gate_select.hip",
+    "fp8.hip",
+    "fp8_quantize.hip",
+    "fp8_stream.hip",
     "rs_predict.hip",
     "layout.hip",
     "mfma_probe.hip",

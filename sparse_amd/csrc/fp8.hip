@@ -1,0 +1,247 @@
+// C ABI of the block-scaled 8-bit operators: argument checks and the order of launches.
+#include "fp8.h"
+
+namespace sparse {
+
+static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static inline size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+constexpr int kF8MaxDim = 1 << 20;
+constexpr int64_t kF8MaxRows = 1ll << 30;
+
+// A workspace handed out front to back in 256-byte steps; with a null base it only counts.
+struct Carve {
+  uint8_t* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    void* p = base == nullptr ? nullptr : base + used;
+    used += up256(bytes);
+    return p;
+  }
+};
+
+struct F8Rows {
+  uint8_t *values, *scales;
+};
+static F8Rows take_rows(Carve& c, int64_t rows, int K) {
+  F8Rows r;
+  r.values = static_cast<uint8_t*>(c.take(static_cast<size_t>(rows) * f8_padded(K)));
+  r.scales = static_cast<uint8_t*>(c.take(static_cast<size_t>(rows) * f8_blocks(K)));
+  return r;
+}
+
+struct LinearWs {
+  F8Rows x;
+  size_t bytes;
+};
+static LinearWs linear_ws(void* ws, int T, int K) {
+  Carve c{static_cast<uint8_t*>(ws)};
+  LinearWs w;
+  w.x = take_rows(c, T, K);
+  w.bytes = c.used;
+  return w;
+}
+
+struct FfnWs {
+  F8Rows x, h, sh;
+  float *hf, *shf;
+  size_t bytes;
+};
+static FfnWs ffn_ws(void* ws, int T, int K, int nseg, int H, int I, int Is) {
+  Carve c{static_cast<uint8_t*>(ws)};
+  FfnWs w = {};
+  const int64_t rows = nseg > 0 ? static_cast<int64_t>(T) * K : 0;
+  w.x = take_rows(c, T, H);
+  w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
+  w.h = take_rows(c, rows, I);
+  if (Is > 0) {
+    w.shf = static_cast<float*>(c.take(static_cast<size_t>(T) * Is * sizeof(float)));
+    w.sh = take_rows(c, T, Is);
+  }
+  w.bytes = c.used;
+  return w;
+}
+
+static int check_matrix(const char* fn, const char* name, const sparse_hip_fp8_matrix* m, int rows, int cols) {
+  SP_REQUIRE(m->rows == rows && m->cols == cols, "%s: %s is [%d,%d], must be [%d,%d]", fn, name, m->rows, m->cols, rows, cols);
+  SP_REQUIRE(m->values_dev && m->scales_dev, "%s: %s has a NULL pointer", fn, name);
+  SP_REQUIRE(aligned16(m->values_dev), "%s: %s values must be 16-byte aligned", fn, name);
+  return SPARSE_HIP_OK;
+}
+
+}  // namespace sparse
+
+using namespace sparse;
+
+extern "C" {
+
+int sparse_hip_fp8_quantize(const void* x_dev, int dtype, int T, int K, void* values_dev, void* scales_dev, void* stream) {
+  SP_REQUIRE(valid_dtype(dtype), "fp8_quantize: unknown dtype %d", dtype);
+  SP_REQUIRE(T >= 0 && K >= 1 && K <= kF8MaxDim, "fp8_quantize: T=%d, K=%d outside [0,..] x [1,%d]", T, K, kF8MaxDim);
+  if (T == 0) return SPARSE_HIP_OK;
+  SP_REQUIRE(x_dev && values_dev && scales_dev, "fp8_quantize: NULL pointer");
+  SP_REQUIRE(aligned16(values_dev), "fp8_quantize: values must be 16-byte aligned");
+  return f8_quantize(x_dev, dtype, T, K, values_dev, scales_dev, as_stream(stream));
+}
+
+size_t sparse_hip_fp8_linear_ws_bytes(int T, int K) {
+  if (T <= 0 || K <= 0 || K > kF8MaxDim) return 0;
+  return linear_ws(nullptr, T, K).bytes;
+}
+
+int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_dev, int dtype, int T,
+                          const sparse_hip_fp8_matrix* weight, void* out_dev, void* ws_dev, void* stream) {
+  SP_REQUIRE(is_16bit(dtype), "fp8_linear: activations must be bf16 or fp16, got dtype %d", dtype);
+  SP_REQUIRE(weight != nullptr, "fp8_linear: NULL weight");
+  SP_REQUIRE(weight->rows >= 1 && weight->rows <= kF8MaxDim && weight->cols >= 1 && weight->cols <= kF8MaxDim,
+             "fp8_linear: weight is [%d,%d], each side must be in [1,%d]", weight->rows, weight->cols, kF8MaxDim);
+  int rc = check_matrix("fp8_linear", "weight", weight, weight->rows, weight->cols);
+  if (rc != SPARSE_HIP_OK) return rc;
+  SP_REQUIRE(T >= 0, "fp8_linear: T=%d", T);
+  if (T == 0) return SPARSE_HIP_OK;
+  SP_REQUIRE((x_dev != nullptr) != (xq_dev != nullptr), "fp8_linear: give x or its 8-bit rows");
+  SP_REQUIRE(out_dev != nullptr, "fp8_linear: NULL output");
+  hipStream_t st = as_stream(stream);
+  F8Product p = {};
+  if (x_dev != nullptr) {
+    SP_REQUIRE(ws_dev != nullptr && aligned16(ws_dev), "fp8_linear: workspace is NULL or not 16-byte aligned");
+    const LinearWs w = linear_ws(ws_dev, T, weight->cols);
+    rc = f8_quantize(x_dev, dtype, T, weight->cols, w.x.values, w.x.scales, st);
+    if (rc != SPARSE_HIP_OK) return rc;
+    p.act_s = w.x.values;
+    p.act_ss = w.x.scales;
+  } else {
+    SP_REQUIRE(xs_dev != nullptr && aligned16(xq_dev), "fp8_linear: 8-bit rows need scales and 16-byte alignment");
+    p.act_s = static_cast<const uint8_t*>(xq_dev);
+    p.act_ss = static_cast<const uint8_t*>(xs_dev);
+  }
+  p.w0 = static_cast<const uint8_t*>(weight->values_dev);
+  p.s0 = weight->scales_dev;
+  p.w1 = p.w0;
+  p.s1 = p.s0;
+  p.out_s = out_dev;
+  p.Ks = weight->cols;
+  p.Ns = weight->rows;
+  p.T = T;
+  p.dtype = dtype;
+  return f8_stream(p, false, false, true, st);
+}
+
+size_t sparse_hip_fp8_slot_bytes(int H, int I) {
+  if (H <= 0 || I <= 0 || H > kF8MaxDim || I > kF8MaxDim) return 0;
+  return f8_slot(H, I).bytes;
+}
+
+size_t sparse_hip_fp8_moe_ffn_ws_bytes(int T, int K, int num_segments, int H, int I, int Is) {
+  if (T <= 0 || K <= 0 || num_segments < 0 || H <= 0 || I <= 0 || Is < 0) return 0;
+  return ffn_ws(nullptr, T, K, num_segments, H, I, Is).bytes;
+}
+
+int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev, const void* topv_dev,
+                           const int32_t* perm_dev, const int32_t* seg_offsets_dev, const sparse_hip_seglist* segs,
+                           int T, int K, void* parts_dev, const sparse_hip_fp8_matrix* shared_gate_w,
+                           const sparse_hip_fp8_matrix* shared_up_w, const sparse_hip_fp8_matrix* shared_down_w,
+                           const void* shared_gate_dev, void* shared_dev, void* ws_dev, void* stream) {
+  static const char fn[] = "fp8_moe_ffn";
+  SP_REQUIRE(experts != nullptr && segs != nullptr, "%s: NULL descriptor", fn);
+  const int H = experts->hidden, I = experts->inter, E = experts->num_experts, dtype = experts->dtype;
+  SP_REQUIRE(is_16bit(dtype), "%s: activations must be bf16 or fp16, got dtype %d", fn, dtype);
+  SP_REQUIRE(E >= 1 && E <= SPARSE_HIP_MAX_EXPERTS, "%s: E=%d outside [1,%d]", fn, E, SPARSE_HIP_MAX_EXPERTS);
+  SP_REQUIRE(H > 0 && H % 64 == 0 && H <= kF8MaxDim, "%s: H=%d must be a positive multiple of 64", fn, H);
+  SP_REQUIRE(I > 0 && I % 64 == 0 && I <= kF8MaxDim, "%s: I=%d must be a positive multiple of 64", fn, I);
+  SP_REQUIRE(T >= 1 && K >= 1 && K <= SPARSE_HIP_MAX_TOPK, "%s: T=%d, K=%d outside [1,..] x [1,%d]", fn, T, K, SPARSE_HIP_MAX_TOPK);
+  SP_REQUIRE(static_cast<int64_t>(T) * K < kF8MaxRows, "%s: T=%d, K=%d: too many rows", fn, T, K);
+  SP_REQUIRE(segs->n >= 0 && segs->n <= SPARSE_HIP_MAX_EXPERTS, "%s: segment count %d outside [0,%d]", fn, segs->n, SPARSE_HIP_MAX_EXPERTS);
+  const F8Slot slot = f8_slot(H, I);
+  const bool routed = segs->n > 0, shared = shared_down_w != nullptr;
+  SP_REQUIRE(x_dev != nullptr, "%s: NULL x", fn);
+  if (routed) {
+    SP_REQUIRE(experts->slab_dev != nullptr && aligned16(experts->slab_dev), "%s: weight slab is NULL or not 16-byte aligned", fn);
+    SP_REQUIRE(experts->slot_stride >= slot.bytes && experts->slot_stride % 16 == 0, "%s: slot_stride=%llu too small or not 16-byte aligned", fn,
+               static_cast<unsigned long long>(experts->slot_stride));
+    SP_REQUIRE(topv_dev && perm_dev && seg_offsets_dev && parts_dev, "%s: NULL pointer", fn);
+    SP_REQUIRE(aligned16(parts_dev), "%s: parts must be 16-byte aligned", fn);
+    if (segs->eids_dev != nullptr) {
+      SP_REQUIRE(segs->count_dev != nullptr && experts->expert_slot_dev != nullptr, "%s: a device segment list needs a count and expert_slot_dev", fn);
+    } else {
+      for (int i = 0; i < segs->n; ++i)
+        SP_REQUIRE(segs->eids[i] >= 0 && segs->eids[i] < E && segs->slots[i] >= 0, "%s: segment %d names expert %d in slot %d", fn, i,
+                   static_cast<int>(segs->eids[i]), static_cast<int>(segs->slots[i]));
+    }
+  }
+  int Is = 0;
+  if (shared) {
+    SP_REQUIRE(shared_gate_w && shared_up_w && shared_dev, "%s: NULL shared-expert pointer", fn);
+    Is = shared_down_w->cols;
+    SP_REQUIRE(Is > 0 && Is % 64 == 0 && Is <= kF8MaxDim, "%s: Is=%d must be a positive multiple of 64", fn, Is);
+    int rc = check_matrix(fn, "shared gate_proj", shared_gate_w, Is, H);
+    if (rc == SPARSE_HIP_OK) rc = check_matrix(fn, "shared up_proj", shared_up_w, Is, H);
+    if (rc == SPARSE_HIP_OK) rc = check_matrix(fn, "shared down_proj", shared_down_w, H, Is);
+    if (rc != SPARSE_HIP_OK) return rc;
+    SP_REQUIRE(aligned16(shared_dev), "%s: shared output must be 16-byte aligned", fn);
+  }
+  if (!routed && !shared) return SPARSE_HIP_OK;
+  SP_REQUIRE(ws_dev != nullptr && aligned16(ws_dev), "%s: workspace is NULL or not 16-byte aligned", fn);
+  hipStream_t st = as_stream(stream);
+  const FfnWs w = ffn_ws(ws_dev, T, K, segs->n, H, I, Is);
+
+  int rc = f8_quantize(x_dev, dtype, T, H, w.x.values, w.x.scales, st);
+  if (rc != SPARSE_HIP_OK) return rc;
+  F8Product p = {};
+  p.slab = static_cast<const uint8_t*>(experts->slab_dev);
+  p.slot_stride = experts->slot_stride;
+  p.expert_slot = experts->expert_slot_dev;
+  p.perm = perm_dev;
+  p.seg_offsets = seg_offsets_dev;
+  p.topv = topv_dev;
+  p.topk = K;
+  p.T = T;
+  p.dtype = dtype;
+  p.segs = *segs;
+  // gate and up: x -> h
+  p.off0 = 0;
+  p.off1 = slot.up;
+  p.soff0 = slot.sgate;
+  p.soff1 = slot.sup;
+  p.act_r = p.act_s = w.x.values;
+  p.act_rs = p.act_ss = w.x.scales;
+  p.gather = 1;
+  p.out_r = w.hf;
+  p.Kr = H;
+  p.Nr = I;
+  if (shared) {
+    p.w0 = static_cast<const uint8_t*>(shared_gate_w->values_dev);
+    p.w1 = static_cast<const uint8_t*>(shared_up_w->values_dev);
+    p.s0 = shared_gate_w->scales_dev;
+    p.s1 = shared_up_w->scales_dev;
+    p.out_s = w.shf;
+    p.Ks = H;
+    p.Ns = Is;
+  }
+  rc = f8_stream(p, true, routed, shared, st);
+  if (rc == SPARSE_HIP_OK && routed) rc = f8_quantize(w.hf, SPARSE_HIP_F32, static_cast<int64_t>(T) * K, I, w.h.values, w.h.scales, st);
+  if (rc == SPARSE_HIP_OK && shared) rc = f8_quantize(w.shf, SPARSE_HIP_F32, T, Is, w.sh.values, w.sh.scales, st);
+  if (rc != SPARSE_HIP_OK) return rc;
+  // down: h -> rows times their route weight (shared expert: times sigmoid of its gate)
+  p.off0 = p.off1 = slot.down;
+  p.soff0 = p.soff1 = slot.sdown;
+  p.act_r = w.h.values;
+  p.act_rs = w.h.scales;
+  p.gather = 0;
+  p.out_r = parts_dev;
+  p.Kr = I;
+  p.Nr = H;
+  if (shared) {
+    p.w0 = p.w1 = static_cast<const uint8_t*>(shared_down_w->values_dev);
+    p.s0 = p.s1 = shared_down_w->scales_dev;
+    p.act_s = w.sh.values;
+    p.act_ss = w.sh.scales;
+    p.gate_s = shared_gate_dev;
+    p.out_s = shared_dev;
+    p.Ks = Is;
+    p.Ns = H;
+  }
+  return f8_stream(p, false, routed, shared, st);
+}
+
+}  // extern "C"

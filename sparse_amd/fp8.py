@@ -1,0 +1,319 @@
+"""Block-scaled 8-bit floating point: quantised rows, weights, expert slabs and the products on them.
+
+Values are ``torch.float8_e4m3fn``.  Rows (activations) carry one power-of-two scale for each run of 128
+values (``torch.float8_e8m0fnu``), weights one fp32 scale for each 128 x 128 block, as 8-bit checkpoints
+store them: ``weight ~ values * scale``.  Inference only: nothing here has a backward.
+
+    w = Weight.from_quantized(values, scales)      # once, at load time; Weight.quantize(w16) otherwise
+    y = linear(x, w)                               # x is quantised inside the call
+    rows = quantize(x); y = linear(rows, w)        # ... or once for several products
+
+    slab = ExpertSlab.from_quantized(experts)      # or ExpertSlab.quantize(expert_weights16)
+    parts, shared = moe_ffn(slab, x, topv, perm, shared=(gate, up, down), shared_gate=logits)
+    ops.combine(parts, perm, shared, T, K, out)
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib, ops
+from ._lib import Fp8Matrix, SegList
+from .ops import HALF_DTYPES, Permutation, _need, _need_half, _ptr, dtype_code, on_device
+
+BLOCK = 128
+E4M3 = torch.float8_e4m3fn
+E8M0 = torch.float8_e8m0fnu
+TOP = 448.0
+
+
+def blocks(n: int) -> int:
+    return -(-int(n) // BLOCK)
+
+
+def padded(n: int) -> int:
+    return blocks(n) * BLOCK
+
+
+# ------------------------------------------------------------------------------- rows
+class Rows:
+    """Quantised rows: ``data [T, padded(K)]`` (zeros behind column K) and ``scales [T, blocks(K)]``."""
+
+    __slots__ = ("data", "scales", "cols", "dtype")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, cols: int, dtype: torch.dtype) -> None:
+        self.data, self.scales, self.cols, self.dtype = data, scales, int(cols), dtype
+
+    @property
+    def values(self) -> torch.Tensor:
+        """The ``[T, K]`` values without the padding."""
+        return self.data[:, :self.cols]
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        full = self.data.float().view(*self.scales.shape, BLOCK) * self.scales.float()[..., None]
+        return full.reshape(self.data.shape)[:, :self.cols].to(dtype)
+
+
+def quantize(x: torch.Tensor, out: Optional[Rows] = None) -> Rows:
+    """Rows ``x [T, K]`` (bf16, fp16 or fp32) to 8 bits.  The scale of a run of 128 is the smallest
+    ``2**s``, ``s >= -120``, with ``max|x| <= 448 * 2**s``; infinities and NaN become NaN and leave the rest
+    of their run as it is."""
+    _need(x, "x")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be [T, K] with K >= 1, got {tuple(x.shape)}")
+    T, K = x.shape
+    code = dtype_code(x.dtype)
+    if out is None:
+        out = Rows(x.new_empty((T, padded(K)), dtype=E4M3), x.new_empty((T, blocks(K)), dtype=E8M0), K, x.dtype)
+    else:
+        _need(out.data, "values", E4M3, (T, padded(K)))
+        _need(out.scales, "scales", E8M0, (T, blocks(K)))
+        out.cols, out.dtype = K, x.dtype
+    with on_device(x, out.data, out.scales) as stream:
+        rc = _lib.load().sparse_hip_fp8_quantize(_ptr(x), code, T, K, _ptr(out.data), _ptr(out.scales), stream)
+    _lib.check(rc, "sparse_hip_fp8_quantize")
+    return out
+
+
+# ----------------------------------------------------------------------------- weights
+def tile_values(q: torch.Tensor) -> torch.Tensor:
+    """8-bit values ``[N, K]`` in the kernels' order, flattened, zeros up to 16 rows and 128 columns:
+    byte (row, k) goes to ``(row//16)*16*Kp + (k//128)*2048 + ((k//16)%2)*1024 + ((k//32)%4)*256 +
+    (row%16)*16 + k%16``."""
+    N, K = q.shape
+    Np, Kp = -(-N // 16) * 16, padded(K)
+    b = q.view(torch.uint8)
+    if (Np, Kp) != (N, K):
+        full = b.new_zeros((Np, Kp))
+        full[:N, :K] = b
+        b = full
+    v = b.reshape(Np // 16, 16, Kp // 128, 4, 2, 16)       # [group, row, block, quarter, half, k16]
+    return v.permute(0, 2, 4, 3, 1, 5).reshape(-1)          # [group, block, half, quarter, row, k16]
+
+
+def untile_values(flat: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
+    """Inverse of ``tile_values``."""
+    Np, Kp = -(-rows // 16) * 16, padded(cols)
+    v = flat.view(torch.uint8).reshape(Np // 16, Kp // 128, 2, 4, 16, 16)
+    return v.permute(0, 4, 1, 3, 2, 5).reshape(Np, Kp)[:rows, :cols].contiguous().view(E4M3)
+
+
+def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(values [N, K] float8_e4m3fn, scales [blocks(N), blocks(K)] fp32)`` of a weight: the scale of a
+    128 x 128 block is the smallest power of two ``2**s``, ``s >= -120``, with ``max|w| <= 448 * 2**s`` (the
+    division is then exact and each value is rounded once).  Done once, at load time."""
+    if w.dim() != 2:
+        raise ValueError(f"a weight must be [N, K], got {tuple(w.shape)}")
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("a weight must be finite to be quantised")
+    N, K = w.shape
+    full = torch.zeros((padded(N), padded(K)), dtype=torch.float32, device=w.device)
+    full[:N, :K] = w
+    v = full.view(blocks(N), BLOCK, blocks(K), BLOCK)
+    m, e = torch.frexp(v.abs().amax(dim=(1, 3)))
+    s = torch.where(m <= 0.875, e - 9, e - 8)               # 448 = 0.875 * 2**9
+    s = torch.where(m == 0, torch.full_like(s, -120), s).clamp_min(-120)
+    q = torch.ldexp(v, -s[:, None, :, None]).reshape(full.shape)[:N, :K].to(E4M3).contiguous()
+    return q, torch.ldexp(torch.ones_like(m), s)
+
+
+def _check_quantized(values: torch.Tensor, scales: torch.Tensor, name: str = "weight") -> None:
+    if values.dim() != 2 or values.dtype != E4M3 or values.numel() == 0:
+        raise ValueError(f"{name} values must be [N, K] {E4M3}, got {tuple(values.shape)} {values.dtype}")
+    want = (blocks(values.shape[0]), blocks(values.shape[1]))
+    if tuple(scales.shape) != want or scales.dtype != torch.float32:
+        raise ValueError(f"{name} scales must be {want} float32, got {tuple(scales.shape)} {scales.dtype}")
+    if values.device != scales.device:
+        raise ValueError(f"{name} values and scales are on different devices")
+
+
+class Weight:
+    """A matrix ``[rows, cols]`` laid out for the kernels, with its block scales."""
+
+    __slots__ = ("data", "scales", "rows", "cols", "desc")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> None:
+        self.data, self.scales, self.rows, self.cols = data, scales, int(rows), int(cols)
+        self.desc = Fp8Matrix(data.data_ptr(), scales.data_ptr(), self.rows, self.cols)
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.rows, self.cols
+
+    @classmethod
+    def from_quantized(cls, values: torch.Tensor, scales: torch.Tensor) -> "Weight":
+        """From a checkpoint's 8-bit values ``[N, K]`` and fp32 scales ``[blocks(N), blocks(K)]``."""
+        _check_quantized(values, scales)
+        return cls(tile_values(values.contiguous()).contiguous(), scales.contiguous().clone(), *values.shape)
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor) -> "Weight":
+        return cls.from_quantized(*quantize_weight(w))
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        wide = torch.float64 if dtype == torch.float64 else torch.float32
+        q = untile_values(self.data, self.rows, self.cols).to(wide)
+        s = self.scales.to(wide).repeat_interleave(BLOCK, 0)[:self.rows].repeat_interleave(BLOCK, 1)[:, :self.cols]
+        return (q * s).to(dtype)
+
+
+def linear(x: Union[torch.Tensor, Rows], weight: Weight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x W^T`` with ``x [T, K]`` (bf16 or fp16) quantised inside the call, or given as ``Rows`` of such an x:
+    ``[T, N]`` in x's dtype, accumulated in fp32 and rounded once."""
+    rows = x if isinstance(x, Rows) else None
+    src = x.data if rows is not None else x
+    _need(src, "x")
+    if x.dtype not in HALF_DTYPES:
+        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
+    if src.dim() != 2:
+        raise ValueError(f"x must be [T, K], got {tuple(src.shape)}")
+    T, K = src.shape[0], (rows.cols if rows is not None else src.shape[1])
+    if K != weight.cols:
+        raise ValueError(f"x has {K} columns, the weight {weight.cols}")
+    dtype = x.dtype
+    code = dtype_code(dtype)
+    if out is None:
+        out = src.new_empty((T, weight.rows), dtype=dtype)
+    else:
+        _need(out, "out", dtype, (T, weight.rows))
+    lib = _lib.load()
+    with on_device(src, weight.data, out) as stream:
+        if rows is not None:
+            _need(rows.data, "values", E4M3, (T, padded(K)))
+            _need(rows.scales, "scales", E8M0, (T, blocks(K)))
+            rc = lib.sparse_hip_fp8_linear(None, _ptr(rows.data), _ptr(rows.scales), code, T, C.byref(weight.desc),
+                                           _ptr(out), None, stream)
+        else:
+            ws = src.new_empty((max(1, lib.sparse_hip_fp8_linear_ws_bytes(T, K)),), dtype=torch.uint8)
+            rc = lib.sparse_hip_fp8_linear(_ptr(src), None, None, code, T, C.byref(weight.desc), _ptr(out), _ptr(ws), stream)
+    _lib.check(rc, "sparse_hip_fp8_linear")
+    return out
+
+
+# ----------------------------------------------------------------------------- experts
+Quantized = Tuple[torch.Tensor, torch.Tensor]
+
+
+def slot_bytes(hidden: int, inter: int) -> int:
+    """Bytes of one expert: gate, up and down values, then their scales, rounded up to 256."""
+    return int(_lib.load().sparse_hip_fp8_slot_bytes(int(hidden), int(inter)))
+
+
+def pack_expert_into(dst: torch.Tensor, expert: Tuple[Quantized, Quantized, Quantized], hidden: int, inter: int) -> None:
+    """Lay one expert's (gate, up, down) (values, scales) pairs into one slot of bytes."""
+    at = 0
+    for (q, s), shape, name in zip(expert, ((inter, hidden), (inter, hidden), (hidden, inter)), ("gate", "up", "down")):
+        _check_quantized(q, s, name)
+        if tuple(q.shape) != shape:
+            raise ValueError(f"{name} must be {shape}, got {tuple(q.shape)}")
+        t = tile_values(q.contiguous())
+        dst[at:at + t.numel()].copy_(t)
+        at += t.numel()
+    for _, s in expert:
+        b = s.contiguous().view(torch.uint8).reshape(-1)
+        dst[at:at + b.numel()].copy_(b)
+        at += b.numel()
+    dst[at:].zero_()
+
+
+class ExpertSlab:
+    """8-bit experts of one layer in HBM, one slot each, and the device-side expert -> slot table."""
+
+    def __init__(self, num_slots: int, num_experts: int, hidden: int, inter: int, device) -> None:
+        if hidden % 64 or inter % 64 or hidden <= 0 or inter <= 0:
+            raise ValueError(f"hidden and inter must be positive multiples of 64, got {hidden}, {inter}")
+        self.hidden, self.inter = int(hidden), int(inter)
+        self.num_slots, self.num_experts = int(num_slots), int(num_experts)
+        self.expert_bytes = slot_bytes(hidden, inter)
+        self.data = torch.empty((self.num_slots, self.expert_bytes), dtype=torch.uint8, device=device)
+        self.expert_slot = torch.arange(self.num_experts, dtype=torch.int32, device=device)
+
+    @classmethod
+    def from_quantized(cls, experts: Sequence[Tuple[Quantized, Quantized, Quantized]], device=None) -> "ExpertSlab":
+        """All experts resident, slot == expert id; ``experts[e]`` is (gate, up, down), each (values, scales)."""
+        gate = experts[0][0][0]
+        slab = cls(len(experts), len(experts), gate.shape[1], gate.shape[0], device if device is not None else gate.device)
+        for e, expert in enumerate(experts):
+            pack_expert_into(slab.data[e], expert, slab.hidden, slab.inter)
+        return slab
+
+    @classmethod
+    def quantize(cls, experts: Sequence[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]], device=None) -> "ExpertSlab":
+        """The same from 16- or 32-bit (gate, up, down) weights."""
+        return cls.from_quantized([tuple(quantize_weight(w) for w in triple) for triple in experts], device)
+
+    def slot_ptr(self, slot: int) -> int:
+        return self.data.data_ptr() + int(slot) * self.expert_bytes
+
+    def descriptor(self, dtype: torch.dtype) -> _lib.Experts:
+        return _lib.Experts(self.data.data_ptr(), self.expert_bytes, self.expert_slot.data_ptr(), self.num_experts,
+                            self.hidden, self.inter, dtype_code(dtype))
+
+
+def moe_ffn_ws_bytes(T: int, K: int, num_segments: int, hidden: int, inter: int, shared_inter: int = 0) -> int:
+    return int(_lib.load().sparse_hip_fp8_moe_ffn_ws_bytes(int(T), int(K), int(num_segments), int(hidden), int(inter),
+                                                           int(shared_inter)))
+
+
+def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Permutation,
+            shared: Optional[Tuple[Weight, Weight, Weight]] = None, shared_gate: Optional[torch.Tensor] = None,
+            segs: Optional[SegList] = None, parts: Optional[torch.Tensor] = None,
+            shared_out: Optional[torch.Tensor] = None, ws: Optional[torch.Tensor] = None
+            ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Routed experts (over ``segs``, by default every active one) and the shared expert of one call of any
+    size on 8-bit weights: returns ``(parts [T*K, H]`` in permuted order, each row times its route weight,
+    ``shared [T, H]`` or None``)`` for ``ops.combine``.  ``x [T, H]`` bf16 or fp16, ``topv [T, K]`` of the same
+    dtype; ``shared_gate [T]``: logits whose sigmoid multiplies the shared rows.  ``ws``: a byte tensor of
+    ``moe_ffn_ws_bytes`` for callers that keep one."""
+    _need_half(x, "x")
+    if x.dim() != 2 or topv.dim() != 2:
+        raise ValueError("x must be [T, H] and topv [T, K]")
+    T, H = x.shape
+    K = topv.shape[1]
+    dtype = x.dtype
+    if H != experts.hidden:
+        raise ValueError(f"x has hidden {H}, the expert slab has {experts.hidden}")
+    _need(topv, "topv", dtype, (T, K))
+    if perm.perm.numel() != T * K or perm.seg_offsets.numel() != experts.num_experts + 1:
+        raise ValueError(f"the permutation does not belong to {T} tokens x {K} over {experts.num_experts} experts")
+    if segs is None:
+        segs = ops.seglist_device(perm, min(experts.num_experts, T * K))
+    if parts is None:
+        parts = x.new_empty((T * K, H))
+    else:
+        _need(parts, "parts", dtype, (T * K, H))
+    mats, Is = (None, None, None), 0
+    if shared is not None:
+        Is = shared[2].cols
+        for m, want, name in zip(shared, ((Is, H), (Is, H), (H, Is)), ("gate_proj", "up_proj", "down_proj")):
+            if m.shape != want:
+                raise ValueError(f"shared {name} must be {want}, got {m.shape}")
+        mats = tuple(C.byref(m.desc) for m in shared)
+        if shared_gate is not None:
+            _need(shared_gate, "shared gate logits", dtype)
+            if shared_gate.numel() != T:
+                raise ValueError("shared gate logits must hold T elements")
+        if shared_out is None:
+            shared_out = x.new_empty((T, H))
+        else:
+            _need(shared_out, "shared out", dtype, (T, H))
+    else:
+        shared_gate = shared_out = None
+    lib = _lib.load()
+    need = lib.sparse_hip_fp8_moe_ffn_ws_bytes(T, K, segs.n, H, experts.inter, Is)
+    with on_device(x, topv, perm.perm, experts.data, parts, shared_gate, shared_out, ws,
+                   None if shared is None else shared[0].data) as stream:
+        if ws is None:
+            ws = x.new_empty((max(1, need),), dtype=torch.uint8)
+        elif not ws.is_contiguous() or ws.numel() * ws.element_size() < need:
+            raise ValueError(f"the workspace must hold {need} contiguous bytes")
+        if T == 0:
+            return parts, shared_out
+        desc = experts.descriptor(dtype)
+        rc = lib.sparse_hip_fp8_moe_ffn(C.byref(desc), _ptr(x), _ptr(topv), _ptr(perm.perm), _ptr(perm.seg_offsets),
+                                        C.byref(segs), T, K, _ptr(parts), *mats, _ptr(shared_gate), _ptr(shared_out),
+                                        _ptr(ws), stream)
+    _lib.check(rc, "sparse_hip_fp8_moe_ffn")
+    return parts, shared_out

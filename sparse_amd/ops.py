@@ -55,6 +55,29 @@ def _need(t: torch.Tensor, name: str, dtype=None, shape=None) -> None:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
+class on_device:
+    """``with on_device(*tensors) as stream``: the tensors' device is the current one inside, ``stream`` is
+    its current stream.  Tensors on different devices are refused."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, *tensors: Optional[torch.Tensor]) -> None:
+        self.index = self.previous = tensors[0].get_device()
+        for t in tensors:
+            if t is not None and t.get_device() != self.index:
+                raise ValueError(f"tensors are on different devices: cuda:{self.index} and {t.device}")
+
+    def __enter__(self) -> int:
+        self.previous = torch.cuda.current_device()
+        if self.previous != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        if self.previous != self.index:
+            torch.cuda.set_device(self.previous)
+
+
 # --------------------------------------------------------------------------- router
 def router_logits(x: torch.Tensor, wg: torch.Tensor, wsg: Optional[torch.Tensor] = None,
                   logits_dtype: Optional[torch.dtype] = None,
@@ -107,6 +130,49 @@ def gate_topk(logits: torch.Tensor, k: int, renorm: bool = False, out_dtype: Opt
                                          int(n_group), int(topk_group), float(scale), dtype_code(odt), _ptr(topv),
                                          _ptr(topi), _ptr(pseudo_logits), _stream())
     _lib.check(rc, "sparse_hip_gate_topk_scaled")
+    return topv, topi
+
+
+SELECT_SCORE = {"softmax": 0, "sigmoid": 1}
+SELECT_GROUP = {"max": 0, "top2": 1}
+
+
+def gate_select(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optional[torch.Tensor] = None,
+                n_group: int = 1, topk_group: int = 1, group_score: str = "max", renorm: bool = False,
+                scale: float = 1.0, out_dtype: Optional[torch.dtype] = None, topv: Optional[torch.Tensor] = None,
+                topi: Optional[torch.Tensor] = None):
+    """Expert selection of a gate balanced by a bias: returns ``(topv [T,k] out_dtype, topi [T,k] int64)``.
+    Scores are the ``softmax`` or the ``sigmoid`` of ``logits [T,E]``; ``bias [E]`` fp32 is added for the
+    ranking only.  With ``topk_group < n_group`` only experts of the ``topk_group`` best groups can be
+    chosen, a group scoring its largest ranked value (``max``) or the sum of its two largest (``top2``).
+    The weights are the chosen experts' scores, divided by their sum with ``renorm``, times ``scale``.
+    Ranking is done in 64 bits, ties go to the lower id."""
+    _need(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [T, E], got {tuple(logits.shape)}")
+    if score not in SELECT_SCORE:
+        raise ValueError(f"score must be softmax|sigmoid, got {score}")
+    if group_score not in SELECT_GROUP:
+        raise ValueError(f"group_score must be max|top2, got {group_score}")
+    T, E = logits.shape
+    k = int(k)
+    odt = out_dtype or logits.dtype
+    if bias is not None:
+        _need(bias, "bias", torch.float32, (E,))
+    ldt, ocode = dtype_code(logits.dtype), dtype_code(odt)
+    if topv is None:
+        topv = logits.new_empty((T, max(0, k)), dtype=odt)
+    else:
+        _need(topv, "topv", odt, (T, k))
+    if topi is None:
+        topi = logits.new_empty((T, max(0, k)), dtype=torch.int64)
+    else:
+        _need(topi, "topi", torch.int64, (T, k))
+    with on_device(logits, bias, topv, topi) as stream:
+        rc = _lib.load().sparse_hip_gate_select(_ptr(logits), ldt, _ptr(bias), T, E, k, SELECT_SCORE[score], int(n_group),
+                                                int(topk_group), SELECT_GROUP[group_score], int(bool(renorm)), float(scale),
+                                                ocode, _ptr(topv), _ptr(topi), stream)
+    _lib.check(rc, "sparse_hip_gate_select")
     return topv, topi
 
 
