@@ -34,6 +34,7 @@ SOURCES = [
     "fp8.hip",
     "fp8_quantize.hip",
     "fp8_stream.hip",
+    "fp8_tile.hip",
     "rs_predict.hip",
     "layout.hip",
     "mfma_probe.hip",
@@ -55,7 +56,8 @@ HIP_FLAGS = [
 # spill adds scratch loads and stores to that count, so a build in which one of these kernels
 # uses scratch memory is refused.
 NO_SCRATCH = {"swiglu_prefill.hip": ("prefill_ffn_kernel",),
-              "swiglu_prefill_merged.hip": ("prefill_merged_kernel",)}
+              "swiglu_prefill_merged.hip": ("prefill_merged_kernel",),
+              "fp8_tile.hip": ("f8_tile_kernel",)}
 RESOURCE_REMARKS = "-Rpass-analysis=kernel-resource-usage"
 
 

@@ -109,4 +109,14 @@ struct F8Product {
 // gate/up (SwiGLU of two products, fp32 out) or a single product, any number of rows
 int f8_stream(const F8Product& p, bool gateup, bool routed, bool dense, hipStream_t st);
 
+// The same for many rows, 16-bit formats: 128 x 256 tiles.  gate/up writes quantised rows; routed and dense
+// tiles come from one set of queues (prefill_queues, which builds them).
+struct PfQueues;
+int prefill_queues(const int32_t* expert_slot, const int32_t* seg_offsets, const sparse_hip_seglist* segs, int T, int K,
+                   int H, int I, int Is, void* tile_ws, PfQueues* q, hipStream_t st);
+size_t prefill_merged_ws_bytes(int T, int K, int nseg, int H, int I, int Is);
+int f8_tile_gateup(const F8Product& p, const PfQueues& q, void* h, void* hs, void* sh, void* shs, hipStream_t st);
+int f8_tile_down(const F8Product& p, const PfQueues& q, hipStream_t st);
+int f8_tile_linear(const F8Product& p, hipStream_t st);
+
 }  // namespace sparse

@@ -1,13 +1,14 @@
 // C ABI of the block-scaled 8-bit operators: argument checks and the order of launches.
 #include "fp8.h"
+#include "prefill_tiles.h"
 
 namespace sparse {
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static inline size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
-constexpr int kF8MaxDim = 1 << 20;
-constexpr int64_t kF8MaxRows = 1ll << 30;
+constexpr int kF8MaxDim = 1 << 16;      // the tile kernel keeps a scale byte per row and block in LDS
+constexpr int64_t kF8MaxRows = 1ll << 28;   // flat rows: the division by topk is a 32-bit multiply
 
 // A workspace handed out front to back in 256-byte steps; with a null base it only counts.
 struct Carve {
@@ -44,7 +45,8 @@ static LinearWs linear_ws(void* ws, int T, int K) {
 
 struct FfnWs {
   F8Rows x, h, sh;
-  float *hf, *shf;
+  float *hf, *shf;    // few rows: the intermediate before it is quantised
+  void* tiles;        // many rows: the tile queues
   size_t bytes;
 };
 static FfnWs ffn_ws(void* ws, int T, int K, int nseg, int H, int I, int Is) {
@@ -52,11 +54,13 @@ static FfnWs ffn_ws(void* ws, int T, int K, int nseg, int H, int I, int Is) {
   FfnWs w = {};
   const int64_t rows = nseg > 0 ? static_cast<int64_t>(T) * K : 0;
   w.x = take_rows(c, T, H);
-  w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
   w.h = take_rows(c, rows, I);
-  if (Is > 0) {
-    w.shf = static_cast<float*>(c.take(static_cast<size_t>(T) * Is * sizeof(float)));
-    w.sh = take_rows(c, T, Is);
+  if (Is > 0) w.sh = take_rows(c, T, Is);
+  if (T > SPARSE_HIP_DECODE_MAX_TOKENS) {
+    w.tiles = c.take(prefill_merged_ws_bytes(T, K, nseg, H, I, Is));
+  } else {
+    w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
+    if (Is > 0) w.shf = static_cast<float*>(c.take(static_cast<size_t>(T) * Is * sizeof(float)));
   }
   w.bytes = c.used;
   return w;
@@ -124,6 +128,7 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   p.Ns = weight->rows;
   p.T = T;
   p.dtype = dtype;
+  if (T > SPARSE_HIP_DECODE_MAX_TOKENS) return f8_tile_linear(p, st);
   return f8_stream(p, false, false, true, st);
 }
 
@@ -151,6 +156,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   SP_REQUIRE(I > 0 && I % 64 == 0 && I <= kF8MaxDim, "%s: I=%d must be a positive multiple of 64", fn, I);
   SP_REQUIRE(T >= 1 && K >= 1 && K <= SPARSE_HIP_MAX_TOPK, "%s: T=%d, K=%d outside [1,..] x [1,%d]", fn, T, K, SPARSE_HIP_MAX_TOPK);
   SP_REQUIRE(static_cast<int64_t>(T) * K < kF8MaxRows, "%s: T=%d, K=%d: too many rows", fn, T, K);
+  SP_REQUIRE(static_cast<uint64_t>(T) * f8_padded(H) < (1ull << 32), "%s: T=%d rows of %d: too large for 32-bit offsets", fn, T, H);
   SP_REQUIRE(segs->n >= 0 && segs->n <= SPARSE_HIP_MAX_EXPERTS, "%s: segment count %d outside [0,%d]", fn, segs->n, SPARSE_HIP_MAX_EXPERTS);
   const F8Slot slot = f8_slot(H, I);
   const bool routed = segs->n > 0, shared = shared_down_w != nullptr;
@@ -185,8 +191,14 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   hipStream_t st = as_stream(stream);
   const FfnWs w = ffn_ws(ws_dev, T, K, segs->n, H, I, Is);
 
+  const bool tiles = T > SPARSE_HIP_DECODE_MAX_TOKENS;
   int rc = f8_quantize(x_dev, dtype, T, H, w.x.values, w.x.scales, st);
   if (rc != SPARSE_HIP_OK) return rc;
+  PfQueues queues = {};
+  if (tiles) {
+    rc = prefill_queues(experts->expert_slot_dev, seg_offsets_dev, segs, T, K, H, I, Is, w.tiles, &queues, st);
+    if (rc != SPARSE_HIP_OK) return rc;
+  }
   F8Product p = {};
   p.slab = static_cast<const uint8_t*>(experts->slab_dev);
   p.slot_stride = experts->slot_stride;
@@ -218,9 +230,12 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
     p.Ks = H;
     p.Ns = Is;
   }
-  rc = f8_stream(p, true, routed, shared, st);
-  if (rc == SPARSE_HIP_OK && routed) rc = f8_quantize(w.hf, SPARSE_HIP_F32, static_cast<int64_t>(T) * K, I, w.h.values, w.h.scales, st);
-  if (rc == SPARSE_HIP_OK && shared) rc = f8_quantize(w.shf, SPARSE_HIP_F32, T, Is, w.sh.values, w.sh.scales, st);
+  if (tiles)
+    rc = f8_tile_gateup(p, queues, w.h.values, w.h.scales, w.sh.values, w.sh.scales, st);
+  else
+    rc = f8_stream(p, true, routed, shared, st);
+  if (!tiles && rc == SPARSE_HIP_OK && routed) rc = f8_quantize(w.hf, SPARSE_HIP_F32, static_cast<int64_t>(T) * K, I, w.h.values, w.h.scales, st);
+  if (!tiles && rc == SPARSE_HIP_OK && shared) rc = f8_quantize(w.shf, SPARSE_HIP_F32, T, Is, w.sh.values, w.sh.scales, st);
   if (rc != SPARSE_HIP_OK) return rc;
   // down: h -> rows times their route weight (shared expert: times sigmoid of its gate)
   p.off0 = p.off1 = slot.down;
@@ -241,7 +256,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
     p.Ks = Is;
     p.Ns = H;
   }
-  return f8_stream(p, false, routed, shared, st);
+  return tiles ? f8_tile_down(p, queues, st) : f8_stream(p, false, routed, shared, st);
 }
 
 }  // extern "C"

@@ -1,0 +1,432 @@
+// Block-scaled 8-bit matrix products of many rows: the tile kernel.
+//
+// A workgroup of four wavefronts computes 128 rows x 256 weight rows (gate/up: 128 gate rows and the 128 up
+// rows of the same neurons) over 128-wide k slabs.  An 8-bit slab row is 128 bytes, as a 64-wide slab row of
+// the 16-bit kernels is, so the movement of data is theirs: activation rows, gathered through the
+// permutation, go to a three-buffer LDS ring by direct global -> LDS copies with 16-byte chunks swizzled by
+// row; weight fragments come straight from the tiled layout into two alternating register sets; everything
+// is requested two slabs ahead and vector memory is awaited by count.  A slab is one 16x16x128 matrix
+// instruction per 16 x 16 tile where the 16-bit kernels have two of half the rate: the same bytes feed
+// twice the arithmetic.
+//
+// Scales: the activations' E8M0 bytes of the whole tile are laid out in LDS once, the eight bytes that a
+// lane's eight row tiles need for a slab side by side, and enter the instruction as its own operand.  The
+// weights' fp32 scales multiply the slab's sum on its way into the accumulator.
+#include <type_traits>
+
+#include "fp8.h"
+#include "prefill_tiles.h"
+
+namespace sparse {
+
+constexpr int kTlRowBytes = kF8Block;               // LDS row of one k slab
+constexpr int kTlSlab = kPfBM * kTlRowBytes;
+constexpr int kTlScaleBytes = kPfBM + 2 * sizeof(float);   // per slab: activation bytes, two weight scales
+static_assert(kTlSlab == kPfLdsA, "the slab geometry is that of the 16-bit kernels");
+
+template <typename T>
+__device__ __forceinline__ T* uniform_ptr(T* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<T*>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+
+struct TileArgs {
+  F8Product p;
+  const PfTile* map;       // NULL: dense operands only, the tile comes from the block number
+  const int32_t* qhdr;
+  uint32_t topk_magic;     // ceil(2^32 / topk); 0 for topk == 1
+  int32_t mt, nt;          // row and column tiles when map is NULL
+  // gate/up: where the quantised rows go
+  uint8_t *q_r, *qs_r, *q_s, *qs_s;
+};
+
+// F: the 16-bit format of outputs, route weights and gate logits
+template <typename F, bool kGateUp>
+__global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kPfStages][kTlSlab];
+  __shared__ float s_row[kPfBM];          // factor of a row (down), exponent of a row's scale (gate/up)
+  __shared__ float s_amax[kGateUp ? 4 : 1][kPfBM];
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_scales[];   // [nk][128] bytes, then [nk][2] floats
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int fr = lane & 15, fq = lane >> 4;
+  constexpr int kWaitVm0 = kWaitVmcnt0, kWaitVm20 = kWaitVmcnt20;
+  const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) uint8_t*)(&lds[0][0])));
+
+  // ---- which tile (wavefront-uniform) ------------------------------------------------
+  int slot, r0, M, bn;
+  if (a.map != nullptr) {
+    const int xcd = blockIdx.x % kPfXcds, rank = blockIdx.x / kPfXcds;
+    if (rank >= a.qhdr[kPfXcds + xcd]) return;   // the grid is sized for the longest possible queue
+    const PfTile tile = a.map[a.qhdr[xcd] + rank];
+    slot = __builtin_amdgcn_readfirstlane(tile.slot);
+    r0 = __builtin_amdgcn_readfirstlane(tile.r0);
+    M = __builtin_amdgcn_readfirstlane(tile.rows);
+    bn = __builtin_amdgcn_readfirstlane(tile.bn);
+  } else {
+    // block b runs on XCD b % 8; an XCD takes a contiguous share of the (column tile, row tile) order
+    const int total = a.mt * a.nt, xcd = blockIdx.x % kPfXcds, rank = blockIdx.x / kPfXcds;
+    const int first = static_cast<int>(static_cast<int64_t>(total) * xcd / kPfXcds);
+    const int end = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / kPfXcds);
+    if (first + rank >= end) return;
+    bn = (first + rank) / a.mt;
+    r0 = (first + rank - bn * a.mt) * kPfBM;
+    M = min(kPfBM, a.p.T - r0);
+    slot = -1;
+  }
+  if (M <= 0) return;
+  const bool dense = slot < 0;
+  const int Kdim = dense ? a.p.Ks : a.p.Kr, N = dense ? a.p.Ns : a.p.Nr;
+  const int nk = (Kdim + kF8Block - 1) / kF8Block;
+  const uint32_t ld = static_cast<uint32_t>(nk) * kF8Block;
+  const int n0 = bn * (kGateUp ? kPfBR / 2 : kPfBR);   // first output column of this tile
+
+  // ---- operand addresses ------------------------------------------------------------
+  // Row r keeps chunk 2q + h at position (q + 4h) ^ f(r), f(r) = ((r >> 1) & 7) ^ ((r & 1) << 2); with
+  // r = 32 wave + 8 it + (lane >> 3), f depends on `it` through its low bit only, which flips bit 0 of the chunk.
+  const int l3 = lane >> 3;
+  const int pos0 = (lane & 7) ^ ((l3 >> 1) ^ ((l3 & 1) << 2));
+  const uint32_t chunk0 = ((pos0 & 3) << 1) | (pos0 >> 2);
+  const bool gather = !dense && a.p.gather != 0;
+  // rows that are not gathered are addressed from the tile's first one, so that 32-bit offsets always reach
+  const size_t row_base = gather ? 0 : static_cast<size_t>(r0);
+  const uint8_t* abase = uniform_ptr((dense ? a.p.act_s : a.p.act_r) + row_base * ld);
+  const uint8_t* sbase = (dense ? a.p.act_ss : a.p.act_rs) + row_base * nk;
+  auto source_row = [&](int m) -> uint32_t {
+    const int mm = min(m, M - 1);
+    if (!gather) return static_cast<uint32_t>(mm);
+    uint32_t g = static_cast<uint32_t>(a.p.perm[r0 + mm]);
+    return a.topk_magic != 0 ? __umulhi(g, a.topk_magic) : g;
+  };
+  uint32_t doff[4];   // byte offset of lane's piece of copy `it` inside k slab 0
+#pragma unroll
+  for (int it = 0; it < 4; ++it)
+    doff[it] = source_row(wave * 32 + it * 8 + l3) * ld + ((chunk0 ^ (it & 1)) << 4);
+  auto stage_slab = [&](int slab, int buf) {
+    const uint8_t* sb = abase + static_cast<size_t>(slab) * kF8Block;
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + buf * kTlSlab + (wave * 4 + it) * 1024);
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(doff[it]), "s"(sb), "s"(dst)
+                   : "memory");
+    }
+  };
+  // The wavefront's 64 weight rows are four 16-row groups (gate/up: groups 0, 1 gate rows of 32 neurons,
+  // groups 2, 3 the up rows of the same neurons); a group's slab is 2 KB, its two halves 1 KB each in lane order.
+  const uint8_t* wbase[4];
+  const float *ws0, *ws1;      // the scales of the tile's two 128-row blocks (gate/up: of gate and of up)
+  const uint32_t woff = lane * 16;
+  {
+    const uint8_t *w0, *w1;
+    const float *s0, *s1;
+    if (dense) {
+      w0 = a.p.w0;
+      w1 = a.p.w1;
+      s0 = a.p.s0;
+      s1 = a.p.s1;
+    } else {
+      const uint8_t* base = a.p.slab + static_cast<uint64_t>(slot) * a.p.slot_stride;
+      w0 = base + a.p.off0;
+      w1 = base + a.p.off1;
+      s0 = reinterpret_cast<const float*>(base + a.p.soff0);
+      s1 = reinterpret_cast<const float*>(base + a.p.soff1);
+    }
+    const int last16 = ((N + 15) & ~15) - 16;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const uint8_t* base = (kGateUp && g >= 2) ? w1 : w0;
+      const int n = min(kGateUp ? (n0 + wave * 32 + (g & 1) * 16) : (n0 + wave * 64 + g * 16), last16);
+      wbase[g] = uniform_ptr(base + static_cast<size_t>(n >> 4) * nk * kF8TileBytes);
+    }
+    const int nblk = (N + kF8Block - 1) / kF8Block, b0 = n0 / kF8Block;
+    ws0 = s0 + static_cast<size_t>(b0) * nk;
+    ws1 = kGateUp ? s1 + static_cast<size_t>(b0) * nk : s0 + static_cast<size_t>(min(b0 + 1, nblk - 1)) * nk;
+  }
+  typedef const __attribute__((address_space(1))) char* gptr_t;
+  auto wload = [&](int g, int slab, int h) __attribute__((always_inline)) {
+    gptr_t p = (gptr_t)(reinterpret_cast<uintptr_t>(wbase[g]) + static_cast<size_t>(slab) * kF8TileBytes + h * 1024);
+    return *reinterpret_cast<const __attribute__((address_space(1))) i32x4*>(p + woff);
+  };
+
+  // ---- scales to LDS -----------------------------------------------------------------
+  {
+    const int m = tid >> 1;
+    const uint8_t* src = sbase + static_cast<size_t>(source_row(m)) * nk;
+    uint8_t* dst = s_scales + (m & 15) * 8 + (m >> 4);
+    for (int kb = tid & 1; kb < nk; kb += 2) dst[kb * kPfBM] = src[kb];
+    float* w = reinterpret_cast<float*>(s_scales + nk * kPfBM);
+    for (int i = tid; i < 2 * nk; i += kPfThreads) w[i] = ((i & 1) ? ws1 : ws0)[i >> 1];
+  }
+  // down: factor of each row, the route weight or the sigmoid of the shared expert's gate
+  if (!kGateUp && tid < kPfBM) {
+    float sc = 1.f;
+    if (tid < M) {
+      const int p = r0 + tid;
+      if (!dense) sc = F::from_bits(static_cast<const uint16_t*>(a.p.topv)[a.p.perm[p]]);
+      else if (a.p.gate_s != nullptr) sc = sigmoid_f32(F::from_bits(static_cast<const uint16_t*>(a.p.gate_s)[p]));
+    }
+    s_row[tid] = sc;
+  }
+  __syncthreads();
+
+  // The tile's rows are processed in sub-tiles of 32; a segment's last tile is specialised on how many of
+  // them hold rows.
+  auto body = [&](auto nmi_c) {
+    constexpr int NMI = decltype(nmi_c)::value;
+    constexpr int NMT = 2 * NMI;                  // 16-row tiles
+    vf32x4 acc[NMT][4];
+#pragma unroll
+    for (int mt = 0; mt < NMT; ++mt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) acc[mt][g] = vf32x4{0.f, 0.f, 0.f, 0.f};
+
+    // While slab kt is multiplied, the rows of slab kt+2 travel to the third LDS buffer and the fragments of
+    // slab kt+2 to the registers the last row pair has just finished with.  Vector memory retires in order:
+    // "the copies of slab kt+1 have landed" is the 8 fragment loads of slab kt-1, the 4 copies and the 8
+    // fragment loads of slab kt still outstanding, vmcnt(20).  Slabs past the end refetch the last one.
+    i32x4 wfrag[2][2][4];   // [stage][k half][16-row group]
+    stage_slab(0, 0);
+    stage_slab(min(1, nk - 1), 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, min(st, nk - 1), h);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kWaitVm20);
+    __syncthreads();
+
+    // fragment of lane (r, q), tile mt, half h: row 16*mt + r, position (q + 4h) ^ f(r)
+    const int fsw = ((fr >> 1) & 7) ^ ((fr & 1) << 2);
+    const int a_row = fr * kTlRowBytes, a_x = (fq ^ fsw) << 4;
+    int cur = 0, nxt2 = 2;
+    auto slab = [&](auto stage_c, int kt) {
+      constexpr int st = decltype(stage_c)::value;
+      constexpr int NP = NMT / 2;                 // pairs of 16-row tiles
+      const int kt2 = min(kt + 2, nk - 1);
+      const uint8_t* la = lds[cur] + a_row;
+      const uint2 sb = *reinterpret_cast<const uint2*>(s_scales + kt * kPfBM + fr * 8);
+      const float2 sw = *reinterpret_cast<const float2*>(s_scales + nk * kPfBM + kt * 8);
+      const float sw0 = kGateUp ? sw.x : (wave < 2 ? sw.x : sw.y), sw1 = kGateUp ? sw.y : sw0;
+      i32x4 fa[2][2][2];   // [parity][tile of the pair][half]
+      if (NP == 1) {       // the copies go first, so that every height issues vector memory in the counted order
+        stage_slab(kt2, nxt2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      auto rd = [&](int pr, i32x4 (&f)[2][2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            f[i][h] = *reinterpret_cast<const i32x4*>(la + (2 * pr + i) * 16 * kTlRowBytes + (a_x ^ (h << 6)));
+      };
+      auto mul = [&](auto mt_c, auto g_c, const i32x4 (&f)[2]) __attribute__((always_inline)) {
+        constexpr int mt = decltype(mt_c)::value, g = decltype(g_c)::value;
+        const int sbv = static_cast<int>(mt < 4 ? sb.x : sb.y);
+        const float w = g < 2 ? sw0 : sw1;
+        const vf32x4 part = f8_mfma<0, mt & 3>(f8_join(wfrag[st][0][g], wfrag[st][1][g]), f8_join(f[0], f[1]),
+                                               vf32x4{0.f, 0.f, 0.f, 0.f}, kF8One, sbv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[mt][g][j] = fmaf(part[j], w, acc[mt][g][j]);
+      };
+      rd(0, fa[0]);
+      auto pair = [&](auto pr_c) __attribute__((always_inline)) {
+        constexpr int pr = decltype(pr_c)::value;
+        if constexpr (pr < NP) {
+          if (pr + 1 < NP) rd(pr + 1, fa[(pr + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);    // the next pair's reads stay ahead of this pair's products
+          auto group = [&](auto g_c) __attribute__((always_inline)) {
+            constexpr int g = decltype(g_c)::value;
+            mul(std::integral_constant<int, 2 * pr>{}, g_c, fa[pr & 1][0]);
+            mul(std::integral_constant<int, 2 * pr + 1>{}, g_c, fa[pr & 1][1]);
+            if constexpr (pr == NP - 1) {       // last user of group g's fragments: request those of slab kt+2
+              __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, kt2, h);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          };
+          group(std::integral_constant<int, 0>{});
+          group(std::integral_constant<int, 1>{});
+          group(std::integral_constant<int, 2>{});
+          group(std::integral_constant<int, 3>{});
+          __builtin_amdgcn_sched_barrier(0);
+          if (NP > 1 && pr == 0) {   // the copies of slab kt+2 go out once the matrix pipe has work
+            stage_slab(kt2, nxt2);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      };
+      pair(std::integral_constant<int, 0>{});
+      pair(std::integral_constant<int, 1>{});
+      pair(std::integral_constant<int, 2>{});
+      pair(std::integral_constant<int, 3>{});
+      __builtin_amdgcn_s_waitcnt(kWaitVm20);
+      __syncthreads();
+      cur = (cur == kPfStages - 1) ? 0 : cur + 1;
+      nxt2 = (nxt2 == kPfStages - 1) ? 0 : nxt2 + 1;
+    };
+    int kt = 0;
+    for (; kt + 2 <= nk; kt += 2) {
+      slab(std::integral_constant<int, 0>{}, kt);
+      slab(std::integral_constant<int, 1>{}, kt + 1);
+    }
+    if (kt < nk) slab(std::integral_constant<int, 0>{}, kt);
+    __builtin_amdgcn_s_waitcnt(kWaitVm0);  // no copy may land in LDS after the epilogue starts to reuse it
+    __syncthreads();
+
+    // ---- epilogue ----------------------------------------------------------------
+    // The product was formed as W * X^T: a lane holds row m = 16*mt + fr and, per 16-row weight group, four
+    // consecutive output columns 4*fq + j.
+    if constexpr (kGateUp) {
+      // SwiGLU, then the row's largest magnitude over the tile's 128 neurons (which are one run of the
+      // quantiser): over a lane's values, its row's four lanes, the four wavefronts.
+#pragma unroll
+      for (int mt = 0; mt < NMT; ++mt) {
+        float m = 0.f;
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float h = silu_f32(acc[mt][p][j]) * acc[mt][2 + p][j];
+            acc[mt][p][j] = n0 + wave * 32 + p * 16 < N ? h : 0.f;   // columns behind the matrix's end (a multiple of 16)
+            m = fmaxf(m, f8_magnitude(acc[mt][p][j]));
+          }
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        if (fq == 0) s_amax[wave][mt * 16 + fr] = m;
+      }
+      __syncthreads();
+      uint8_t* st = &lds[0][0];      // 128 rows x 128 bytes, 16-byte chunks swizzled by row
+#pragma unroll
+      for (int mt = 0; mt < NMT; ++mt) {
+        const int m = mt * 16 + fr;
+        const float top = fmaxf(fmaxf(s_amax[0][m], s_amax[1][m]), fmaxf(s_amax[2][m], s_amax[3][m]));
+        const float inv = f8_inverse(f8_exponent(top));
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int chunk = (wave * 2 + p) ^ (m & 7);
+          *reinterpret_cast<uint32_t*>(st + m * 128 + chunk * 16 + fq * 4) =
+              f8_pack4(acc[mt][p][0] * inv, acc[mt][p][1] * inv, acc[mt][p][2] * inv, acc[mt][p][3] * inv);
+        }
+      }
+      __syncthreads();
+      const int nb = (N + kF8Block - 1) / kF8Block;
+      uint8_t* out = dense ? a.q_s : a.q_r;
+      uint8_t* outs = dense ? a.qs_s : a.qs_r;
+#pragma unroll
+      for (int it = 0; it < NMI; ++it) {
+        const int m = it * 32 + (tid >> 3), c = tid & 7;
+        const i32x4 v = *reinterpret_cast<const i32x4*>(st + m * 128 + (c ^ (m & 7)) * 16);
+        if (m < M) *reinterpret_cast<i32x4*>(out + (static_cast<size_t>(r0 + m) * nb + bn) * kF8Block + c * 16) = v;
+      }
+      if (tid < M) {
+        const float top = fmaxf(fmaxf(s_amax[0][tid], s_amax[1][tid]), fmaxf(s_amax[2][tid], s_amax[3][tid]));
+        outs[static_cast<size_t>(r0 + tid) * nb + bn] = static_cast<uint8_t>(f8_exponent(top) + kF8Bias);
+      }
+    } else {
+      // 16-bit rows times their factor, staged per wavefront in two 32-column passes into 16-byte stores
+      uint8_t* st = &lds[0][0] + wave * (kPfBM * 64);
+      uint16_t* out = static_cast<uint16_t*>(dense ? a.p.out_s : a.p.out_r);
+      // whole 16-byte stores need rows that start on 16-byte boundaries
+      const bool whole = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll
+      for (int pass = 0; pass < 2; ++pass) {
+        if (pass) __syncthreads();  // staging rows are reused
+#pragma unroll
+        for (int mt = 0; mt < NMT; ++mt) {
+          const int m = mt * 16 + fr;
+          const float sc = s_row[m];
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const vf32x4 v = acc[mt][2 * pass + p];
+            uint2 pk;
+            pk.x = F::pack2(v[0] * sc, v[1] * sc);
+            pk.y = F::pack2(v[2] * sc, v[3] * sc);
+            const int chunk = (2 * p + (fq >> 1)) ^ ((m >> 1) & 3);
+            *reinterpret_cast<uint2*>(st + m * 64 + chunk * 16 + (fq & 1) * 8) = pk;
+          }
+        }
+        __syncthreads();
+        const int ncol0 = n0 + wave * 64 + pass * 32;
+#pragma unroll
+        for (int it = 0; it < 2 * NMI; ++it) {
+          const int m = it * 16 + (lane >> 2), q = lane & 3;
+          const uint4 val = *reinterpret_cast<const uint4*>(st + m * 64 + (q ^ ((m >> 1) & 3)) * 16);
+          const int n = ncol0 + q * 8;
+          if (m >= M || n >= N) continue;
+          uint16_t* o = out + static_cast<size_t>(r0 + m) * N + n;
+          if (whole) {
+            *reinterpret_cast<uint4*>(o) = val;
+          } else {
+            const uint32_t v[4] = {val.x, val.y, val.z, val.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (n + j < N) o[j] = static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1)));
+          }
+        }
+      }
+    }
+  };
+  switch ((M + 31) >> 5) {
+    case 1: body(std::integral_constant<int, 1>{}); break;
+    case 2: body(std::integral_constant<int, 2>{}); break;
+    case 3: body(std::integral_constant<int, 3>{}); break;
+    default: body(std::integral_constant<int, 4>{}); break;
+  }
+}
+
+template <bool kGateUp>
+static int launch_tile(const TileArgs& a, int64_t grid, hipStream_t st) {
+  SP_REQUIRE(grid < (1ll << 31), "fp8 product: grid too large");
+  const int Kmax = a.p.Ks > a.p.Kr ? a.p.Ks : a.p.Kr;
+  const unsigned dyn = static_cast<unsigned>(f8_blocks(Kmax)) * kTlScaleBytes;
+  if (a.p.dtype == SPARSE_HIP_F16)
+    hipLaunchKernelGGL((f8_tile_kernel<Fp16, kGateUp>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
+  else
+    hipLaunchKernelGGL((f8_tile_kernel<Bf16, kGateUp>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
+  SP_LAUNCH_CHECK("f8_tile_kernel");
+  return SPARSE_HIP_OK;
+}
+
+static inline int64_t queue_grid(int cap) { return (static_cast<int64_t>(cap - 1) / kPfXcds + 2) * kPfXcds; }
+static inline uint32_t magic(int topk) { return topk == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + topk - 1) / topk); }
+
+int f8_tile_gateup(const F8Product& p, const PfQueues& q, void* h, void* hs, void* sh, void* shs, hipStream_t st) {
+  TileArgs a = {};
+  a.p = p;
+  a.map = q.map_gu;
+  a.qhdr = q.hdr;
+  a.topk_magic = magic(p.topk);
+  a.q_r = static_cast<uint8_t*>(h);
+  a.qs_r = static_cast<uint8_t*>(hs);
+  a.q_s = static_cast<uint8_t*>(sh);
+  a.qs_s = static_cast<uint8_t*>(shs);
+  return launch_tile<true>(a, queue_grid(q.cap_gu), st);
+}
+
+int f8_tile_down(const F8Product& p, const PfQueues& q, hipStream_t st) {
+  TileArgs a = {};
+  a.p = p;
+  a.map = q.map_dn;
+  a.qhdr = q.hdr + 16;
+  return launch_tile<false>(a, queue_grid(q.cap_dn), st);
+}
+
+int f8_tile_linear(const F8Product& p, hipStream_t st) {
+  TileArgs a = {};
+  a.p = p;
+  a.mt = (p.T + kPfBM - 1) / kPfBM;
+  a.nt = (p.Ns + kPfBR - 1) / kPfBR;
+  const int64_t total = static_cast<int64_t>(a.mt) * a.nt;
+  SP_REQUIRE(total < (1ll << 30), "fp8_linear: too many tiles");
+  return launch_tile<false>(a, (total + kPfXcds - 1) / kPfXcds * kPfXcds, st);
+}
+
+}  // namespace sparse

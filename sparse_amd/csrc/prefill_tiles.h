@@ -22,4 +22,14 @@ struct PfTile {
   int32_t bn;    // column tile
 };
 
+// The tile queues of a call's two launches (gate/up, down), built on the device: header hdr[0..7] first
+// entry of XCD x's queue, hdr[8..15] entries in it, the same for the down launch from hdr[16] on; the
+// maps hold `cap` entries at most.
+struct PfQueues {
+  const int32_t* hdr;
+  const PfTile* map_gu;
+  const PfTile* map_dn;
+  int32_t cap_gu, cap_dn;
+};
+
 }  // namespace sparse

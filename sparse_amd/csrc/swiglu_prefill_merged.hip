@@ -485,6 +485,34 @@ static int launch_merged(PfxArgs& a, int cap, bool fp16, hipStream_t st) {
   return SPARSE_HIP_OK;
 }
 
+// Builds both launches' queues of a call in `tile_ws` (prefill_merged_ws_bytes) and says where they are.
+int prefill_queues(const int32_t* expert_slot, const int32_t* seg_offsets, const sparse_hip_seglist* segs, int Ttok,
+                   int K, int H, int I, int Is, void* tile_ws, PfQueues* q, hipStream_t st) {
+  const PfxLayout l = pfx_layout(Ttok, K, segs->n, H, I, Is);
+  int32_t* hdr = static_cast<int32_t*>(tile_ws);
+  PfTile* map_gu = reinterpret_cast<PfTile*>(static_cast<uint8_t*>(tile_ws) + kPfWsHeader);
+  PfTile* map_dn = map_gu + l.cap_gu;
+  PfxMapArgs m = {};
+  m.expert_slot = expert_slot;
+  m.seg_offsets = seg_offsets;
+  m.segs = *segs;
+  m.hdr = hdr;
+  m.map_gu = map_gu;
+  m.map_dn = map_dn;
+  m.nt_gu = l.nt_gu;
+  m.nt_dn = l.nt_dn;
+  m.nts_gu = l.nts_gu;
+  m.nts_dn = l.nts_dn;
+  m.mt_shared = l.mt_shared;
+  m.T = Ttok;
+  m.cap_gu = l.cap_gu;
+  m.cap_dn = l.cap_dn;
+  hipLaunchKernelGGL(prefill_queue_kernel, dim3(l.nt_gu + l.nt_dn + 2), dim3(256), 0, st, m);
+  SP_LAUNCH_CHECK("prefill_queue_kernel");
+  *q = PfQueues{hdr, map_gu, map_dn, l.cap_gu, l.cap_dn};
+  return SPARSE_HIP_OK;
+}
+
 // Routed experts (segs->n > 0) and / or the shared expert (sh_down_w != nullptr) of one call.
 int prefill_merged(const sparse_hip_experts* ex, const void* x, const void* topv, const int32_t* perm,
                    const int32_t* seg_offsets, const sparse_hip_seglist* segs, int Ttok, int K, void* inter_ws,
@@ -493,28 +521,10 @@ int prefill_merged(const sparse_hip_experts* ex, const void* x, const void* topv
                    hipStream_t st) {
   const int H = ex->hidden, I = ex->inter;
   const bool shared = sh_down_w != nullptr;
-  const PfxLayout l = pfx_layout(Ttok, K, segs->n, H, I, shared ? Is : 0);
-  int32_t* hdr = static_cast<int32_t*>(tile_ws);
-  PfTile* map_gu = reinterpret_cast<PfTile*>(static_cast<uint8_t*>(tile_ws) + kPfWsHeader);
-  PfTile* map_dn = map_gu + l.cap_gu;
+  PfQueues qs;
   {
-    PfxMapArgs m = {};
-    m.expert_slot = ex->expert_slot_dev;
-    m.seg_offsets = seg_offsets;
-    m.segs = *segs;
-    m.hdr = hdr;
-    m.map_gu = map_gu;
-    m.map_dn = map_dn;
-    m.nt_gu = l.nt_gu;
-    m.nt_dn = l.nt_dn;
-    m.nts_gu = l.nts_gu;
-    m.nts_dn = l.nts_dn;
-    m.mt_shared = l.mt_shared;
-    m.T = Ttok;
-    m.cap_gu = l.cap_gu;
-    m.cap_dn = l.cap_dn;
-    hipLaunchKernelGGL(prefill_queue_kernel, dim3(l.nt_gu + l.nt_dn + 2), dim3(256), 0, st, m);
-    SP_LAUNCH_CHECK("prefill_queue_kernel");
+    int rc = prefill_queues(ex->expert_slot_dev, seg_offsets, segs, Ttok, K, H, I, shared ? Is : 0, tile_ws, &qs, st);
+    if (rc != SPARSE_HIP_OK) return rc;
   }
   const bool fp16 = ex->dtype == SPARSE_HIP_F16;
   PfxArgs a = {};
@@ -538,9 +548,9 @@ int prefill_merged(const sparse_hip_experts* ex, const void* x, const void* topv
   a.out_s = static_cast<uint16_t*>(sh_inter_ws);
   a.Kdim_s = H;
   a.Ndim_s = shared ? Is : 64;
-  a.map = map_gu;
-  a.qhdr = hdr;
-  int rc = launch_merged<true>(a, l.cap_gu, fp16, st);
+  a.map = qs.map_gu;
+  a.qhdr = qs.hdr;
+  int rc = launch_merged<true>(a, qs.cap_gu, fp16, st);
   if (rc != SPARSE_HIP_OK) return rc;
   // down: inter -> parts * route weight (shared: * sigmoid(gate) where there is one)
   a.mat_offset = 2ull * I * H;
@@ -556,9 +566,9 @@ int prefill_merged(const sparse_hip_experts* ex, const void* x, const void* topv
   a.out_s = static_cast<uint16_t*>(shared_out);
   a.Kdim_s = shared ? Is : 64;
   a.Ndim_s = H;
-  a.map = map_dn;
-  a.qhdr = hdr + 16;
-  return launch_merged<false>(a, l.cap_dn, fp16, st);
+  a.map = qs.map_dn;
+  a.qhdr = qs.hdr + 16;
+  return launch_merged<false>(a, qs.cap_dn, fp16, st);
 }
 
 }  // namespace sparse

@@ -336,3 +336,13 @@ def test_no_tokens(device):
     x = torch.empty(0, 64, device=device, dtype=torch.bfloat16)
     assert fp8.linear(x, w).shape == (0, 32)
     assert fp8.quantize(x).values.shape == (0, 64)
+
+
+@pytest.mark.parametrize("T", [1, 33])
+def test_linear_long_rows(device, T):
+    """The longest rows: a scale for each of 512 runs."""
+    K, N = 65536, 16
+    q, s = rand_weight(N, K)
+    x = rand_rows(T, K, torch.bfloat16)
+    want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s))
+    within(fp8.linear(x.to(device), fp8.Weight.from_quantized(q.to(device), s.to(device))), want, bound, torch.bfloat16)
