@@ -115,12 +115,12 @@ SIGNATURES = {
     "sparse_hip_gate_select": (_i, [_vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, C.c_float, _i, _vp, _vp, _vp]),
     "sparse_hip_fp8_quantize": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
     "sparse_hip_fp8_linear_ws_bytes": (_sz, [_i, _i]),
-    "sparse_hip_fp8_linear": (_i, [_vp, _vp, _vp, _i, _i, _mat, _vp, _vp, _vp]),
+    "sparse_hip_fp8_linear": (_i, [_vp, _vp, _vp, _i, _i, _mat, _i, _vp, _vp, _vp]),
     "sparse_hip_fp8_slot_bytes": (_sz, [_i, _i]),
     "sparse_hip_fp8_moe_ffn_ws_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "sparse_hip_fp8_moe_ffn": (
-        _i, [C.POINTER(Experts), _vp, _vp, _vp, _vp, C.POINTER(SegList), _i, _i, _vp, _mat, _mat, _mat, _vp, _vp, _vp,
-             _vp]),
+        _i, [C.POINTER(Experts), _vp, _vp, _vp, _vp, C.POINTER(SegList), _i, _i, _vp, _mat, _mat, _mat, _vp, _i, _vp,
+             _vp, _vp]),
     "sparse_hip_expert_upload_async": (_i, [_vp, _vp, _sz, _vp, _vp]),
     "sparse_hip_event_create": (_i, [_i, C.POINTER(_vp)]),
     "sparse_hip_event_destroy": (_i, [_vp]),

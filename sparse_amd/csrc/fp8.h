@@ -103,7 +103,8 @@ struct F8Product {
   const void* gate_s;                               // [T] logits of the rows' sigmoid factor, or NULL
   void* out_s;
   int32_t Ks, Ns, T;
-  int32_t dtype;                                    // of topv, gate_s and 16/32-bit outputs
+  int32_t dtype;                                    // of topv, gate_s and outputs
+  int32_t pow2;                                     // every weight scale is a power of two
   sparse_hip_seglist segs;
 };
 // gate/up (SwiGLU of two products, fp32 out) or a single product, any number of rows

@@ -94,7 +94,7 @@ size_t sparse_hip_fp8_linear_ws_bytes(int T, int K) {
 }
 
 int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_dev, int dtype, int T,
-                          const sparse_hip_fp8_matrix* weight, void* out_dev, void* ws_dev, void* stream) {
+                          const sparse_hip_fp8_matrix* weight, int pow2_scales, void* out_dev, void* ws_dev, void* stream) {
   SP_REQUIRE(is_16bit(dtype), "fp8_linear: activations must be bf16 or fp16, got dtype %d", dtype);
   SP_REQUIRE(weight != nullptr, "fp8_linear: NULL weight");
   SP_REQUIRE(weight->rows >= 1 && weight->rows <= kF8MaxDim && weight->cols >= 1 && weight->cols <= kF8MaxDim,
@@ -128,6 +128,7 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   p.Ns = weight->rows;
   p.T = T;
   p.dtype = dtype;
+  p.pow2 = pow2_scales;
   if (T > SPARSE_HIP_DECODE_MAX_TOKENS) return f8_tile_linear(p, st);
   return f8_stream(p, false, false, true, st);
 }
@@ -146,7 +147,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
                            const int32_t* perm_dev, const int32_t* seg_offsets_dev, const sparse_hip_seglist* segs,
                            int T, int K, void* parts_dev, const sparse_hip_fp8_matrix* shared_gate_w,
                            const sparse_hip_fp8_matrix* shared_up_w, const sparse_hip_fp8_matrix* shared_down_w,
-                           const void* shared_gate_dev, void* shared_dev, void* ws_dev, void* stream) {
+                           const void* shared_gate_dev, int pow2_scales, void* shared_dev, void* ws_dev, void* stream) {
   static const char fn[] = "fp8_moe_ffn";
   SP_REQUIRE(experts != nullptr && segs != nullptr, "%s: NULL descriptor", fn);
   const int H = experts->hidden, I = experts->inter, E = experts->num_experts, dtype = experts->dtype;
@@ -209,6 +210,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   p.topk = K;
   p.T = T;
   p.dtype = dtype;
+  p.pow2 = pow2_scales;
   p.segs = *segs;
   // gate and up: x -> h
   p.off0 = 0;

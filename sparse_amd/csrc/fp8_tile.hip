@@ -43,7 +43,8 @@ struct TileArgs {
 };
 
 // F: the 16-bit format of outputs, route weights and gate logits
-template <typename F, bool kGateUp>
+// kPow2: every weight scale is a power of two, and enters the instruction as its exponent
+template <typename F, bool kGateUp, bool kPow2>
 __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kPfStages][kTlSlab];
   __shared__ float s_row[kPfBM];          // factor of a row (down), exponent of a row's scale (gate/up)
@@ -230,10 +231,14 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
         constexpr int mt = decltype(mt_c)::value, g = decltype(g_c)::value;
         const int sbv = static_cast<int>(mt < 4 ? sb.x : sb.y);
         const float w = g < 2 ? sw0 : sw1;
-        const vf32x4 part = f8_mfma<0, mt & 3>(f8_join(wfrag[st][0][g], wfrag[st][1][g]), f8_join(f[0], f[1]),
-                                               vf32x4{0.f, 0.f, 0.f, 0.f}, kF8One, sbv);
+        const i32x8 wf = f8_join(wfrag[st][0][g], wfrag[st][1][g]), xf = f8_join(f[0], f[1]);
+        if constexpr (kPow2) {
+          acc[mt][g] = f8_mfma<0, mt & 3>(wf, xf, acc[mt][g], static_cast<int>(__float_as_uint(w) >> 23), sbv);
+        } else {
+          const vf32x4 part = f8_mfma<0, mt & 3>(wf, xf, vf32x4{0.f, 0.f, 0.f, 0.f}, kF8One, sbv);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[mt][g][j] = fmaf(part[j], w, acc[mt][g][j]);
+          for (int j = 0; j < 4; ++j) acc[mt][g][j] = fmaf(part[j], w, acc[mt][g][j]);
+        }
       };
       rd(0, fa[0]);
       auto pair = [&](auto pr_c) __attribute__((always_inline)) {
@@ -387,10 +392,14 @@ static int launch_tile(const TileArgs& a, int64_t grid, hipStream_t st) {
   SP_REQUIRE(grid < (1ll << 31), "fp8 product: grid too large");
   const int Kmax = a.p.Ks > a.p.Kr ? a.p.Ks : a.p.Kr;
   const unsigned dyn = static_cast<unsigned>(f8_blocks(Kmax)) * kTlScaleBytes;
-  if (a.p.dtype == SPARSE_HIP_F16)
-    hipLaunchKernelGGL((f8_tile_kernel<Fp16, kGateUp>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
-  else
-    hipLaunchKernelGGL((f8_tile_kernel<Bf16, kGateUp>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
+#define SP_TILE_LAUNCH(F, P) \
+  hipLaunchKernelGGL((f8_tile_kernel<F, kGateUp, P>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a)
+  if (a.p.dtype == SPARSE_HIP_F16) {
+    if (a.p.pow2) SP_TILE_LAUNCH(Fp16, true); else SP_TILE_LAUNCH(Fp16, false);
+  } else {
+    if (a.p.pow2) SP_TILE_LAUNCH(Bf16, true); else SP_TILE_LAUNCH(Bf16, false);
+  }
+#undef SP_TILE_LAUNCH
   SP_LAUNCH_CHECK("f8_tile_kernel");
   return SPARSE_HIP_OK;
 }

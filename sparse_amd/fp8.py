@@ -129,13 +129,21 @@ def _check_quantized(values: torch.Tensor, scales: torch.Tensor, name: str = "we
         raise ValueError(f"{name} values and scales are on different devices")
 
 
+def are_pow2(scales: torch.Tensor) -> bool:
+    """Whether every scale is a power of two in fp32's normal range (8-bit products of many rows then take it
+    as an exponent)."""
+    m, _ = torch.frexp(scales)
+    return bool(((m == 0.5) & (scales >= 2.0 ** -126)).all())
+
+
 class Weight:
     """A matrix ``[rows, cols]`` laid out for the kernels, with its block scales."""
 
-    __slots__ = ("data", "scales", "rows", "cols", "desc")
+    __slots__ = ("data", "scales", "rows", "cols", "pow2", "desc")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> None:
         self.data, self.scales, self.rows, self.cols = data, scales, int(rows), int(cols)
+        self.pow2 = are_pow2(scales)
         self.desc = Fp8Matrix(data.data_ptr(), scales.data_ptr(), self.rows, self.cols)
 
     @property
@@ -184,10 +192,11 @@ def linear(x: Union[torch.Tensor, Rows], weight: Weight, out: Optional[torch.Ten
             _need(rows.data, "values", E4M3, (T, padded(K)))
             _need(rows.scales, "scales", E8M0, (T, blocks(K)))
             rc = lib.sparse_hip_fp8_linear(None, _ptr(rows.data), _ptr(rows.scales), code, T, C.byref(weight.desc),
-                                           _ptr(out), None, stream)
+                                           int(weight.pow2), _ptr(out), None, stream)
         else:
             ws = src.new_empty((max(1, lib.sparse_hip_fp8_linear_ws_bytes(T, K)),), dtype=torch.uint8)
-            rc = lib.sparse_hip_fp8_linear(_ptr(src), None, None, code, T, C.byref(weight.desc), _ptr(out), _ptr(ws), stream)
+            rc = lib.sparse_hip_fp8_linear(_ptr(src), None, None, code, T, C.byref(weight.desc), int(weight.pow2),
+                                           _ptr(out), _ptr(ws), stream)
     _lib.check(rc, "sparse_hip_fp8_linear")
     return out
 
@@ -228,6 +237,7 @@ class ExpertSlab:
         self.num_slots, self.num_experts = int(num_slots), int(num_experts)
         self.expert_bytes = slot_bytes(hidden, inter)
         self.data = torch.empty((self.num_slots, self.expert_bytes), dtype=torch.uint8, device=device)
+        self.pow2 = False       # whether every scale of the slots in use is a power of two
         self.expert_slot = torch.arange(self.num_experts, dtype=torch.int32, device=device)
 
     @classmethod
@@ -237,6 +247,7 @@ class ExpertSlab:
         slab = cls(len(experts), len(experts), gate.shape[1], gate.shape[0], device if device is not None else gate.device)
         for e, expert in enumerate(experts):
             pack_expert_into(slab.data[e], expert, slab.hidden, slab.inter)
+        slab.pow2 = are_pow2(torch.cat([s.reshape(-1) for expert in experts for _, s in expert]))
         return slab
 
     @classmethod
@@ -302,6 +313,7 @@ def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Perm
     else:
         shared_gate = shared_out = None
     lib = _lib.load()
+    pow2 = int(experts.pow2 and (shared is None or all(m.pow2 for m in shared)))
     need = lib.sparse_hip_fp8_moe_ffn_ws_bytes(T, K, segs.n, H, experts.inter, Is)
     with on_device(x, topv, perm.perm, experts.data, parts, shared_gate, shared_out, ws,
                    None if shared is None else shared[0].data) as stream:
@@ -313,7 +325,7 @@ def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Perm
             return parts, shared_out
         desc = experts.descriptor(dtype)
         rc = lib.sparse_hip_fp8_moe_ffn(C.byref(desc), _ptr(x), _ptr(topv), _ptr(perm.perm), _ptr(perm.seg_offsets),
-                                        C.byref(segs), T, K, _ptr(parts), *mats, _ptr(shared_gate), _ptr(shared_out),
-                                        _ptr(ws), stream)
+                                        C.byref(segs), T, K, _ptr(parts), *mats, _ptr(shared_gate), pow2,
+                                        _ptr(shared_out), _ptr(ws), stream)
     _lib.check(rc, "sparse_hip_fp8_moe_ffn")
     return parts, shared_out

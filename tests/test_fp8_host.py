@@ -36,6 +36,19 @@ def test_weight_round_trip():
         fp8.quantize_weight(torch.tensor([[1.0, float("nan")]]))
 
 
+def test_power_of_two_scales_are_recognised():
+    q, s = fp8.quantize_weight(torch.randn(130, 257))
+    assert fp8.Weight.from_quantized(q, s).pow2
+    for bad in (3.0, 0.0, -2.0, float("inf"), float("nan"), 2.0 ** -127):
+        t = s.clone()
+        t[1, 2] = bad
+        assert not fp8.Weight.from_quantized(q, t).pow2
+    ex = tuple(fp8.quantize_weight(torch.randn(*sh)) for sh in ((64, 192), (64, 192), (192, 64)))
+    assert fp8.ExpertSlab.from_quantized([ex, ex]).pow2
+    odd = (ex[0], (ex[1][0], ex[1][1] * 1.5), ex[2])
+    assert not fp8.ExpertSlab.from_quantized([ex, odd, ex]).pow2
+
+
 def test_slot_layout():
     H, I = 192, 64
     assert fp8.slot_bytes(H, I) == (2 * 64 * 256 + 192 * 128 + 4 * (2 + 2 + 2) + 255) // 256 * 256
@@ -117,7 +130,7 @@ def test_quantize_and_linear_refusals():
     assert lib.sparse_hip_fp8_quantize(None, 1, 0, 1, None, None, None) == 0
 
     def lin(m=_lib.Fp8Matrix(P, P, 32, 64), x=P, xq=None, xs=None, dt=1, T=2, out=P, ws=P):
-        return lib.sparse_hip_fp8_linear(x, xq, xs, dt, T, None if m is None else C.byref(m), out, ws, None)
+        return lib.sparse_hip_fp8_linear(x, xq, xs, dt, T, None if m is None else C.byref(m), 0, out, ws, None)
 
     refused(lin(dt=5), "dtype")
     refused(lin(dt=0), "bf16 or fp16")
@@ -156,7 +169,7 @@ def test_moe_ffn_refusals():
         ex = _lib.Experts(slab, stride, None, E, h, i, dt)
         sg = segs() if sg is None else sg
         return lib.sparse_hip_fp8_moe_ffn(C.byref(ex), x, topv, P, P, C.byref(sg), T, K, parts,
-                                          *(None if v is None else C.byref(v) for v in m), None, sh, ws, None)
+                                          *(None if v is None else C.byref(v) for v in m), None, 0, sh, ws, None)
 
     refused(call(dt=0), "bf16 or fp16")
     refused(call(E=257), "E=257")
