@@ -33,7 +33,7 @@ SOURCES = [
     "gate_select.hip",
     "fp8.hip",
     "fp8_quantize.hip",
-    "fp8_stream.hip",
+    "fp8_few.hip",
     "fp8_tile.hip",
     "rs_predict.hip",
     "layout.hip",

@@ -35,6 +35,14 @@ __device__ __forceinline__ int f8_exponent(float amax) {
 }
 // 2^-s for an exponent in [-120, 120]
 __device__ __forceinline__ float f8_inverse(int s) { return __uint_as_float(static_cast<uint32_t>(127 - s) << 23); }
+// Largest of magnitudes over the 16 lanes of a DPP row, in every one of them.
+__device__ __forceinline__ float f8_row16_max(float v) {
+  v = fmaxf(v, dpp_move<0x121, 0xf>(0.f, v));   // row_ror:1, 2, 4, 8
+  v = fmaxf(v, dpp_move<0x122, 0xf>(0.f, v));
+  v = fmaxf(v, dpp_move<0x124, 0xf>(0.f, v));
+  v = fmaxf(v, dpp_move<0x128, 0xf>(0.f, v));
+  return v;
+}
 // The magnitude that counts towards amax: NaN and infinities do not (they become NaN in 8 bits).
 __device__ __forceinline__ float f8_magnitude(float v) {
   const float a = fabsf(v);
@@ -93,7 +101,7 @@ struct F8Product {
   uint64_t slot_stride, off0, off1, soff0, soff1;   // bytes: matrices (second: up) and their scales in a slot
   const int32_t *expert_slot, *perm, *seg_offsets;
   const void* topv;
-  const uint8_t *act_r, *act_rs;                    // values, scales; gathered through perm when gather != 0
+  const uint8_t *act_r, *act_rs;                    // rows, scales of 8-bit ones; gathered through perm when gather != 0
   void* out_r;
   int32_t topk, Kr, Nr, gather;
   // dense operands
@@ -107,8 +115,10 @@ struct F8Product {
   int32_t pow2;                                     // every weight scale is a power of two
   sparse_hip_seglist segs;
 };
-// gate/up (SwiGLU of two products, fp32 out) or a single product, any number of rows
-int f8_stream(const F8Product& p, bool gateup, bool routed, bool dense, hipStream_t st);
+// Few rows: gate/up (SwiGLU of two products, fp32 out) or a single product, of rows that are quantised on the
+// way in (from the 16-bit type, from fp32) or were before.  Routed calls: T <= 32.
+enum { kF8From16 = 0, kF8From32 = 1, kF8From8 = 2 };
+int f8_few(const F8Product& p, int source, bool gateup, bool routed, bool dense, hipStream_t st);
 
 // The same for many rows, 16-bit formats: 128 x 256 tiles.  gate/up writes quantised rows; routed and dense
 // tiles come from one set of queues (prefill_queues, which builds them).

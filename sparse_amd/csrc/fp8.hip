@@ -21,6 +21,10 @@ struct Carve {
   }
 };
 
+// Up to here the down projection quantises the intermediate itself, each workgroup its rows; from here on
+// every workgroup of the shared expert would read all rows as fp32, and a launch of its own is cheaper.
+constexpr int kF8InlineRows = 8;
+
 struct F8Rows {
   uint8_t *values, *scales;
 };
@@ -37,8 +41,8 @@ struct LinearWs {
 };
 static LinearWs linear_ws(void* ws, int T, int K) {
   Carve c{static_cast<uint8_t*>(ws)};
-  LinearWs w;
-  w.x = take_rows(c, T, K);
+  LinearWs w = {};
+  if (T > SPARSE_HIP_DECODE_MAX_TOKENS) w.x = take_rows(c, T, K);
   w.bytes = c.used;
   return w;
 }
@@ -53,10 +57,12 @@ static FfnWs ffn_ws(void* ws, int T, int K, int nseg, int H, int I, int Is) {
   Carve c{static_cast<uint8_t*>(ws)};
   FfnWs w = {};
   const int64_t rows = nseg > 0 ? static_cast<int64_t>(T) * K : 0;
-  w.x = take_rows(c, T, H);
-  w.h = take_rows(c, rows, I);
-  if (Is > 0) w.sh = take_rows(c, T, Is);
+  if (T > kF8InlineRows) {
+    w.h = take_rows(c, rows, I);
+    if (Is > 0) w.sh = take_rows(c, T, Is);
+  }
   if (T > SPARSE_HIP_DECODE_MAX_TOKENS) {
+    w.x = take_rows(c, T, H);
     w.tiles = c.take(prefill_merged_ws_bytes(T, K, nseg, H, I, Is));
   } else {
     w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
@@ -107,7 +113,13 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   SP_REQUIRE(out_dev != nullptr, "fp8_linear: NULL output");
   hipStream_t st = as_stream(stream);
   F8Product p = {};
-  if (x_dev != nullptr) {
+  const bool tiles = T > SPARSE_HIP_DECODE_MAX_TOKENS;
+  int source = kF8From8;
+  if (x_dev == nullptr) {
+    SP_REQUIRE(xs_dev != nullptr && aligned16(xq_dev), "fp8_linear: 8-bit rows need scales and 16-byte alignment");
+    p.act_s = static_cast<const uint8_t*>(xq_dev);
+    p.act_ss = static_cast<const uint8_t*>(xs_dev);
+  } else if (tiles) {
     SP_REQUIRE(ws_dev != nullptr && aligned16(ws_dev), "fp8_linear: workspace is NULL or not 16-byte aligned");
     const LinearWs w = linear_ws(ws_dev, T, weight->cols);
     rc = f8_quantize(x_dev, dtype, T, weight->cols, w.x.values, w.x.scales, st);
@@ -115,9 +127,8 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
     p.act_s = w.x.values;
     p.act_ss = w.x.scales;
   } else {
-    SP_REQUIRE(xs_dev != nullptr && aligned16(xq_dev), "fp8_linear: 8-bit rows need scales and 16-byte alignment");
-    p.act_s = static_cast<const uint8_t*>(xq_dev);
-    p.act_ss = static_cast<const uint8_t*>(xs_dev);
+    source = kF8From16;
+    p.act_s = static_cast<const uint8_t*>(x_dev);
   }
   p.w0 = static_cast<const uint8_t*>(weight->values_dev);
   p.s0 = weight->scales_dev;
@@ -129,8 +140,7 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   p.T = T;
   p.dtype = dtype;
   p.pow2 = pow2_scales;
-  if (T > SPARSE_HIP_DECODE_MAX_TOKENS) return f8_tile_linear(p, st);
-  return f8_stream(p, false, false, true, st);
+  return tiles ? f8_tile_linear(p, st) : f8_few(p, source, false, false, true, st);
 }
 
 size_t sparse_hip_fp8_slot_bytes(int H, int I) {
@@ -192,12 +202,13 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   hipStream_t st = as_stream(stream);
   const FfnWs w = ffn_ws(ws_dev, T, K, segs->n, H, I, Is);
 
-  const bool tiles = T > SPARSE_HIP_DECODE_MAX_TOKENS;
-  int rc = f8_quantize(x_dev, dtype, T, H, w.x.values, w.x.scales, st);
-  if (rc != SPARSE_HIP_OK) return rc;
+  const bool tiles = T > SPARSE_HIP_DECODE_MAX_TOKENS, before = T > kF8InlineRows;
+  int rc = SPARSE_HIP_OK;
   PfQueues queues = {};
   if (tiles) {
-    rc = prefill_queues(experts->expert_slot_dev, seg_offsets_dev, segs, T, K, H, I, Is, w.tiles, &queues, st);
+    rc = f8_quantize(x_dev, dtype, T, H, w.x.values, w.x.scales, st);
+    if (rc == SPARSE_HIP_OK)
+      rc = prefill_queues(experts->expert_slot_dev, seg_offsets_dev, segs, T, K, H, I, Is, w.tiles, &queues, st);
     if (rc != SPARSE_HIP_OK) return rc;
   }
   F8Product p = {};
@@ -217,7 +228,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   p.off1 = slot.up;
   p.soff0 = slot.sgate;
   p.soff1 = slot.sup;
-  p.act_r = p.act_s = w.x.values;
+  p.act_r = p.act_s = tiles ? w.x.values : static_cast<const uint8_t*>(x_dev);
   p.act_rs = p.act_ss = w.x.scales;
   p.gather = 1;
   p.out_r = w.hf;
@@ -232,17 +243,19 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
     p.Ks = H;
     p.Ns = Is;
   }
-  if (tiles)
+  if (tiles) {
     rc = f8_tile_gateup(p, queues, w.h.values, w.h.scales, w.sh.values, w.sh.scales, st);
-  else
-    rc = f8_stream(p, true, routed, shared, st);
-  if (!tiles && rc == SPARSE_HIP_OK && routed) rc = f8_quantize(w.hf, SPARSE_HIP_F32, static_cast<int64_t>(T) * K, I, w.h.values, w.h.scales, st);
-  if (!tiles && rc == SPARSE_HIP_OK && shared) rc = f8_quantize(w.shf, SPARSE_HIP_F32, T, Is, w.sh.values, w.sh.scales, st);
+  } else {
+    rc = f8_few(p, kF8From16, true, routed, shared, st);
+    if (before && rc == SPARSE_HIP_OK && routed)
+      rc = f8_quantize(w.hf, SPARSE_HIP_F32, static_cast<int64_t>(T) * K, I, w.h.values, w.h.scales, st);
+    if (before && rc == SPARSE_HIP_OK && shared) rc = f8_quantize(w.shf, SPARSE_HIP_F32, T, Is, w.sh.values, w.sh.scales, st);
+  }
   if (rc != SPARSE_HIP_OK) return rc;
   // down: h -> rows times their route weight (shared expert: times sigmoid of its gate)
   p.off0 = p.off1 = slot.down;
   p.soff0 = p.soff1 = slot.sdown;
-  p.act_r = w.h.values;
+  p.act_r = before ? w.h.values : reinterpret_cast<const uint8_t*>(w.hf);
   p.act_rs = w.h.scales;
   p.gather = 0;
   p.out_r = parts_dev;
@@ -251,14 +264,14 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   if (shared) {
     p.w0 = p.w1 = static_cast<const uint8_t*>(shared_down_w->values_dev);
     p.s0 = p.s1 = shared_down_w->scales_dev;
-    p.act_s = w.sh.values;
+    p.act_s = before ? w.sh.values : reinterpret_cast<const uint8_t*>(w.shf);
     p.act_ss = w.sh.scales;
     p.gate_s = shared_gate_dev;
     p.out_s = shared_dev;
     p.Ks = Is;
     p.Ns = H;
   }
-  return tiles ? f8_tile_down(p, queues, st) : f8_stream(p, false, routed, shared, st);
+  return tiles ? f8_tile_down(p, queues, st) : f8_few(p, before ? kF8From8 : kF8From32, false, routed, shared, st);
 }
 
 }  // extern "C"

@@ -7,15 +7,6 @@ constexpr int kQzThreads = 256;
 constexpr int kQzLane = 8;                       // values per lane: 16 lanes make a run
 constexpr int kQzRuns = kQzThreads * kQzLane / kF8Block;
 
-// Largest over the 16 lanes of a DPP row, in every one of them.
-__device__ __forceinline__ float row16_max(float v) {
-  v = fmaxf(v, dpp_move<0x121, 0xf>(0.f, v));   // row_ror:1
-  v = fmaxf(v, dpp_move<0x122, 0xf>(0.f, v));
-  v = fmaxf(v, dpp_move<0x124, 0xf>(0.f, v));
-  v = fmaxf(v, dpp_move<0x128, 0xf>(0.f, v));
-  return v;
-}
-
 // kVec: rows start on 16-byte boundaries and K is a multiple of 8
 template <typename T, bool kVec>
 __global__ __launch_bounds__(kQzThreads) void f8_quantize_kernel(const T* __restrict__ x, int64_t runs, int K, int nb,
@@ -44,7 +35,7 @@ __global__ __launch_bounds__(kQzThreads) void f8_quantize_kernel(const T* __rest
   float m = 0.f;
 #pragma unroll
   for (int j = 0; j < kQzLane; ++j) m = fmaxf(m, f8_magnitude(v[j]));
-  m = row16_max(m);
+  m = f8_row16_max(m);
   const int s = f8_exponent(m);
   const float inv = f8_inverse(s);
   uint2 q;

@@ -153,26 +153,34 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
     return *reinterpret_cast<const __attribute__((address_space(1))) i32x4*>(p + woff);
   };
 
-  // ---- scales to LDS -----------------------------------------------------------------
-  {
-    const int m = tid >> 1;
-    const uint8_t* src = sbase + static_cast<size_t>(source_row(m)) * nk;
+  // ---- scales to LDS, row factors ------------------------------------------------------
+  // Called once the first slabs are on their way.  Bytes are fetched eight at a time before the first is
+  // stored: one by one, each would wait a memory latency (a 16-slab tile then spent 8 of them here).
+  const uint8_t* my_scales = sbase + static_cast<size_t>(source_row(tid >> 1)) * nk;
+  auto fill_scales = [&]() __attribute__((always_inline)) {
+    const int m = tid >> 1, half = tid & 1;
     uint8_t* dst = s_scales + (m & 15) * 8 + (m >> 4);
-    for (int kb = tid & 1; kb < nk; kb += 2) dst[kb * kPfBM] = src[kb];
     float* w = reinterpret_cast<float*>(s_scales + nk * kPfBM);
-    for (int i = tid; i < 2 * nk; i += kPfThreads) w[i] = ((i & 1) ? ws1 : ws0)[i >> 1];
-  }
-  // down: factor of each row, the route weight or the sigmoid of the shared expert's gate
-  if (!kGateUp && tid < kPfBM) {
-    float sc = 1.f;
-    if (tid < M) {
-      const int p = r0 + tid;
-      if (!dense) sc = F::from_bits(static_cast<const uint16_t*>(a.p.topv)[a.p.perm[p]]);
-      else if (a.p.gate_s != nullptr) sc = sigmoid_f32(F::from_bits(static_cast<const uint16_t*>(a.p.gate_s)[p]));
+    for (int kb0 = 0; kb0 < nk; kb0 += 16) {
+      uint8_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = my_scales[min(kb0 + 2 * i + half, nk - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (kb0 + 2 * i + half < nk) dst[(kb0 + 2 * i + half) * kPfBM] = v[i];
     }
-    s_row[tid] = sc;
-  }
-  __syncthreads();
+    for (int i = tid; i < 2 * nk; i += kPfThreads) w[i] = ((i & 1) ? ws1 : ws0)[i >> 1];
+    // down: factor of each row, the route weight or the sigmoid of the shared expert's gate
+    if (!kGateUp && tid < kPfBM) {
+      float sc = 1.f;
+      if (tid < M) {
+        const int p = r0 + tid;
+        if (!dense) sc = F::from_bits(static_cast<const uint16_t*>(a.p.topv)[a.p.perm[p]]);
+        else if (a.p.gate_s != nullptr) sc = sigmoid_f32(F::from_bits(static_cast<const uint16_t*>(a.p.gate_s)[p]));
+      }
+      s_row[tid] = sc;
+    }
+  };
 
   // The tile's rows are processed in sub-tiles of 32; a segment's last tile is specialised on how many of
   // them hold rows.
@@ -199,6 +207,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
       for (int g = 0; g < 4; ++g)
 #pragma unroll
         for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, min(st, nk - 1), h);
+    __builtin_amdgcn_sched_barrier(0);
+    fill_scales();
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(kWaitVm20);
     __syncthreads();

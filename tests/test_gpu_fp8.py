@@ -22,6 +22,11 @@ def within(got, want, bound, dtype):
     assert worst <= 0, f"off by {worst} more than allowed; largest error {float(err.max())}"
 
 
+def grouped(T):
+    """Calls of up to 32 tokens add products in fp32, larger ones in the 8-bit instruction's groups."""
+    return T > 32
+
+
 def rand_rows(T, K, dtype, seed=0):
     g = torch.Generator().manual_seed(seed + 17 * T + K)
     loud = torch.exp(torch.randn(K, generator=g))
@@ -115,13 +120,24 @@ def test_linear(device, dtype, T, K, N):
     for pow2 in (False, True):
         x, (q, s) = rand_rows(T, K, dtype), rand_weight(N, K, pow2=pow2)
         w = fp8.Weight.from_quantized(q.to(device), s.to(device))
-        want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s))
+        want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s), grouped(T))
         x = x.to(device)
         y = fp8.linear(x, w)
         assert y.dtype == dtype
         within(y, want, bound, dtype)
         assert torch.equal(fp8.linear(fp8.quantize(x), w), y), "rows quantised before or inside the call"
         assert torch.equal(w.dequantize(torch.float64).cpu(), ref_fp8.weight(q, s))
+
+
+@pytest.mark.parametrize("T", [1, 7, 40])
+def test_linear_far_from_one(device, T):
+    """Rows near both ends of the range, runs whose scale is the lowest."""
+    x = torch.randn(T, 300, generator=torch.Generator().manual_seed(T))
+    q, s = rand_weight(48, 300)
+    for lo, hi in ((2.0 ** -124, 2.0 ** 100), (2.0 ** 90, 2.0 ** -60), (2.0 ** -133, 2.0 ** 120)):
+        xs = (x * lo).to(torch.bfloat16)
+        want, bound = ref_fp8.product(ref_fp8.rows(xs), (q, s * hi), grouped(T))
+        within(fp8.linear(xs.to(device), fp8.Weight.from_quantized(q.to(device), (s * hi).to(device))), want, bound, torch.bfloat16)
 
 
 @pytest.mark.parametrize("T", [1, 18])
@@ -131,7 +147,7 @@ def test_linear_large_weight(device, T):
     q = (torch.randn(N, K, generator=g, device=device) * 60).to(fp8.E4M3)
     s = torch.rand(44, 16, generator=g, device=device) * 1e-3 + 1e-4
     x = rand_rows(T, K, torch.bfloat16)
-    want, bound = ref_fp8.product(ref_fp8.rows(x), (q.cpu(), s.cpu()))
+    want, bound = ref_fp8.product(ref_fp8.rows(x), (q.cpu(), s.cpu()), grouped(T))
     within(fp8.linear(x.to(device), fp8.Weight.from_quantized(q, s)), want, bound, torch.bfloat16)
 
 
@@ -200,7 +216,7 @@ def on_gpu(c, device):
 
 
 def oracle(c):
-    return ref_fp8.experts(c["x"], c["topi"], c["topv"], c["ex"], c["sh"], c["sg"])
+    return ref_fp8.experts(c["x"], c["topi"], c["topv"], c["ex"], c["sh"], c["sg"], grouped(c["x"].shape[0]))
 
 
 CASES = [  # T, H, E, I, K, Is, gate
@@ -344,5 +360,5 @@ def test_linear_long_rows(device, T):
     K, N = 65536, 16
     q, s = rand_weight(N, K)
     x = rand_rows(T, K, torch.bfloat16)
-    want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s))
+    want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s), grouped(T))
     within(fp8.linear(x.to(device), fp8.Weight.from_quantized(q.to(device), s.to(device))), want, bound, torch.bfloat16)
