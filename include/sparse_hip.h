@@ -499,6 +499,12 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
  * aligned; calls that share one must be ordered on one stream.
  */
 size_t sparse_hip_fp8_slot_bytes(int H, int I);
+/*
+ * Measurement aid: which kernels the 8-bit products of more than two rows take, for the whole process.  0 (the
+ * default): by size; 1: those that stream weights past the rows; 2: tiles.  Both are right at any size; they
+ * differ in the order of their sums.  A workspace's size depends on it.  Returns the setting before.
+ */
+int sparse_hip_fp8_path(int which);
 size_t sparse_hip_fp8_moe_ffn_ws_bytes(int T, int K, int num_segments, int H, int I, int Is);
 int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev, const void* topv_dev,
                            const int32_t* perm_dev, const int32_t* seg_offsets_dev,

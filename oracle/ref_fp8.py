@@ -110,7 +110,7 @@ def product(x, w, grouped):
     return y, ((K // 8 if grouped else K) + 4 * blocks(K) + 16) * EPS32 * mag
 
 
-def swiglu(x, gate, up, down, grouped):
+def swiglu(x, gate, up, down, grouped, grouped_down):
     """SwiGLU of (already quantised) rows on (values, scales) weights, with the bound of an fp32 implementation.
 
     An error of h moves a quantised value only where a rounding border lies within it; how far is found by
@@ -129,9 +129,9 @@ def swiglu(x, gate, up, down, grouped):
         for s in (exponent(runs(h.abs() + d).amax(-1)), exponent(runs((h.abs() - d).clamp_min(0)).amax(-1)), exponent(top)):
             back = torch.ldexp(round_e4m3(torch.ldexp(runs(lo_hi), -s[..., None])), s[..., None])
             off = torch.maximum(off, (back.reshape(h.shape[0], -1)[:, :h.shape[1]] - mid).abs())
-    y, ey = product(mid, down, grouped)
+    y, ey = product(mid, down, grouped_down)
     w = weight(*down).abs()
-    if not grouped:
+    if not grouped_down:
         return y, ey + off @ w.t()
     # eight products of a group that holds a moved value: its largest, times 2^-13, each
     moved = (runs(off) > 0).view(off.shape[0], -1, 8).any(-1, keepdim=True)
@@ -141,7 +141,7 @@ def swiglu(x, gate, up, down, grouped):
     return y, ey + off @ w.t() + cut @ wg.t() / 8
 
 
-def experts(x, topi, topv, triples, shared=None, shared_gate=None, grouped=True):
+def experts(x, topi, topv, triples, shared=None, shared_gate=None, grouped=True, grouped_down=True):
     """(parts, bound, shared rows, bound): permuted rows (expert id, flat index) times their route weight.
     ``triples[e]`` / ``shared``: (gate, up, down), each (values, scales)."""
     K = topi.shape[1]
@@ -151,12 +151,12 @@ def experts(x, topi, topv, triples, shared=None, shared_gate=None, grouped=True)
     for e, t in enumerate(triples):
         items = torch.nonzero(flat == e).reshape(-1)
         if items.numel():
-            y, b = swiglu(xq[items // K], *t, grouped)
+            y, b = swiglu(xq[items // K], *t, grouped, grouped_down)
             out.append(y * w[items, None])
             bound.append(b * w[items, None].abs())
     sh = shb = None
     if shared is not None:
-        sh, shb = swiglu(xq, *shared, grouped)
+        sh, shb = swiglu(xq, *shared, grouped, grouped_down)
         if shared_gate is not None:
             f = torch.sigmoid(shared_gate.double())[:, None]
             sh, shb = sh * f, shb * f + 2.0 ** -20 * (sh * f).abs()

@@ -34,6 +34,7 @@ SOURCES = [
     "fp8.hip",
     "fp8_quantize.hip",
     "fp8_few.hip",
+    "fp8_rows.hip",
     "fp8_tile.hip",
     "rs_predict.hip",
     "layout.hip",

@@ -72,6 +72,51 @@ __device__ __forceinline__ vf32x4 f8_mfma(i32x8 a, i32x8 b, vf32x4 c, int sa, in
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, kSa, sa, kSb, sb);
 }
 
+// Four consecutive columns n .. n + 3 of a row of N, times `sc`, rounded once.
+template <typename F>
+__device__ __forceinline__ void f8_store4(uint16_t* o, vf32x4 v, float sc, int N, int n) {
+  uint2 pk;
+  pk.x = F::pack2(v[0] * sc, v[1] * sc);
+  pk.y = F::pack2(v[2] * sc, v[3] * sc);
+  if (N % 4 == 0 && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
+    *reinterpret_cast<uint2*>(o) = pk;
+  } else {
+    const uint32_t e[2] = {pk.x, pk.y};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < N) o[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
+  }
+}
+
+// Eight e4m3 bytes as bf16, which holds them exactly.
+template <bool kHigh>
+__device__ __forceinline__ uint32_t f8_widen2(uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, kHigh));
+}
+__device__ __forceinline__ bf16x8 f8_widen8(uint32_t lo, uint32_t hi) {
+  const u32x4 v = {f8_widen2<false>(lo), f8_widen2<true>(lo), f8_widen2<false>(hi), f8_widen2<true>(hi)};
+  return __builtin_bit_cast(bf16x8, v);
+}
+// The 32 bytes of one operand of a 128-wide block as the operands of four 32-wide bf16 instructions, and the
+// product of two such: products added in fp32 (no scales), where the 8-bit instruction cuts them off.
+struct F8Wide {
+  bf16x8 v[4];
+};
+__device__ __forceinline__ F8Wide f8_widen(i32x4 lo, i32x4 hi) {
+  F8Wide r;
+  r.v[0] = f8_widen8(lo[0], lo[1]);
+  r.v[1] = f8_widen8(lo[2], lo[3]);
+  r.v[2] = f8_widen8(hi[0], hi[1]);
+  r.v[3] = f8_widen8(hi[2], hi[3]);
+  return r;
+}
+__device__ __forceinline__ vf32x4 f8_mfma_wide(const F8Wide& a, const F8Wide& b) {
+  vf32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[j], b.v[j], c, 0, 0, 0);
+  return c;
+}
+
 // How a slot of the expert slab is laid out: gate values [I, Hp] | up [I, Hp] | down [H, Ip], then their
 // scales [nI, nH] | [nI, nH] | [nH, nI] in fp32 (Hp, Ip: rounded up to 128; nH, nI: number of blocks).
 struct F8Slot {
@@ -91,8 +136,15 @@ inline F8Slot f8_slot(int H, int I) {
 }
 
 // ---- launches of the other files ---------------------------------------------------------------
-// rows of x (dtype code) -> values [T, Kp], scales [T, blocks]
-int f8_quantize(const void* x, int dtype, int64_t T, int K, void* values, void* scales, hipStream_t st);
+// rows of x (dtype code) -> values [T, Kp], scales [T, blocks]; a second matrix of the same type in the same
+// launch if T2 > 0
+struct F8Quantize {
+  const void* x;
+  int64_t T;
+  int32_t K;
+  void *values, *scales;
+};
+int f8_quantize(const F8Quantize& a, const F8Quantize& b, int dtype, hipStream_t st);
 
 // One matrix product of a call, over the routed segments of an expert slab, a dense matrix, or both.
 struct F8Product {
@@ -115,10 +167,14 @@ struct F8Product {
   int32_t pow2;                                     // every weight scale is a power of two
   sparse_hip_seglist segs;
 };
-// Few rows: gate/up (SwiGLU of two products, fp32 out) or a single product, of rows that are quantised on the
-// way in (from the 16-bit type, from fp32) or were before.  Routed calls: T <= 32.
+// Two rows at most: gate/up (SwiGLU of two products, fp32 out) or a single product, of rows that are
+// quantised on the way in (from the 16-bit type, from fp32) or were before.
+constexpr int kF8FewRows = 2;
 enum { kF8From16 = 0, kF8From32 = 1, kF8From8 = 2 };
 int f8_few(const F8Product& p, int source, bool gateup, bool routed, bool dense, hipStream_t st);
+
+// The same of more rows, 8-bit ones.
+int f8_rows(const F8Product& p, bool gateup, bool routed, bool dense, hipStream_t st);
 
 // The same for many rows, 16-bit formats: 128 x 256 tiles.  gate/up writes quantised rows; routed and dense
 // tiles come from one set of queues (prefill_queues, which builds them).

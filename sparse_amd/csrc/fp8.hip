@@ -1,10 +1,36 @@
 // C ABI of the block-scaled 8-bit operators: argument checks and the order of launches.
+#include <atomic>
+
 #include "fp8.h"
 #include "prefill_tiles.h"
 
 namespace sparse {
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Which kernels serve more than kF8FewRows rows: 0 by size, 1 the streaming ones, 2 the tiles.
+static std::atomic<int> g_path{0};
+
+// The streaming kernel reads the weights once for every 32 rows, the tile kernel once or twice in all, but it
+// starts slowly (10 us for its first tile, then 1.2 us a 128-wide slab while few tiles are there to overlap)
+// and reads weights that are used once at 4.5 TB/s where the streaming kernel reaches 6.  Measured on both
+// sides of the border, streaming / tiles:
+//   linear  2048 x 5632: 128 rows 21 / 29 us, 256 rows 34 / 29;  4096 x 4096: 128 rows 30 / 48, 256 rows 53 / 49
+//   experts 60 of 1408 x 2048, 4 a token, shared 5632: 64 tokens 108 / 126 us, 128 tokens 149 / 137
+//           16 of 704 x 1024, 3 a token: 256 tokens 38 / 41 us, 384 tokens 47 / 42
+//           8 of 704 x 2048, 2 a token, shared 1408: 128 tokens 38 / 42 us, 192 tokens 48 / 42
+static bool linear_tiles(int T, int N) {
+  const int path = g_path.load(std::memory_order_relaxed);
+  if (T <= kF8FewRows || path == 1) return false;
+  return path == 2 || static_cast<int64_t>((T + 31) / 32) * N > 28672;
+}
+static bool ffn_tiles(int T, int K, int nseg, int H, int I, int Is) {
+  const int path = g_path.load(std::memory_order_relaxed);
+  if (T <= kF8FewRows || path == 1) return false;
+  // work of the rows against a fixed cost and one for the weights
+  const double h = H, rows = T * h * (static_cast<double>(nseg > 0 ? K : 0) * I + Is);
+  return path == 2 || rows > (1 << 29) + 7.0 * h * (static_cast<double>(nseg) * I + Is);
+}
+
 static inline size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 constexpr int kF8MaxDim = 1 << 16;      // the tile kernel keeps a scale byte per row and block in LDS
@@ -20,10 +46,6 @@ struct Carve {
     return p;
   }
 };
-
-// Up to here the down projection quantises the intermediate itself, each workgroup its rows; from here on
-// every workgroup of the shared expert would read all rows as fp32, and a launch of its own is cheaper.
-constexpr int kF8InlineRows = 8;
 
 struct F8Rows {
   uint8_t *values, *scales;
@@ -42,7 +64,7 @@ struct LinearWs {
 static LinearWs linear_ws(void* ws, int T, int K) {
   Carve c{static_cast<uint8_t*>(ws)};
   LinearWs w = {};
-  if (T > SPARSE_HIP_DECODE_MAX_TOKENS) w.x = take_rows(c, T, K);
+  if (T > kF8FewRows) w.x = take_rows(c, T, K);
   w.bytes = c.used;
   return w;
 }
@@ -57,12 +79,12 @@ static FfnWs ffn_ws(void* ws, int T, int K, int nseg, int H, int I, int Is) {
   Carve c{static_cast<uint8_t*>(ws)};
   FfnWs w = {};
   const int64_t rows = nseg > 0 ? static_cast<int64_t>(T) * K : 0;
-  if (T > kF8InlineRows) {
+  if (T > kF8FewRows) {
+    w.x = take_rows(c, T, H);
     w.h = take_rows(c, rows, I);
     if (Is > 0) w.sh = take_rows(c, T, Is);
   }
-  if (T > SPARSE_HIP_DECODE_MAX_TOKENS) {
-    w.x = take_rows(c, T, H);
+  if (ffn_tiles(T, K, nseg, H, I, Is)) {
     w.tiles = c.take(prefill_merged_ws_bytes(T, K, nseg, H, I, Is));
   } else {
     w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
@@ -85,13 +107,18 @@ using namespace sparse;
 
 extern "C" {
 
+int sparse_hip_fp8_path(int which) {
+  SP_REQUIRE(which >= 0 && which <= 2, "fp8_path: %d outside [0,2]", which);
+  return g_path.exchange(which);
+}
+
 int sparse_hip_fp8_quantize(const void* x_dev, int dtype, int T, int K, void* values_dev, void* scales_dev, void* stream) {
   SP_REQUIRE(valid_dtype(dtype), "fp8_quantize: unknown dtype %d", dtype);
   SP_REQUIRE(T >= 0 && K >= 1 && K <= kF8MaxDim, "fp8_quantize: T=%d, K=%d outside [0,..] x [1,%d]", T, K, kF8MaxDim);
   if (T == 0) return SPARSE_HIP_OK;
   SP_REQUIRE(x_dev && values_dev && scales_dev, "fp8_quantize: NULL pointer");
   SP_REQUIRE(aligned16(values_dev), "fp8_quantize: values must be 16-byte aligned");
-  return f8_quantize(x_dev, dtype, T, K, values_dev, scales_dev, as_stream(stream));
+  return f8_quantize({x_dev, T, K, values_dev, scales_dev}, {}, dtype, as_stream(stream));
 }
 
 size_t sparse_hip_fp8_linear_ws_bytes(int T, int K) {
@@ -113,16 +140,15 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   SP_REQUIRE(out_dev != nullptr, "fp8_linear: NULL output");
   hipStream_t st = as_stream(stream);
   F8Product p = {};
-  const bool tiles = T > SPARSE_HIP_DECODE_MAX_TOKENS;
   int source = kF8From8;
   if (x_dev == nullptr) {
     SP_REQUIRE(xs_dev != nullptr && aligned16(xq_dev), "fp8_linear: 8-bit rows need scales and 16-byte alignment");
     p.act_s = static_cast<const uint8_t*>(xq_dev);
     p.act_ss = static_cast<const uint8_t*>(xs_dev);
-  } else if (tiles) {
+  } else if (T > kF8FewRows) {
     SP_REQUIRE(ws_dev != nullptr && aligned16(ws_dev), "fp8_linear: workspace is NULL or not 16-byte aligned");
     const LinearWs w = linear_ws(ws_dev, T, weight->cols);
-    rc = f8_quantize(x_dev, dtype, T, weight->cols, w.x.values, w.x.scales, st);
+    rc = f8_quantize({x_dev, T, weight->cols, w.x.values, w.x.scales}, {}, dtype, st);
     if (rc != SPARSE_HIP_OK) return rc;
     p.act_s = w.x.values;
     p.act_ss = w.x.scales;
@@ -140,7 +166,8 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   p.T = T;
   p.dtype = dtype;
   p.pow2 = pow2_scales;
-  return tiles ? f8_tile_linear(p, st) : f8_few(p, source, false, false, true, st);
+  if (T <= kF8FewRows) return f8_few(p, source, false, false, true, st);
+  return linear_tiles(T, weight->rows) ? f8_tile_linear(p, st) : f8_rows(p, false, false, true, st);
 }
 
 size_t sparse_hip_fp8_slot_bytes(int H, int I) {
@@ -202,15 +229,15 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   hipStream_t st = as_stream(stream);
   const FfnWs w = ffn_ws(ws_dev, T, K, segs->n, H, I, Is);
 
-  const bool tiles = T > SPARSE_HIP_DECODE_MAX_TOKENS, before = T > kF8InlineRows;
+  // One or two tokens: rows are quantised inside the products.  More: in launches of their own, beside products
+  // that stream weights; beside the tile kernel x only, which quantises the intermediate in its epilogue.
+  const bool few = T <= kF8FewRows, tiles = ffn_tiles(T, K, segs->n, H, I, Is);
   int rc = SPARSE_HIP_OK;
   PfQueues queues = {};
-  if (tiles) {
-    rc = f8_quantize(x_dev, dtype, T, H, w.x.values, w.x.scales, st);
-    if (rc == SPARSE_HIP_OK)
-      rc = prefill_queues(experts->expert_slot_dev, seg_offsets_dev, segs, T, K, H, I, Is, w.tiles, &queues, st);
-    if (rc != SPARSE_HIP_OK) return rc;
-  }
+  if (!few) rc = f8_quantize({x_dev, T, H, w.x.values, w.x.scales}, {}, dtype, st);
+  if (tiles && rc == SPARSE_HIP_OK)
+    rc = prefill_queues(experts->expert_slot_dev, seg_offsets_dev, segs, T, K, H, I, Is, w.tiles, &queues, st);
+  if (rc != SPARSE_HIP_OK) return rc;
   F8Product p = {};
   p.slab = static_cast<const uint8_t*>(experts->slab_dev);
   p.slot_stride = experts->slot_stride;
@@ -228,7 +255,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   p.off1 = slot.up;
   p.soff0 = slot.sgate;
   p.soff1 = slot.sup;
-  p.act_r = p.act_s = tiles ? w.x.values : static_cast<const uint8_t*>(x_dev);
+  p.act_r = p.act_s = few ? static_cast<const uint8_t*>(x_dev) : w.x.values;
   p.act_rs = p.act_ss = w.x.scales;
   p.gather = 1;
   p.out_r = w.hf;
@@ -245,17 +272,19 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   }
   if (tiles) {
     rc = f8_tile_gateup(p, queues, w.h.values, w.h.scales, w.sh.values, w.sh.scales, st);
-  } else {
+  } else if (few) {
     rc = f8_few(p, kF8From16, true, routed, shared, st);
-    if (before && rc == SPARSE_HIP_OK && routed)
-      rc = f8_quantize(w.hf, SPARSE_HIP_F32, static_cast<int64_t>(T) * K, I, w.h.values, w.h.scales, st);
-    if (before && rc == SPARSE_HIP_OK && shared) rc = f8_quantize(w.shf, SPARSE_HIP_F32, T, Is, w.sh.values, w.sh.scales, st);
+  } else {
+    rc = f8_rows(p, true, routed, shared, st);
+    if (rc == SPARSE_HIP_OK)
+      rc = f8_quantize({w.hf, routed ? static_cast<int64_t>(T) * K : 0, I, w.h.values, w.h.scales},
+                       {w.shf, shared ? T : 0, Is, w.sh.values, w.sh.scales}, SPARSE_HIP_F32, st);
   }
   if (rc != SPARSE_HIP_OK) return rc;
   // down: h -> rows times their route weight (shared expert: times sigmoid of its gate)
   p.off0 = p.off1 = slot.down;
   p.soff0 = p.soff1 = slot.sdown;
-  p.act_r = before ? w.h.values : reinterpret_cast<const uint8_t*>(w.hf);
+  p.act_r = few ? reinterpret_cast<const uint8_t*>(w.hf) : w.h.values;
   p.act_rs = w.h.scales;
   p.gather = 0;
   p.out_r = parts_dev;
@@ -264,14 +293,15 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   if (shared) {
     p.w0 = p.w1 = static_cast<const uint8_t*>(shared_down_w->values_dev);
     p.s0 = p.s1 = shared_down_w->scales_dev;
-    p.act_s = before ? w.sh.values : reinterpret_cast<const uint8_t*>(w.shf);
+    p.act_s = few ? reinterpret_cast<const uint8_t*>(w.shf) : w.sh.values;
     p.act_ss = w.sh.scales;
     p.gate_s = shared_gate_dev;
     p.out_s = shared_dev;
     p.Ks = Is;
     p.Ns = H;
   }
-  return tiles ? f8_tile_down(p, queues, st) : f8_few(p, before ? kF8From8 : kF8From32, false, routed, shared, st);
+  if (tiles) return f8_tile_down(p, queues, st);
+  return few ? f8_few(p, kF8From32, false, routed, shared, st) : f8_rows(p, false, routed, shared, st);
 }
 
 }  // extern "C"

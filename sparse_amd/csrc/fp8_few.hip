@@ -22,23 +22,13 @@ namespace sparse {
 
 constexpr int kFwThreads = 256;
 constexpr int kFwWaves = kFwThreads / 64;
-constexpr int kFwBatch = 3;       // runs a group of 16 lanes fetches at a time, after the first of a chunk
 constexpr int kSrc16 = kF8From16, kSrc32 = kF8From32, kSrc8 = kF8From8;
 
-// LDS row of a chunk: values, scales, and as much more as spreads 16 rows over the banks
-__host__ __device__ constexpr int fw_values(int kw) { return kFwWaves * kw * kF8Block * 2; }
-__host__ __device__ constexpr int fw_stride(int kw) { return fw_values(kw) + 80; }
-static_assert(kFwWaves * 2 * sizeof(float) <= 64, "the scales of a chunk fit behind its values");
-
-// Two e4m3 bytes (the low or the high half of `w`) as bf16, exactly; the wide forms of four and of eight.
-template <bool kHigh>
-__device__ __forceinline__ uint32_t fw_widen2(uint32_t w) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, kHigh));
-}
-__device__ __forceinline__ bf16x8 fw_widen8(uint32_t lo, uint32_t hi) {
-  const u32x4 v = {fw_widen2<false>(lo), fw_widen2<true>(lo), fw_widen2<false>(hi), fw_widen2<true>(hi)};
-  return __builtin_bit_cast(bf16x8, v);
-}
+constexpr int KW = 2;                             // blocks of a chunk per wavefront
+constexpr int KC = kFwWaves * KW;                 // blocks of a chunk
+constexpr int kFwValues = KC * kF8Block * 2;      // LDS row of a chunk: values, scales
+constexpr int kFwStride = kFwValues + KC * 4;
+static_assert(kFwThreads / 16 == kF8FewRows * KC, "one run of a chunk for each 16 lanes");
 
 // Eight values of a run, one sixteenth of it, on their way to LDS.
 __device__ __forceinline__ u32x4 fw_round(const float (&v)[8], float& scale) {
@@ -48,7 +38,7 @@ __device__ __forceinline__ u32x4 fw_round(const float (&v)[8], float& scale) {
   const int s = f8_exponent(f8_row16_max(m));
   const float inv = f8_inverse(s);
   scale = __uint_as_float(static_cast<uint32_t>(s + kF8Bias) << 23);
-  return __builtin_bit_cast(u32x4, fw_widen8(f8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+  return __builtin_bit_cast(u32x4, f8_widen8(f8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
                                              f8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)));
 }
 template <typename F, int kSrc>
@@ -103,15 +93,15 @@ struct Source<F, kSrc8> {
   }
   __device__ __forceinline__ u32x4 rounded(float& scale) const {
     scale = __uint_as_float(static_cast<uint32_t>(e) << 23);
-    return __builtin_bit_cast(u32x4, fw_widen8(v.x, v.y));
+    return __builtin_bit_cast(u32x4, f8_widen8(v.x, v.y));
   }
 };
 
-// kGateUp: the two matrices are gate and up, fp32 SwiGLU out.  Otherwise NM 16-row groups of one matrix.
-template <typename F, bool kGateUp, int NM, int NT, int KW, int kSrc>
+// kGateUp: NM = 2 matrices, gate and up, fp32 SwiGLU out.  Otherwise one.
+template <typename F, bool kGateUp, int NM, int kSrc>
 __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, int tiles_r, int tiles_s, int vec) {
-  constexpr int KC = kFwWaves * KW, kStride = fw_stride(KW);
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  constexpr int kStage = 2 * kF8FewRows * kFwStride, kSums = kFwWaves * NM * 64 * static_cast<int>(sizeof(vf32x4));
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kStage > kSums ? kStage : kSums];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, q = lane >> 4;
   const bool dense = static_cast<int>(blockIdx.x) < tiles_s;
@@ -150,58 +140,34 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
     s0 = reinterpret_cast<const float*>(slot + a.soff0);
     s1 = reinterpret_cast<const float*>(slot + a.soff1);
   }
-  const int m0 = blockIdx.y * 16 * NT;     // a dense call of more rows takes them in groups
-  M = min(M - m0, min(16 * NT, a.T));      // (a segment has at most T rows)
+  M = min(M, kF8FewRows);                   // (the ids of a token are distinct: a segment has T rows at most)
   if (M <= 0) return;
-  r0 += m0;
   const int nb = (K + kF8Block - 1) / kF8Block;
-  const int n0 = tile * 16 * (kGateUp ? 1 : NM);
+  const int n0 = tile * 16;
   const uint8_t* wp[NM];
   const float* sp[NM];
 #pragma unroll
   for (int mi = 0; mi < NM; ++mi) {
-    const int last16 = ((N + 15) & ~15) - 16;
-    const int n = kGateUp ? n0 : min(n0 + mi * 16, last16);   // behind the last group: computed, not stored
-    wp[mi] = (kGateUp && mi ? w1 : w0) + static_cast<size_t>(n >> 4) * nb * kF8TileBytes + lane * 16;
-    sp[mi] = (kGateUp && mi ? s1 : s0) + static_cast<size_t>(n / kF8Block) * nb;
+    wp[mi] = (mi ? w1 : w0) + static_cast<size_t>(tile) * nb * kF8TileBytes + lane * 16;
+    sp[mi] = (mi ? s1 : s0) + static_cast<size_t>(n0 / kF8Block) * nb;
   }
 
-  vf32x4 acc[NM][NT];
+  vf32x4 acc[NM];
 #pragma unroll
-  for (int mi = 0; mi < NM; ++mi)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) acc[mi][nt] = vf32x4{0.f, 0.f, 0.f, 0.f};
+  for (int mi = 0; mi < NM; ++mi) acc[mi] = vf32x4{0.f, 0.f, 0.f, 0.f};
 
   // The factor of the row whose sum this lane stores at the end, asked for now.
-  const int my_m = (wave / NM) * 16 + r;   // wavefront f stores fragment f = nt * NM + mi
   float factor = 1.f;
-  if (!kGateUp && wave < NT * NM && my_m < M) {
-    if (!dense) factor = F::from_bits(static_cast<const uint16_t*>(a.topv)[a.perm[r0 + my_m]]);
-    else if (a.gate_s != nullptr) factor = F::from_bits(static_cast<const uint16_t*>(a.gate_s)[r0 + my_m]);
+  if (!kGateUp && wave == 0 && r < M) {
+    if (!dense) factor = F::from_bits(static_cast<const uint16_t*>(a.topv)[a.perm[r0 + r]]);
+    else if (a.gate_s != nullptr) factor = F::from_bits(static_cast<const uint16_t*>(a.gate_s)[r0 + r]);
   }
 
   // ---- the chunks --------------------------------------------------------------------------
   // Two register stages in turn: while a chunk is multiplied the next one's loads are in flight.  Loads
   // complete in order, so a chunk's rows, which are wanted first, are requested before its weights; only the
   // first chunk's weights go ahead of its rows, whose addresses wait for the permutation.
-  const int group = threadIdx.x >> 4, gl = threadIdx.x & 15;
-  const int runs = M * KC;               // run i of a chunk: row i / KC, block i % KC
-  auto request = [&](int i, int c0) {    // runs past the end repeat the last row
-    const int m = min(i / KC, M - 1), kb = min(c0 + i % KC, nb - 1);
-    size_t row = r0 + m;
-    if (!dense && a.gather) row = static_cast<uint32_t>(a.perm[r0 + m]) / static_cast<uint32_t>(a.topk);
-    Source<F, kSrc> src;
-    src.load(dense ? a.act_s : a.act_r, dense ? a.act_ss : a.act_rs, row, K, nb, kb, gl * 8, vec != 0);
-    return src;
-  };
-  auto lay = [&](const Source<F, kSrc>& src, int i, uint8_t* buf) {
-    float scale;
-    const u32x4 out = src.rounded(scale);
-    if (i >= runs) return;
-    uint8_t* row = buf + (i / KC) * kStride;
-    *reinterpret_cast<u32x4*>(row + (i % KC) * (kF8Block * 2) + gl * 16) = out;
-    if (gl == 0) *reinterpret_cast<float*>(row + fw_values(KW) + (i % KC) * 4) = scale;
-  };
+  const int my_m = threadIdx.x / (16 * KC), my_kb = (threadIdx.x >> 4) % KC, gl = threadIdx.x & 15;
   struct Stage {
     i32x4 w[KW][NM][2];
     float ws[KW][NM];
@@ -221,56 +187,43 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
       }
     }
   };
-  auto load_rows = [&](Stage& st, int chunk) __attribute__((always_inline)) { st.src = request(group, chunk * KC); };
+  auto load_rows = [&](Stage& st, int chunk) __attribute__((always_inline)) {   // (a second row that is not there repeats the first)
+    const int m = min(my_m, M - 1), kb = min(chunk * KC + my_kb, nb - 1);
+    size_t row = r0 + m;
+    if (!dense && a.gather) row = static_cast<uint32_t>(a.perm[r0 + m]) / static_cast<uint32_t>(a.topk);
+    st.src.load(dense ? a.act_s : a.act_r, dense ? a.act_ss : a.act_rs, row, K, nb, kb, gl * 8, vec != 0);
+  };
   auto use = [&](const Stage& st, int chunk, uint8_t* buf) __attribute__((always_inline)) {
     const int c0 = chunk * KC;
-    lay(st.src, group, buf);
-    for (int p = 1; p * 16 < runs; p += kFwBatch) {     // more rows than the stage holds
-      Source<F, kSrc> more[kFwBatch];
-#pragma unroll
-      for (int j = 0; j < kFwBatch; ++j) more[j] = request((p + j) * 16 + group, c0);
-#pragma unroll
-      for (int j = 0; j < kFwBatch; ++j) lay(more[j], (p + j) * 16 + group, buf);
+    float scale;
+    const u32x4 rounded = st.src.rounded(scale);
+    if (my_m < M) {
+      uint8_t* row = buf + my_m * kFwStride;
+      *reinterpret_cast<u32x4*>(row + my_kb * (kF8Block * 2) + gl * 16) = rounded;
+      if (gl == 0) *reinterpret_cast<float*>(row + kFwValues + my_kb * 4) = scale;
     }
     __syncthreads();     // (the other buffer may still be read by a slower wavefront: this one is not)
 #pragma unroll
     for (int i = 0; i < KW; ++i) {
       const int kl = wave + i * kFwWaves;
       if (c0 + kl < nb) {
-        vf32x4 part[NM][NT];
+        const uint8_t* row = buf + min(r, M - 1) * kFwStride;    // columns past the rows are not stored
+        const uint8_t* values = row + kl * (kF8Block * 2) + q * 64;
+        F8Wide x;
 #pragma unroll
-        for (int mi = 0; mi < NM; ++mi)
+        for (int j = 0; j < 4; ++j) x.v[j] = *reinterpret_cast<const bf16x8*>(values + j * 16);
+        const float xs = *reinterpret_cast<const float*>(row + kFwValues + kl * 4);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) part[mi][nt] = vf32x4{0.f, 0.f, 0.f, 0.f};
+        for (int mi = 0; mi < NM; ++mi) {
+          const vf32x4 part = f8_mfma_wide(f8_widen(st.w[i][mi][0], st.w[i][mi][1]), x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {    // 32 k of the block: a lane's bytes 8 j .. 8 j + 7
-          bf16x8 b[NT];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            b[nt] = *reinterpret_cast<const bf16x8*>(buf + min(nt * 16 + r, M - 1) * kStride + kl * (kF8Block * 2) + q * 64 + j * 16);
-#pragma unroll
-          for (int mi = 0; mi < NM; ++mi) {
-            const i32x4 half = st.w[i][mi][j >> 1];
-            const bf16x8 wa = fw_widen8(half[2 * (j & 1)], half[2 * (j & 1) + 1]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              part[mi][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wa, b[nt], part[mi][nt], 0, 0, 0);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const float xs = *reinterpret_cast<const float*>(buf + min(nt * 16 + r, M - 1) * kStride + fw_values(KW) + kl * 4);
-#pragma unroll
-          for (int mi = 0; mi < NM; ++mi)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[mi][nt][j] = fmaf(part[mi][nt][j] * xs, st.ws[i][mi], acc[mi][nt][j]);
+          for (int j = 0; j < 4; ++j) acc[mi][j] = fmaf(part[j] * xs, st.ws[i][mi], acc[mi][j]);
         }
       }
     }
   };
   const int chunks = (nb + KC - 1) / KC;
-  const int buf_rows = min(a.T, 16 * NT);
-  uint8_t *const buf0 = lds, *const buf1 = lds + buf_rows * kStride;
+  uint8_t *const buf0 = lds, *const buf1 = lds + kF8FewRows * kFwStride;
   Stage s0_, s1_;
   load_weights(s0_, 0);
   __builtin_amdgcn_sched_barrier(0);
@@ -304,74 +257,39 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
   __syncthreads();
   vf32x4* red = reinterpret_cast<vf32x4*>(lds);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int mi = 0; mi < NM; ++mi) red[(wave * NT * NM + nt * NM + mi) * 64 + lane] = acc[mi][nt];
+  for (int mi = 0; mi < NM; ++mi) red[(wave * NM + mi) * 64 + lane] = acc[mi];
   __syncthreads();
-  auto sum = [&](int f) {
-    vf32x4 v = red[f * 64 + lane];
+  auto sum = [&](int mi) {
+    vf32x4 v = red[mi * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < kFwWaves; ++w) v += red[(w * NT * NM + f) * 64 + lane];
+    for (int w = 1; w < kFwWaves; ++w) v += red[(w * NM + mi) * 64 + lane];
     return v;
   };
+  if (wave != 0 || r >= M) return;
+  const int n = n0 + q * 4;
+  const size_t at = static_cast<size_t>(r0 + r) * N + n;
   if (kGateUp) {
-    for (int nt = wave; nt < NT; nt += kFwWaves) {
-      const int m = nt * 16 + r;
-      if (m >= M) continue;
-      const vf32x4 g = sum(nt * NM), u = sum(nt * NM + 1);
-      vf32x4 h;
+    const vf32x4 g = sum(0), u = sum(NM - 1);
+    vf32x4 h;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) h[j] = silu_f32(g[j]) * u[j];
-      *reinterpret_cast<vf32x4*>(static_cast<float*>(dense ? a.out_s : a.out_r) + static_cast<size_t>(r0 + m) * N + n0 + q * 4) = h;
-    }
-  } else {
-    static_assert(NT * NM <= kFwWaves, "one fragment per wavefront at most");
-    const int mi = wave % NM, m = my_m, n = n0 + mi * 16 + q * 4;
-    if (wave < NT * NM && m < M && n < N) {
-      const vf32x4 v = sum(wave);
-      const float sc = dense && a.gate_s != nullptr ? sigmoid_f32(factor) : factor;
-      uint16_t* o = static_cast<uint16_t*>(dense ? a.out_s : a.out_r) + static_cast<size_t>(r0 + m) * N + n;
-      uint2 pk;
-      pk.x = F::pack2(v[0] * sc, v[1] * sc);
-      pk.y = F::pack2(v[2] * sc, v[3] * sc);
-      if (N % 4 == 0 && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
-        *reinterpret_cast<uint2*>(o) = pk;
-      } else {
-        const uint32_t e[2] = {pk.x, pk.y};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < N) o[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
-      }
-    }
+    for (int j = 0; j < 4; ++j) h[j] = silu_f32(g[j]) * u[j];
+    *reinterpret_cast<vf32x4*>(static_cast<float*>(dense ? a.out_s : a.out_r) + at) = h;
+  } else if (n < N) {
+    const float sc = dense && a.gate_s != nullptr ? sigmoid_f32(factor) : factor;
+    f8_store4<F>(static_cast<uint16_t*>(dense ? a.out_s : a.out_r) + at, sum(0), sc, N, n);
   }
-}
-
-template <typename F, bool kGateUp, int NM, int NT, int KW, int kSrc>
-static int launch_few(const F8Product& p, int tiles_r, int tiles_s, int vec, hipStream_t st) {
-  const int64_t grid = tiles_s + static_cast<int64_t>(tiles_r) * p.segs.n;
-  const int64_t groups = tiles_r == 0 ? (p.T + 16 * NT - 1) / (16 * NT) : 1;
-  if (grid == 0) return SPARSE_HIP_OK;
-  SP_REQUIRE(grid < (1ll << 31) && groups < 65536, "fp8 product: grid too large");
-  const int rows = p.T < 16 * NT ? p.T : 16 * NT;
-  const int stage = 2 * rows * fw_stride(KW), red = kFwWaves * NM * NT * 64 * static_cast<int>(sizeof(vf32x4));
-  hipLaunchKernelGGL((f8_few_kernel<F, kGateUp, NM, NT, KW, kSrc>), dim3(static_cast<unsigned>(grid), static_cast<unsigned>(groups)),
-                     dim3(kFwThreads), static_cast<unsigned>(stage > red ? stage : red), st, p, tiles_r, tiles_s, vec);
-  SP_LAUNCH_CHECK("f8_few_kernel");
-  return SPARSE_HIP_OK;
 }
 
 template <typename F, bool kGateUp, int NM, int kSrc>
-static int few_by_rows(const F8Product& p, int tiles_r, int tiles_s, int vec, hipStream_t st) {
-  // A chunk is eight blocks, or four for 17 rows and more: two buffers of the rows then take 34 KB of LDS at
-  // most for 8 rows and 71 KB for 32.
-  if constexpr (kSrc == kSrc32) {
-    SP_REQUIRE(p.T <= 16, "fp8 product: %d rows of fp32", p.T);
-    return launch_few<F, kGateUp, NM, 1, 2, kSrc>(p, tiles_r, tiles_s, vec, st);
-  } else if (p.T <= 16) {
-    return launch_few<F, kGateUp, NM, 1, 2, kSrc>(p, tiles_r, tiles_s, vec, st);
-  } else {
-    return launch_few<F, kGateUp, NM, 2, 1, kSrc>(p, tiles_r, tiles_s, vec, st);
-  }
+static int launch_few(const F8Product& p, int tiles_r, int tiles_s, int vec, hipStream_t st) {
+  const int64_t grid = tiles_s + static_cast<int64_t>(tiles_r) * p.segs.n;
+  if (grid == 0) return SPARSE_HIP_OK;
+  SP_REQUIRE(grid < (1ll << 31), "fp8 product: grid too large");
+  SP_REQUIRE(p.T <= kF8FewRows, "fp8 product: %d rows", p.T);
+  hipLaunchKernelGGL((f8_few_kernel<F, kGateUp, NM, kSrc>), dim3(static_cast<unsigned>(grid)),
+                     dim3(kFwThreads), 0, st, p, tiles_r, tiles_s, vec);
+  SP_LAUNCH_CHECK("f8_few_kernel");
+  return SPARSE_HIP_OK;
 }
 
 template <typename F>
@@ -380,15 +298,10 @@ static int few_as(const F8Product& p, int source, bool gateup, bool routed, bool
   // 16-byte loads of the rows need aligned rows of a multiple of eight values
   const int K = dense ? p.Ks : p.Kr;
   const int vec = K % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.act_s) | reinterpret_cast<uintptr_t>(p.act_r)) & 15) == 0;
-  if (gateup) return few_by_rows<F, true, 2, kSrc16>(p, groups_r, groups_s, vec, st);
-  // Two 16-row groups per workgroup halve the rows' traffic; one keeps the device full when groups are few.
-  const bool two = groups_s + static_cast<int64_t>(groups_r) * (p.segs.n < p.T * p.topk ? p.segs.n : p.T * p.topk) >= 2048;
-  const int tr = two ? (groups_r + 1) / 2 : groups_r, ts = two ? (groups_s + 1) / 2 : groups_s;
-#define SP_FEW(S) (two ? few_by_rows<F, false, 2, S>(p, tr, ts, vec, st) : few_by_rows<F, false, 1, S>(p, tr, ts, vec, st))
-  if (source == kF8From16) return SP_FEW(kSrc16);
-  if (source == kF8From32) return SP_FEW(kSrc32);
-  return SP_FEW(kSrc8);
-#undef SP_FEW
+  if (gateup) return launch_few<F, true, 2, kSrc16>(p, groups_r, groups_s, vec, st);
+  if (source == kF8From16) return launch_few<F, false, 1, kSrc16>(p, groups_r, groups_s, vec, st);
+  if (source == kF8From32) return launch_few<F, false, 1, kSrc32>(p, groups_r, groups_s, vec, st);
+  return launch_few<F, false, 1, kSrc8>(p, groups_r, groups_s, vec, st);
 }
 
 int f8_few(const F8Product& p, int source, bool gateup, bool routed, bool dense, hipStream_t st) {

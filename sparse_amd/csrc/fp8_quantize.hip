@@ -7,16 +7,26 @@ constexpr int kQzThreads = 256;
 constexpr int kQzLane = 8;                       // values per lane: 16 lanes make a run
 constexpr int kQzRuns = kQzThreads * kQzLane / kF8Block;
 
+struct QuantizeArgs {
+  const void* x[2];
+  int64_t runs[2];
+  int32_t K[2], nb[2];
+  uint8_t *values[2], *scales[2];
+  uint32_t first_blocks;     // workgroups of the first matrix
+};
+
 // kVec: rows start on 16-byte boundaries and K is a multiple of 8
 template <typename T, bool kVec>
-__global__ __launch_bounds__(kQzThreads) void f8_quantize_kernel(const T* __restrict__ x, int64_t runs, int K, int nb,
-                                                                 uint8_t* __restrict__ values,
-                                                                 uint8_t* __restrict__ scales) {
-  const int64_t run = static_cast<int64_t>(blockIdx.x) * kQzRuns + (threadIdx.x >> 4);
-  if (run >= runs) return;                       // 16 lanes leave together
-  const int64_t t = run / nb;
+__global__ __launch_bounds__(kQzThreads) void f8_quantize_kernel(const QuantizeArgs a) {
+  const int which = blockIdx.x >= a.first_blocks;
+  const uint32_t block = blockIdx.x - (which ? a.first_blocks : 0u);
+  const int64_t run = static_cast<int64_t>(block) * kQzRuns + (threadIdx.x >> 4);
+  if (run >= a.runs[which]) return;              // 16 lanes leave together
+  const int K = a.K[which], nb = a.nb[which];
+  // (a row's number fits 32 bits; so does almost every run's, and the short division is several times faster)
+  const int64_t t = run < (1ll << 32) ? static_cast<uint32_t>(run) / static_cast<uint32_t>(nb) : run / nb;
   const int k = static_cast<int>(run - t * nb) * kF8Block + (threadIdx.x & 15) * kQzLane;
-  const T* row = x + t * K;
+  const T* row = static_cast<const T*>(a.x[which]) + t * K;
   float v[kQzLane];
   if (kVec) {
     // a multiple of 8: a lane's eight values are all inside the row or all behind it
@@ -41,30 +51,40 @@ __global__ __launch_bounds__(kQzThreads) void f8_quantize_kernel(const T* __rest
   uint2 q;
   q.x = f8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
   q.y = f8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-  *reinterpret_cast<uint2*>(values + t * nb * kF8Block + k) = q;
-  if ((threadIdx.x & 15) == 0) scales[run] = static_cast<uint8_t>(s + kF8Bias);
+  *reinterpret_cast<uint2*>(a.values[which] + t * nb * kF8Block + k) = q;
+  if ((threadIdx.x & 15) == 0) a.scales[which][run] = static_cast<uint8_t>(s + kF8Bias);
 }
 
 template <typename T>
-static int quantize_as(const void* x, int64_t Trows, int K, void* values, void* scales, hipStream_t st) {
-  const int nb = f8_blocks(K);
-  const int64_t runs = Trows * nb, grid = (runs + kQzRuns - 1) / kQzRuns;
-  SP_REQUIRE(grid < (1ll << 31), "fp8_quantize: too many rows");
-  const bool vec = K % kQzLane == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  if (vec)
-    hipLaunchKernelGGL((f8_quantize_kernel<T, true>), dim3(static_cast<unsigned>(grid)), dim3(kQzThreads), 0, st,
-                       static_cast<const T*>(x), runs, K, nb, static_cast<uint8_t*>(values), static_cast<uint8_t*>(scales));
-  else
-    hipLaunchKernelGGL((f8_quantize_kernel<T, false>), dim3(static_cast<unsigned>(grid)), dim3(kQzThreads), 0, st,
-                       static_cast<const T*>(x), runs, K, nb, static_cast<uint8_t*>(values), static_cast<uint8_t*>(scales));
+static int quantize_as(const F8Quantize& a, const F8Quantize& b, hipStream_t st) {
+  QuantizeArgs q = {};
+  int64_t blocks[2];
+  bool vec = true;
+  for (int i = 0; i < 2; ++i) {
+    const F8Quantize& m = i ? b : a;
+    q.x[i] = m.x;
+    q.K[i] = m.K;
+    q.nb[i] = f8_blocks(m.K);
+    q.runs[i] = m.T * q.nb[i];
+    q.values[i] = static_cast<uint8_t*>(m.values);
+    q.scales[i] = static_cast<uint8_t*>(m.scales);
+    blocks[i] = (q.runs[i] + kQzRuns - 1) / kQzRuns;
+    vec = vec && m.K % kQzLane == 0 && (reinterpret_cast<uintptr_t>(m.x) & 15) == 0;
+  }
+  SP_REQUIRE(blocks[0] + blocks[1] < (1ll << 31), "fp8_quantize: too many rows");
+  if (blocks[0] + blocks[1] == 0) return SPARSE_HIP_OK;
+  q.first_blocks = static_cast<uint32_t>(blocks[0]);
+  const dim3 grid(static_cast<unsigned>(blocks[0] + blocks[1]));
+  if (vec) hipLaunchKernelGGL((f8_quantize_kernel<T, true>), grid, dim3(kQzThreads), 0, st, q);
+  else hipLaunchKernelGGL((f8_quantize_kernel<T, false>), grid, dim3(kQzThreads), 0, st, q);
   SP_LAUNCH_CHECK("f8_quantize_kernel");
   return SPARSE_HIP_OK;
 }
 
-int f8_quantize(const void* x, int dtype, int64_t Trows, int K, void* values, void* scales, hipStream_t st) {
-  if (dtype == SPARSE_HIP_BF16) return quantize_as<uint16_t>(x, Trows, K, values, scales, st);
-  if (dtype == SPARSE_HIP_F16) return quantize_as<f16_t>(x, Trows, K, values, scales, st);
-  return quantize_as<float>(x, Trows, K, values, scales, st);
+int f8_quantize(const F8Quantize& a, const F8Quantize& b, int dtype, hipStream_t st) {
+  if (dtype == SPARSE_HIP_BF16) return quantize_as<uint16_t>(a, b, st);
+  if (dtype == SPARSE_HIP_F16) return quantize_as<f16_t>(a, b, st);
+  return quantize_as<float>(a, b, st);
 }
 
 }  // namespace sparse

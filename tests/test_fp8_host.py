@@ -143,8 +143,8 @@ def test_quantize_and_linear_refusals():
     refused(lin(x=None), "give x or")
     refused(lin(xq=P, xs=P), "give x or")
     refused(lin(out=None), "NULL output")
-    refused(lin(ws=None), "workspace")
-    refused(lin(ws=P + 4), "workspace")
+    refused(lin(T=3, ws=None), "workspace")
+    refused(lin(T=3, ws=P + 4), "workspace")
     refused(lin(x=None, xq=P), "scales")
     assert lin(T=0) == 0
 

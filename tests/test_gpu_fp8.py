@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import ref_fp8
-from sparse_amd import fp8, ops
+from sparse_amd import _lib, fp8, ops
 
 pytestmark = pytest.mark.gpu
 HALF = [torch.bfloat16, torch.float16]
@@ -23,8 +23,22 @@ def within(got, want, bound, dtype):
 
 
 def grouped(T):
-    """Calls of up to 32 tokens add products in fp32, larger ones in the 8-bit instruction's groups."""
-    return T > 32
+    """Calls of one or two rows add products in fp32, larger ones in the 8-bit instruction's groups."""
+    return T > 2
+
+
+@pytest.fixture(params=["stream", "tiles"])
+def path(request):
+    """Both families of kernels, whatever the size would choose."""
+    lib = _lib.load()
+    before = lib.sparse_hip_fp8_path({"stream": 1, "tiles": 2}[request.param])
+    yield request.param
+    lib.sparse_hip_fp8_path(before)
+
+
+def grouped_gate_up(T, path):
+    """Only the tiles take gate and up projections in the 8-bit instruction."""
+    return T > 2 and path == "tiles"
 
 
 def rand_rows(T, K, dtype, seed=0):
@@ -116,7 +130,7 @@ SIZES = [(1, 128, 16), (1, 1, 1), (2, 64, 17), (15, 130, 100), (16, 127, 130), (
 
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("T,K,N", SIZES)
-def test_linear(device, dtype, T, K, N):
+def test_linear(path, device, dtype, T, K, N):
     for pow2 in (False, True):
         x, (q, s) = rand_rows(T, K, dtype), rand_weight(N, K, pow2=pow2)
         w = fp8.Weight.from_quantized(q.to(device), s.to(device))
@@ -130,7 +144,7 @@ def test_linear(device, dtype, T, K, N):
 
 
 @pytest.mark.parametrize("T", [1, 7, 40])
-def test_linear_far_from_one(device, T):
+def test_linear_far_from_one(path, device, T):
     """Rows near both ends of the range, runs whose scale is the lowest."""
     x = torch.randn(T, 300, generator=torch.Generator().manual_seed(T))
     q, s = rand_weight(48, 300)
@@ -141,7 +155,7 @@ def test_linear_far_from_one(device, T):
 
 
 @pytest.mark.parametrize("T", [1, 18])
-def test_linear_large_weight(device, T):
+def test_linear_large_weight(path, device, T):
     K, N = 2048, 5632
     g = torch.Generator(device=device).manual_seed(3)
     q = (torch.randn(N, K, generator=g, device=device) * 60).to(fp8.E4M3)
@@ -151,7 +165,7 @@ def test_linear_large_weight(device, T):
     within(fp8.linear(x.to(device), fp8.Weight.from_quantized(q, s)), want, bound, torch.bfloat16)
 
 
-def test_linear_nan_stays_in_its_row(device):
+def test_linear_nan_stays_in_its_row(path, device):
     q, s = rand_weight(64, 256)
     w = fp8.Weight.from_quantized(q.to(device), s.to(device))
     for T in (4, 200):
@@ -164,7 +178,7 @@ def test_linear_nan_stays_in_its_row(device):
         assert torch.equal(y[rest], clean[rest])
 
 
-def test_linear_row_does_not_depend_on_its_neighbours(device):
+def test_linear_row_does_not_depend_on_its_neighbours(path, device):
     """Within one size class of calls a row's bits do not depend on the other rows."""
     q, s = rand_weight(160, 640)
     w = fp8.Weight.from_quantized(q.to(device), s.to(device))
@@ -173,7 +187,7 @@ def test_linear_row_does_not_depend_on_its_neighbours(device):
     assert torch.equal(fp8.linear(x.flip(0).contiguous(), w), y.flip(0))
 
 
-def test_linear_writes_only_its_output(device):
+def test_linear_writes_only_its_output(path, device):
     q, s = rand_weight(33, 200)
     w = fp8.Weight.from_quantized(q.to(device), s.to(device))
     for T in (1, 5, 140):
@@ -215,8 +229,8 @@ def on_gpu(c, device):
     return dict(slab=slab, x=dev(c["x"]), topv=dev(c["topv"]), topi=topi, perm=ops.permute_build(topi, c["E"]), sh=sh, sg=dev(c["sg"]))
 
 
-def oracle(c):
-    return ref_fp8.experts(c["x"], c["topi"], c["topv"], c["ex"], c["sh"], c["sg"], grouped(c["x"].shape[0]))
+def oracle(c, path):
+    return ref_fp8.experts(c["x"], c["topi"], c["topv"], c["ex"], c["sh"], c["sg"], grouped_gate_up(len(c["x"]), path), grouped(len(c["x"])))
 
 
 CASES = [  # T, H, E, I, K, Is, gate
@@ -229,12 +243,12 @@ CASES = [  # T, H, E, I, K, Is, gate
 
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("case", CASES)
-def test_experts(device, dtype, case):
+def test_experts(path, device, dtype, case):
     for pow2 in (False, True):
         c = make_case(*case, dtype, pow2=pow2)
         d = on_gpu(c, device)
         parts, shared = fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"], shared=d["sh"], shared_gate=d["sg"])
-        want, bound, wsh, bsh = oracle(c)
+        want, bound, wsh, bsh = oracle(c, path)
         within(parts, want, bound, dtype)
         if c["sh"]:
             within(shared, wsh, bsh, dtype)
@@ -243,19 +257,19 @@ def test_experts(device, dtype, case):
 
 
 @pytest.mark.parametrize("T", [3, 40])
-def test_every_token_on_the_same_experts(device, T):
+def test_every_token_on_the_same_experts(path, device, T):
     """Segments as long as the call beside empty ones.  (The ids of one token are distinct: the permutation
     build keeps one bit per token and expert.)"""
     for topi in (torch.zeros(T, 1, dtype=torch.int64) + 2, torch.tensor([[5, 1, 4]]).repeat(T, 1)):
         c = make_case(T, 128, 6, 128, topi.shape[1], 0, False, torch.bfloat16, topi=topi)
         d = on_gpu(c, device)
         parts, _ = fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"])
-        want, bound, _, _ = oracle(c)
+        want, bound, _, _ = oracle(c, path)
         within(parts, want, bound, torch.bfloat16)
 
 
 @pytest.mark.parametrize("T", [5, 90])
-def test_host_segments_touch_only_their_rows(device, T):
+def test_host_segments_touch_only_their_rows(path, device, T):
     c = make_case(T, 128, 8, 192, 3, 0, False, torch.bfloat16)
     d = on_gpu(c, device)
     full, _ = fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"])
@@ -279,7 +293,7 @@ def test_host_segments_touch_only_their_rows(device, T):
 
 
 @pytest.mark.parametrize("T", [4, 70])
-def test_shared_expert_alone(device, T):
+def test_shared_expert_alone(path, device, T):
     c = make_case(T, 192, 4, 64, 2, 320, True, torch.float16)
     d = on_gpu(c, device)
     _, both = fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"], shared=d["sh"], shared_gate=d["sg"])
@@ -288,7 +302,7 @@ def test_shared_expert_alone(device, T):
 
 
 @pytest.mark.parametrize("T", [1, 6, 50])
-def test_experts_in_a_graph_and_on_another_stream(device, T):
+def test_experts_in_a_graph_and_on_another_stream(path, device, T):
     c = make_case(T, 256, 8, 128, 2, 192, True, torch.bfloat16)
     d = on_gpu(c, device)
 
@@ -318,7 +332,7 @@ def test_experts_in_a_graph_and_on_another_stream(device, T):
             assert all(torch.equal(a, b) for a, b in zip(out, eager))
 
 
-def test_the_operators_together(device):
+def test_the_operators_together(path, device):
     """Gate, permutation, experts and combine as a layer runs them, against the same chain in 64 bits."""
     for T in (1, 9, 120):
         c = make_case(T, 256, 16, 192, 4, 256, True, torch.bfloat16, seed=11)
@@ -334,7 +348,7 @@ def test_the_operators_together(device):
         _, ref_i = ref_fp8.gate_select(logits, 4, bias=bias, **kw)
         assert torch.equal(topi.cpu(), ref_i)
         c["topi"], c["topv"] = ref_i, topv.cpu()
-        want, bound, wsh, bsh = oracle(c)
+        want, bound, wsh, bsh = oracle(c, path)
         inv = perm.inv_perm.cpu().long().view(T, 4)
         total, slack = wsh.clone(), bsh + ref_fp8.half_step(torch.bfloat16, wsh.abs() + bsh)
         mag = wsh.abs() + slack
@@ -355,7 +369,7 @@ def test_no_tokens(device):
 
 
 @pytest.mark.parametrize("T", [1, 33])
-def test_linear_long_rows(device, T):
+def test_linear_long_rows(path, device, T):
     """The longest rows: a scale for each of 512 runs."""
     K, N = 65536, 16
     q, s = rand_weight(N, K)
