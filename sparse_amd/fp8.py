@@ -21,7 +21,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import Fp8Matrix, SegList
-from .ops import HALF_DTYPES, Permutation, _need, _need_half, _ptr, dtype_code, on_device
+from .ops import HALF_DTYPES, Permutation, _need, _need_half, _ptr, _same_device, call_on, dtype_code
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
@@ -49,7 +49,7 @@ class Rows:
     @property
     def values(self) -> torch.Tensor:
         """The ``[T, K]`` values without the padding."""
-        return self.data[:, :self.cols]
+        return self.data if self.data.shape[1] == self.cols else self.data[:, :self.cols]
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         full = self.data.float().view(*self.scales.shape, BLOCK) * self.scales.float()[..., None]
@@ -64,15 +64,17 @@ def quantize(x: torch.Tensor, out: Optional[Rows] = None) -> Rows:
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must be [T, K] with K >= 1, got {tuple(x.shape)}")
     T, K = x.shape
-    code = dtype_code(x.dtype)
+    code, index = dtype_code(x.dtype), x.get_device()
     if out is None:
-        out = Rows(x.new_empty((T, padded(K)), dtype=E4M3), x.new_empty((T, blocks(K)), dtype=E8M0), K, x.dtype)
+        nb = -(-K // BLOCK)
+        out = Rows(x.new_empty((T, nb * BLOCK), dtype=E4M3), x.new_empty((T, nb), dtype=E8M0), K, x.dtype)
     else:
         _need(out.data, "values", E4M3, (T, padded(K)))
         _need(out.scales, "scales", E8M0, (T, blocks(K)))
         out.cols, out.dtype = K, x.dtype
-    with on_device(x, out.data, out.scales) as stream:
-        rc = _lib.load().sparse_hip_fp8_quantize(_ptr(x), code, T, K, _ptr(out.data), _ptr(out.scales), stream)
+        _same_device(index, out.data, out.scales)
+    rc = call_on(index, _lib.load().sparse_hip_fp8_quantize, x.data_ptr(), code, T, K, out.data.data_ptr(),
+                 out.scales.data_ptr())
     _lib.check(rc, "sparse_hip_fp8_quantize")
     return out
 
@@ -139,12 +141,13 @@ def are_pow2(scales: torch.Tensor) -> bool:
 class Weight:
     """A matrix ``[rows, cols]`` laid out for the kernels, with its block scales."""
 
-    __slots__ = ("data", "scales", "rows", "cols", "pow2", "desc")
+    __slots__ = ("data", "scales", "rows", "cols", "pow2", "desc", "ref")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> None:
         self.data, self.scales, self.rows, self.cols = data, scales, int(rows), int(cols)
         self.pow2 = are_pow2(scales)
         self.desc = Fp8Matrix(data.data_ptr(), scales.data_ptr(), self.rows, self.cols)
+        self.ref = C.byref(self.desc)
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -170,33 +173,36 @@ class Weight:
 def linear(x: Union[torch.Tensor, Rows], weight: Weight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x W^T`` with ``x [T, K]`` (bf16 or fp16) quantised inside the call, or given as ``Rows`` of such an x:
     ``[T, N]`` in x's dtype, accumulated in fp32 and rounded once."""
-    rows = x if isinstance(x, Rows) else None
-    src = x.data if rows is not None else x
+    dtype = x.dtype
+    if dtype not in HALF_DTYPES:
+        raise ValueError(f"x must be bfloat16 or float16, got {dtype}")
+    rows = type(x) is Rows
+    src = x.data if rows else x
     _need(src, "x")
-    if x.dtype not in HALF_DTYPES:
-        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
     if src.dim() != 2:
         raise ValueError(f"x must be [T, K], got {tuple(src.shape)}")
-    T, K = src.shape[0], (rows.cols if rows is not None else src.shape[1])
+    T, K = src.shape
+    if rows:
+        K = x.cols
+        _need(src, "values", E4M3, (T, padded(K)))
+        _need(x.scales, "scales", E8M0, (T, blocks(K)))
     if K != weight.cols:
         raise ValueError(f"x has {K} columns, the weight {weight.cols}")
-    dtype = x.dtype
-    code = dtype_code(dtype)
+    index = src.get_device()
     if out is None:
         out = src.new_empty((T, weight.rows), dtype=dtype)
     else:
         _need(out, "out", dtype, (T, weight.rows))
+    _same_device(index, weight.data, out)
     lib = _lib.load()
-    with on_device(src, weight.data, out) as stream:
-        if rows is not None:
-            _need(rows.data, "values", E4M3, (T, padded(K)))
-            _need(rows.scales, "scales", E8M0, (T, blocks(K)))
-            rc = lib.sparse_hip_fp8_linear(None, _ptr(rows.data), _ptr(rows.scales), code, T, C.byref(weight.desc),
-                                           int(weight.pow2), _ptr(out), None, stream)
-        else:
-            ws = src.new_empty((max(1, lib.sparse_hip_fp8_linear_ws_bytes(T, K)),), dtype=torch.uint8)
-            rc = lib.sparse_hip_fp8_linear(_ptr(src), None, None, code, T, C.byref(weight.desc), int(weight.pow2),
-                                           _ptr(out), _ptr(ws), stream)
+    if rows:
+        rc = call_on(index, lib.sparse_hip_fp8_linear, None, src.data_ptr(), x.scales.data_ptr(), dtype_code(dtype), T,
+                     weight.ref, weight.pow2, out.data_ptr(), None)
+    else:
+        need = lib.sparse_hip_fp8_linear_ws_bytes(T, K)       # 0: the product quantises its rows itself
+        ws = src.new_empty((need,), dtype=torch.uint8) if need else None
+        rc = call_on(index, lib.sparse_hip_fp8_linear, src.data_ptr(), None, None, dtype_code(dtype), T, weight.ref,
+                     weight.pow2, out.data_ptr(), _ptr(ws))
     _lib.check(rc, "sparse_hip_fp8_linear")
     return out
 
@@ -237,6 +243,7 @@ class ExpertSlab:
         self.num_slots, self.num_experts = int(num_slots), int(num_experts)
         self.expert_bytes = slot_bytes(hidden, inter)
         self.data = torch.empty((self.num_slots, self.expert_bytes), dtype=torch.uint8, device=device)
+        self._refs: dict = {}
         self.pow2 = False       # whether every scale of the slots in use is a power of two
         self.expert_slot = torch.arange(self.num_experts, dtype=torch.int32, device=device)
 
@@ -258,9 +265,14 @@ class ExpertSlab:
     def slot_ptr(self, slot: int) -> int:
         return self.data.data_ptr() + int(slot) * self.expert_bytes
 
-    def descriptor(self, dtype: torch.dtype) -> _lib.Experts:
-        return _lib.Experts(self.data.data_ptr(), self.expert_bytes, self.expert_slot.data_ptr(), self.num_experts,
-                            self.hidden, self.inter, dtype_code(dtype))
+    def descriptor(self, dtype: torch.dtype):
+        """The slab as the C entry takes it, for activations of ``dtype``; built once per dtype."""
+        ref = self._refs.get(dtype)
+        if ref is None:
+            ref = C.byref(_lib.Experts(self.data.data_ptr(), self.expert_bytes, self.expert_slot.data_ptr(),
+                                       self.num_experts, self.hidden, self.inter, dtype_code(dtype)))
+            self._refs[dtype] = ref
+        return ref
 
 
 def moe_ffn_ws_bytes(T: int, K: int, num_segments: int, hidden: int, inter: int, shared_inter: int = 0) -> int:
@@ -283,25 +295,29 @@ def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Perm
         raise ValueError("x must be [T, H] and topv [T, K]")
     T, H = x.shape
     K = topv.shape[1]
-    dtype = x.dtype
+    dtype, E, index = x.dtype, experts.num_experts, x.get_device()
     if H != experts.hidden:
         raise ValueError(f"x has hidden {H}, the expert slab has {experts.hidden}")
     _need(topv, "topv", dtype, (T, K))
-    if perm.perm.numel() != T * K or perm.seg_offsets.numel() != experts.num_experts + 1:
-        raise ValueError(f"the permutation does not belong to {T} tokens x {K} over {experts.num_experts} experts")
+    if perm.perm.numel() != T * K or perm.seg_offsets.numel() != E + 1:
+        raise ValueError(f"the permutation does not belong to {T} tokens x {K} over {E} experts")
     if segs is None:
-        segs = ops.seglist_device(perm, min(experts.num_experts, T * K))
+        segs = ops.seglist_device(perm, min(E, T * K))
     if parts is None:
         parts = x.new_empty((T * K, H))
     else:
         _need(parts, "parts", dtype, (T * K, H))
-    mats, Is = (None, None, None), 0
+    gate = up = down = None
+    Is, pow2 = 0, experts.pow2
     if shared is not None:
-        Is = shared[2].cols
-        for m, want, name in zip(shared, ((Is, H), (Is, H), (H, Is)), ("gate_proj", "up_proj", "down_proj")):
-            if m.shape != want:
+        gate, up, down = shared
+        Is = down.cols
+        for m, want, name in ((gate, (Is, H), "gate_proj"), (up, (Is, H), "up_proj"), (down, (H, Is), "down_proj")):
+            if (m.rows, m.cols) != want:
                 raise ValueError(f"shared {name} must be {want}, got {m.shape}")
-        mats = tuple(C.byref(m.desc) for m in shared)
+            pow2 = pow2 and m.pow2
+        _same_device(index, gate.data, up.data, down.data)
+        gate, up, down = gate.ref, up.ref, down.ref
         if shared_gate is not None:
             _need(shared_gate, "shared gate logits", dtype)
             if shared_gate.numel() != T:
@@ -312,20 +328,17 @@ def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Perm
             _need(shared_out, "shared out", dtype, (T, H))
     else:
         shared_gate = shared_out = None
+    if T == 0:
+        return parts, shared_out
     lib = _lib.load()
-    pow2 = int(experts.pow2 and (shared is None or all(m.pow2 for m in shared)))
     need = lib.sparse_hip_fp8_moe_ffn_ws_bytes(T, K, segs.n, H, experts.inter, Is)
-    with on_device(x, topv, perm.perm, experts.data, parts, shared_gate, shared_out, ws,
-                   None if shared is None else shared[0].data) as stream:
-        if ws is None:
-            ws = x.new_empty((max(1, need),), dtype=torch.uint8)
-        elif not ws.is_contiguous() or ws.numel() * ws.element_size() < need:
-            raise ValueError(f"the workspace must hold {need} contiguous bytes")
-        if T == 0:
-            return parts, shared_out
-        desc = experts.descriptor(dtype)
-        rc = lib.sparse_hip_fp8_moe_ffn(C.byref(desc), _ptr(x), _ptr(topv), _ptr(perm.perm), _ptr(perm.seg_offsets),
-                                        C.byref(segs), T, K, _ptr(parts), *mats, _ptr(shared_gate), pow2,
-                                        _ptr(shared_out), _ptr(ws), stream)
+    if ws is None:
+        ws = x.new_empty((max(1, need),), dtype=torch.uint8)
+    elif not ws.is_contiguous() or ws.numel() * ws.element_size() < need:
+        raise ValueError(f"the workspace must hold {need} contiguous bytes")
+    _same_device(index, topv, perm.perm, experts.data, parts, shared_gate, shared_out, ws)
+    rc = call_on(index, lib.sparse_hip_fp8_moe_ffn, experts.descriptor(dtype), x.data_ptr(), topv.data_ptr(),
+                 perm.perm.data_ptr(), perm.seg_offsets.data_ptr(), C.byref(segs), T, K, parts.data_ptr(), gate, up, down,
+                 _ptr(shared_gate), pow2, _ptr(shared_out), ws.data_ptr())
     _lib.check(rc, "sparse_hip_fp8_moe_ffn")
     return parts, shared_out

@@ -55,27 +55,23 @@ def _need(t: torch.Tensor, name: str, dtype=None, shape=None) -> None:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-class on_device:
-    """``with on_device(*tensors) as stream``: the tensors' device is the current one inside, ``stream`` is
-    its current stream.  Tensors on different devices are refused."""
+# the stream handle without building a Stream object around it (0.1 instead of 1.1 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-    __slots__ = ("index", "previous")
 
-    def __init__(self, *tensors: Optional[torch.Tensor]) -> None:
-        self.index = self.previous = tensors[0].get_device()
-        for t in tensors:
-            if t is not None and t.get_device() != self.index:
-                raise ValueError(f"tensors are on different devices: cuda:{self.index} and {t.device}")
+def call_on(index: int, fn, *args) -> int:
+    """``fn(*args, stream)`` with device ``index`` current, on its current stream."""
+    if torch.cuda.current_device() == index:
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
 
-    def __enter__(self) -> int:
-        self.previous = torch.cuda.current_device()
-        if self.previous != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
 
-    def __exit__(self, *exc) -> None:
-        if self.previous != self.index:
-            torch.cuda.set_device(self.previous)
+def _same_device(index: int, *tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors are on different devices: cuda:{index} and {t.device}")
 
 
 # --------------------------------------------------------------------------- router
@@ -157,9 +153,9 @@ def gate_select(logits: torch.Tensor, k: int, score: str = "softmax", bias: Opti
     T, E = logits.shape
     k = int(k)
     odt = out_dtype or logits.dtype
+    index = logits.get_device()
     if bias is not None:
         _need(bias, "bias", torch.float32, (E,))
-    ldt, ocode = dtype_code(logits.dtype), dtype_code(odt)
     if topv is None:
         topv = logits.new_empty((T, max(0, k)), dtype=odt)
     else:
@@ -168,10 +164,10 @@ def gate_select(logits: torch.Tensor, k: int, score: str = "softmax", bias: Opti
         topi = logits.new_empty((T, max(0, k)), dtype=torch.int64)
     else:
         _need(topi, "topi", torch.int64, (T, k))
-    with on_device(logits, bias, topv, topi) as stream:
-        rc = _lib.load().sparse_hip_gate_select(_ptr(logits), ldt, _ptr(bias), T, E, k, SELECT_SCORE[score], int(n_group),
-                                                int(topk_group), SELECT_GROUP[group_score], int(bool(renorm)), float(scale),
-                                                ocode, _ptr(topv), _ptr(topi), stream)
+    _same_device(index, bias, topv, topi)
+    rc = call_on(index, _lib.load().sparse_hip_gate_select, logits.data_ptr(), dtype_code(logits.dtype), _ptr(bias), T, E, k,
+                 SELECT_SCORE[score], n_group, topk_group, SELECT_GROUP[group_score], bool(renorm), scale, dtype_code(odt),
+                 topv.data_ptr(), topi.data_ptr())
     _lib.check(rc, "sparse_hip_gate_select")
     return topv, topi
 
