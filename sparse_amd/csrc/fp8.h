@@ -145,6 +145,9 @@ struct F8Quantize {
   void *values, *scales;
 };
 int f8_quantize(const F8Quantize& a, const F8Quantize& b, int dtype, hipStream_t st);
+// one matrix, and in the same launch the tile queues of its call
+struct PfxMapArgs;
+int f8_quantize_and_queue(const F8Quantize& a, int dtype, const PfxMapArgs& queue, hipStream_t st);
 
 // One matrix product of a call, over the routed segments of an expert slab, a dense matrix, or both.
 struct F8Product {
@@ -177,11 +180,8 @@ int f8_few(const F8Product& p, int source, bool gateup, bool routed, bool dense,
 int f8_rows(const F8Product& p, bool gateup, bool routed, bool dense, hipStream_t st);
 
 // The same for many rows, 16-bit formats: 128 x 256 tiles.  gate/up writes quantised rows; routed and dense
-// tiles come from one set of queues (prefill_queues, which builds them).
+// tiles come from one set of queues.
 struct PfQueues;
-int prefill_queues(const int32_t* expert_slot, const int32_t* seg_offsets, const sparse_hip_seglist* segs, int T, int K,
-                   int H, int I, int Is, void* tile_ws, PfQueues* q, hipStream_t st);
-size_t prefill_merged_ws_bytes(int T, int K, int nseg, int H, int I, int Is);
 int f8_tile_gateup(const F8Product& p, const PfQueues& q, void* h, void* hs, void* sh, void* shs, hipStream_t st);
 int f8_tile_down(const F8Product& p, const PfQueues& q, hipStream_t st);
 int f8_tile_linear(const F8Product& p, hipStream_t st);

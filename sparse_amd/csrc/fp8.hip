@@ -2,7 +2,7 @@
 #include <atomic>
 
 #include "fp8.h"
-#include "prefill_tiles.h"
+#include "prefill_queue.h"
 
 namespace sparse {
 
@@ -85,7 +85,7 @@ static FfnWs ffn_ws(void* ws, int T, int K, int nseg, int H, int I, int Is) {
     if (Is > 0) w.sh = take_rows(c, T, Is);
   }
   if (ffn_tiles(T, K, nseg, H, I, Is)) {
-    w.tiles = c.take(prefill_merged_ws_bytes(T, K, nseg, H, I, Is));
+    w.tiles = c.take(prefill_queue_ws_bytes(T, K, nseg, H, I, Is));
   } else {
     w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
     if (Is > 0) w.shf = static_cast<float*>(c.take(static_cast<size_t>(T) * Is * sizeof(float)));
@@ -234,9 +234,13 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   const bool few = T <= kF8FewRows, tiles = ffn_tiles(T, K, segs->n, H, I, Is);
   int rc = SPARSE_HIP_OK;
   PfQueues queues = {};
-  if (!few) rc = f8_quantize({x_dev, T, H, w.x.values, w.x.scales}, {}, dtype, st);
-  if (tiles && rc == SPARSE_HIP_OK)
-    rc = prefill_queues(experts->expert_slot_dev, seg_offsets_dev, segs, T, K, H, I, Is, w.tiles, &queues, st);
+  if (tiles) {
+    PfxMapArgs queue_args;
+    queues = prefill_queue_args(experts->expert_slot_dev, seg_offsets_dev, *segs, T, K, H, I, Is, w.tiles, &queue_args);
+    rc = f8_quantize_and_queue({x_dev, T, H, w.x.values, w.x.scales}, dtype, queue_args, st);
+  } else if (!few) {
+    rc = f8_quantize({x_dev, T, H, w.x.values, w.x.scales}, {}, dtype, st);
+  }
   if (rc != SPARSE_HIP_OK) return rc;
   F8Product p = {};
   p.slab = static_cast<const uint8_t*>(experts->slab_dev);

@@ -1,5 +1,6 @@
 // Rows to e4m3 with a power-of-two scale for each run of 128 values.
 #include "fp8.h"
+#include "prefill_queue.h"
 
 namespace sparse {
 
@@ -17,9 +18,9 @@ struct QuantizeArgs {
 
 // kVec: rows start on 16-byte boundaries and K is a multiple of 8
 template <typename T, bool kVec>
-__global__ __launch_bounds__(kQzThreads) void f8_quantize_kernel(const QuantizeArgs a) {
-  const int which = blockIdx.x >= a.first_blocks;
-  const uint32_t block = blockIdx.x - (which ? a.first_blocks : 0u);
+__device__ __forceinline__ void quantize_block(const QuantizeArgs& a, uint32_t block) {
+  const int which = block >= a.first_blocks;
+  if (which) block -= a.first_blocks;
   const int64_t run = static_cast<int64_t>(block) * kQzRuns + (threadIdx.x >> 4);
   if (run >= a.runs[which]) return;              // 16 lanes leave together
   const int K = a.K[which], nb = a.nb[which];
@@ -55,8 +56,21 @@ __global__ __launch_bounds__(kQzThreads) void f8_quantize_kernel(const QuantizeA
   if ((threadIdx.x & 15) == 0) a.scales[which][run] = static_cast<uint8_t>(s + kF8Bias);
 }
 
+template <typename T, bool kVec>
+__global__ __launch_bounds__(kQzThreads) void f8_quantize_kernel(const QuantizeArgs a) {
+  quantize_block<T, kVec>(a, blockIdx.x);
+}
+// The queue build is 20 workgroups that wait for memory most of their 5 to 10 us; beside the quantiser they cost
+// nothing.  They go first.
+static_assert(kQzThreads == 256, "the queue build counts on 256 threads");
+template <typename T, bool kVec>
+__global__ __launch_bounds__(kQzThreads) void f8_quantize_queue_kernel(const QuantizeArgs a, const PfxMapArgs queue, uint32_t queue_blocks) {
+  if (blockIdx.x < queue_blocks) prefill_queue_block(queue, blockIdx.x);
+  else quantize_block<T, kVec>(a, blockIdx.x - queue_blocks);
+}
+
 template <typename T>
-static int quantize_as(const F8Quantize& a, const F8Quantize& b, hipStream_t st) {
+static int quantize_as(const F8Quantize& a, const F8Quantize& b, const PfxMapArgs* queue, hipStream_t st) {
   QuantizeArgs q = {};
   int64_t blocks[2];
   bool vec = true;
@@ -71,10 +85,17 @@ static int quantize_as(const F8Quantize& a, const F8Quantize& b, hipStream_t st)
     blocks[i] = (q.runs[i] + kQzRuns - 1) / kQzRuns;
     vec = vec && m.K % kQzLane == 0 && (reinterpret_cast<uintptr_t>(m.x) & 15) == 0;
   }
-  SP_REQUIRE(blocks[0] + blocks[1] < (1ll << 31), "fp8_quantize: too many rows");
+  SP_REQUIRE(blocks[0] + blocks[1] < (1ll << 31) - (1 << 20), "fp8_quantize: too many rows");
   if (blocks[0] + blocks[1] == 0) return SPARSE_HIP_OK;
   q.first_blocks = static_cast<uint32_t>(blocks[0]);
-  const dim3 grid(static_cast<unsigned>(blocks[0] + blocks[1]));
+  const uint32_t extra = queue != nullptr ? queue->nt_gu + queue->nt_dn + 2 : 0;
+  const dim3 grid(static_cast<unsigned>(blocks[0] + blocks[1] + extra));
+  if (queue != nullptr) {
+    if (vec) hipLaunchKernelGGL((f8_quantize_queue_kernel<T, true>), grid, dim3(kQzThreads), 0, st, q, *queue, extra);
+    else hipLaunchKernelGGL((f8_quantize_queue_kernel<T, false>), grid, dim3(kQzThreads), 0, st, q, *queue, extra);
+    SP_LAUNCH_CHECK("f8_quantize_queue_kernel");
+    return SPARSE_HIP_OK;
+  }
   if (vec) hipLaunchKernelGGL((f8_quantize_kernel<T, true>), grid, dim3(kQzThreads), 0, st, q);
   else hipLaunchKernelGGL((f8_quantize_kernel<T, false>), grid, dim3(kQzThreads), 0, st, q);
   SP_LAUNCH_CHECK("f8_quantize_kernel");
@@ -82,9 +103,14 @@ static int quantize_as(const F8Quantize& a, const F8Quantize& b, hipStream_t st)
 }
 
 int f8_quantize(const F8Quantize& a, const F8Quantize& b, int dtype, hipStream_t st) {
-  if (dtype == SPARSE_HIP_BF16) return quantize_as<uint16_t>(a, b, st);
-  if (dtype == SPARSE_HIP_F16) return quantize_as<f16_t>(a, b, st);
-  return quantize_as<float>(a, b, st);
+  if (dtype == SPARSE_HIP_BF16) return quantize_as<uint16_t>(a, b, nullptr, st);
+  if (dtype == SPARSE_HIP_F16) return quantize_as<f16_t>(a, b, nullptr, st);
+  return quantize_as<float>(a, b, nullptr, st);
+}
+
+int f8_quantize_and_queue(const F8Quantize& a, int dtype, const PfxMapArgs& queue, hipStream_t st) {
+  if (dtype == SPARSE_HIP_F16) return quantize_as<f16_t>(a, {}, &queue, st);
+  return quantize_as<uint16_t>(a, {}, &queue, st);
 }
 
 }  // namespace sparse

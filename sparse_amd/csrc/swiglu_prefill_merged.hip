@@ -21,7 +21,7 @@
 #include <type_traits>
 
 #include "common.h"
-#include "prefill_tiles.h"
+#include "prefill_queue.h"
 
 namespace sparse {
 
@@ -327,138 +327,10 @@ __global__ __launch_bounds__(kPfThreads, 2) void prefill_merged_kernel(const Pfx
 }
 
 // ---- queues -------------------------------------------------------------------------------------
-struct PfxMapArgs {
-  const int32_t* expert_slot;
-  const int32_t* seg_offsets;
-  sparse_hip_seglist segs;
-  int32_t* hdr;            // per launch (gate/up, down) 16 ints: first entry [8], entries [8]
-  PfTile* map_gu;          // entry 0 of each map is the idle entry
-  PfTile* map_dn;
-  int32_t nt_gu, nt_dn;    // column tiles of a routed expert
-  int32_t nts_gu, nts_dn;  // column tiles of the shared expert (0: none)
-  int32_t mt_shared;       // row tiles of the shared expert
-  int32_t T;               // tokens (rows of the shared expert)
-  int32_t cap_gu, cap_dn;  // entries in each map
-};
-
-// Share x of n items cut into kPfXcds contiguous shares starts here.
-__device__ __forceinline__ int pfx_start(int n, int x) { return static_cast<int>(static_cast<int64_t>(n) * x / kPfXcds); }
-__device__ __forceinline__ int pfx_share_of(int n, int i) {
-  int x = min(kPfXcds - 1, static_cast<int>(static_cast<int64_t>(i) * kPfXcds / max(n, 1)));
-  while (x + 1 < kPfXcds && pfx_start(n, x + 1) <= i) ++x;
-  while (x > 0 && pfx_start(n, x) > i) --x;
-  return x;
-}
-// Queue x of a launch with R routed and S shared tiles: its share of the shared tiles, then its share
-// of the routed ones (the shared expert's down tiles are the long ones, so they go first).
-__device__ __forceinline__ int pfx_queue_base(int R, int S, int x) { return 1 + pfx_start(S, x) + pfx_start(R, x); }
-
-// Workgroups [0, nt_gu) and [nt_gu, nt_gu + nt_dn): one per routed column tile of the two launches --
-// segment s -> its row-tile count, scan, then thread s writes the entries of (segment s, this column
-// tile, row tile 0 ..), routed order (segment, column tile, row tile).  The two last workgroups write
-// the shared expert's entries (column tile, row tile) and the queue headers of their launch.
-__global__ __launch_bounds__(256) void prefill_queue_kernel(const PfxMapArgs a) {
-  __shared__ int32_t s_scan[SPARSE_HIP_MAX_EXPERTS];
-  const int tid = threadIdx.x;
-  int nseg = a.segs.n;
-  if (a.segs.eids_dev != nullptr) nseg = min(nseg, a.segs.count_dev[0]);
-  int mt = 0, slot = 0, r0 = 0, rows = 0;
-  if (tid < nseg) {
-    const int e = (a.segs.eids_dev != nullptr) ? a.segs.eids_dev[tid] : a.segs.eids[tid];
-    r0 = a.seg_offsets[e];
-    rows = a.seg_offsets[e + 1] - r0;
-    mt = (rows + kPfBM - 1) / kPfBM;
-    slot = (a.segs.eids_dev != nullptr) ? a.expert_slot[e] : a.segs.slots[tid];
-  }
-  s_scan[tid] = mt;
-  __syncthreads();
-  for (int off = 1; off < 256; off <<= 1) {
-    const int v = (tid >= off) ? s_scan[tid - off] : 0;
-    __syncthreads();
-    s_scan[tid] += v;
-    __syncthreads();
-  }
-  const int total_mt = s_scan[255];
-  const int b = blockIdx.x;
-  if (b < a.nt_gu + a.nt_dn) {
-    const int which = b < a.nt_gu ? 0 : 1;
-    const int bn = which == 0 ? b : b - a.nt_gu;
-    PfTile* map = which == 0 ? a.map_gu : a.map_dn;
-    const int nt = which == 0 ? a.nt_gu : a.nt_dn;
-    const int cap = which == 0 ? a.cap_gu : a.cap_dn;
-    const int R = total_mt * nt, S = a.mt_shared * (which == 0 ? a.nts_gu : a.nts_dn);
-    if (mt > 0) {
-      const int g0 = (s_scan[tid] - mt) * nt + bn * mt;
-      for (int bm = 0; bm < mt; ++bm) {
-        const int g = g0 + bm;
-        const int x = pfx_share_of(R, g);
-        const int pos = pfx_queue_base(R, S, x) + (pfx_start(S, x + 1) - pfx_start(S, x)) + (g - pfx_start(R, x));
-        if (pos < cap) map[pos] = PfTile{slot, r0 + bm * kPfBM, min(kPfBM, rows - bm * kPfBM), bn};
-      }
-    }
-    return;
-  }
-  const int which = b - (a.nt_gu + a.nt_dn);
-  PfTile* map = which == 0 ? a.map_gu : a.map_dn;
-  const int nt = which == 0 ? a.nt_gu : a.nt_dn;
-  const int cap = which == 0 ? a.cap_gu : a.cap_dn;
-  const int R = total_mt * nt, S = a.mt_shared * (which == 0 ? a.nts_gu : a.nts_dn);
-  // The shared expert's tiles.  Where the tile grid divides evenly, XCD x takes a block of it -- a quarter
-  // of the row tiles by half of the column tiles -- and walks the block down its rows first, so that the
-  // 64 workgroups an XCD runs at a time cover about 8 x 8 tiles: each activation row tile and each weight
-  // tile is then fetched into that L2 once per 8 users.  (Column by column over all row tiles, an XCD reads
-  // the whole activation matrix, four times its L2, once per column tile.)  Otherwise: contiguous shares
-  // of the (column tile, row tile) order.
-  const int nts = which == 0 ? a.nts_gu : a.nts_dn;
-  const bool blocked = a.mt_shared % 4 == 0 && nts % 2 == 0 && nts > 0;
-  const int RG = a.mt_shared / 4, per_xcd = S / kPfXcds;
-  for (int h = tid; h < S; h += 256) {
-    int bn, bm, x, local;
-    if (blocked) {
-      x = h / per_xcd;
-      local = h - x * per_xcd;
-      bm = (x & 3) * RG + local % RG;
-      bn = (x >> 2) * (nts / 2) + local / RG;
-    } else {
-      bn = h / a.mt_shared;
-      bm = h - bn * a.mt_shared;
-      x = pfx_share_of(S, h);
-      local = h - pfx_start(S, x);
-    }
-    const int pos = pfx_queue_base(R, S, x) + local;
-    if (pos < cap) map[pos] = PfTile{-1, bm * kPfBM, min(kPfBM, a.T - bm * kPfBM), bn};
-  }
-  if (tid == 0) map[0] = PfTile{0, 0, 0, 0};
-  if (tid < kPfXcds) {
-    int32_t* hdr = a.hdr + which * 16;
-    hdr[tid] = pfx_queue_base(R, S, tid);
-    hdr[kPfXcds + tid] = (pfx_start(S, tid + 1) - pfx_start(S, tid)) + (pfx_start(R, tid + 1) - pfx_start(R, tid));
-  }
-}
-
-static inline int pfx_max_mtiles(int Ttok, int K, int nseg) { return (Ttok * K + kPfBM - 1) / kPfBM + nseg; }
-
-struct PfxLayout {
-  int nt_gu, nt_dn, nts_gu, nts_dn, mt_shared, cap_gu, cap_dn;
-};
-static PfxLayout pfx_layout(int Ttok, int K, int nseg, int H, int I, int Is) {
-  PfxLayout l;
-  l.nt_gu = (I + kPfBR / 2 - 1) / (kPfBR / 2);
-  l.nt_dn = (H + kPfBR - 1) / kPfBR;
-  l.nts_gu = Is > 0 ? (Is + kPfBR / 2 - 1) / (kPfBR / 2) : 0;
-  l.nts_dn = Is > 0 ? l.nt_dn : 0;
-  l.mt_shared = Is > 0 ? (Ttok + kPfBM - 1) / kPfBM : 0;
-  const int mt = nseg > 0 ? pfx_max_mtiles(Ttok, K, nseg) : 0;
-  l.cap_gu = 1 + mt * l.nt_gu + l.mt_shared * l.nts_gu;
-  l.cap_dn = 1 + mt * l.nt_dn + l.mt_shared * l.nts_dn;
-  return l;
-}
-
-constexpr size_t kPfWsHeader = 256;   // two launches x 16 ints, padded
+__global__ __launch_bounds__(256) void prefill_queue_kernel(const PfxMapArgs a) { prefill_queue_block(a, blockIdx.x); }
 
 size_t prefill_merged_ws_bytes(int Ttok, int K, int nseg, int H, int I, int Is) {
-  const PfxLayout l = pfx_layout(Ttok, K, nseg, H, I, Is);
-  return kPfWsHeader + (static_cast<size_t>(l.cap_gu) + l.cap_dn) * sizeof(PfTile);
+  return prefill_queue_ws_bytes(Ttok, K, nseg, H, I, Is);
 }
 
 extern std::atomic<int> g_prefill_drain_waits;
@@ -485,34 +357,6 @@ static int launch_merged(PfxArgs& a, int cap, bool fp16, hipStream_t st) {
   return SPARSE_HIP_OK;
 }
 
-// Builds both launches' queues of a call in `tile_ws` (prefill_merged_ws_bytes) and says where they are.
-int prefill_queues(const int32_t* expert_slot, const int32_t* seg_offsets, const sparse_hip_seglist* segs, int Ttok,
-                   int K, int H, int I, int Is, void* tile_ws, PfQueues* q, hipStream_t st) {
-  const PfxLayout l = pfx_layout(Ttok, K, segs->n, H, I, Is);
-  int32_t* hdr = static_cast<int32_t*>(tile_ws);
-  PfTile* map_gu = reinterpret_cast<PfTile*>(static_cast<uint8_t*>(tile_ws) + kPfWsHeader);
-  PfTile* map_dn = map_gu + l.cap_gu;
-  PfxMapArgs m = {};
-  m.expert_slot = expert_slot;
-  m.seg_offsets = seg_offsets;
-  m.segs = *segs;
-  m.hdr = hdr;
-  m.map_gu = map_gu;
-  m.map_dn = map_dn;
-  m.nt_gu = l.nt_gu;
-  m.nt_dn = l.nt_dn;
-  m.nts_gu = l.nts_gu;
-  m.nts_dn = l.nts_dn;
-  m.mt_shared = l.mt_shared;
-  m.T = Ttok;
-  m.cap_gu = l.cap_gu;
-  m.cap_dn = l.cap_dn;
-  hipLaunchKernelGGL(prefill_queue_kernel, dim3(l.nt_gu + l.nt_dn + 2), dim3(256), 0, st, m);
-  SP_LAUNCH_CHECK("prefill_queue_kernel");
-  *q = PfQueues{hdr, map_gu, map_dn, l.cap_gu, l.cap_dn};
-  return SPARSE_HIP_OK;
-}
-
 // Routed experts (segs->n > 0) and / or the shared expert (sh_down_w != nullptr) of one call.
 int prefill_merged(const sparse_hip_experts* ex, const void* x, const void* topv, const int32_t* perm,
                    const int32_t* seg_offsets, const sparse_hip_seglist* segs, int Ttok, int K, void* inter_ws,
@@ -521,11 +365,10 @@ int prefill_merged(const sparse_hip_experts* ex, const void* x, const void* topv
                    hipStream_t st) {
   const int H = ex->hidden, I = ex->inter;
   const bool shared = sh_down_w != nullptr;
-  PfQueues qs;
-  {
-    int rc = prefill_queues(ex->expert_slot_dev, seg_offsets, segs, Ttok, K, H, I, shared ? Is : 0, tile_ws, &qs, st);
-    if (rc != SPARSE_HIP_OK) return rc;
-  }
+  PfxMapArgs m;
+  const PfQueues qs = prefill_queue_args(ex->expert_slot_dev, seg_offsets, *segs, Ttok, K, H, I, shared ? Is : 0, tile_ws, &m);
+  hipLaunchKernelGGL(prefill_queue_kernel, dim3(m.nt_gu + m.nt_dn + 2), dim3(256), 0, st, m);
+  SP_LAUNCH_CHECK("prefill_queue_kernel");
   const bool fp16 = ex->dtype == SPARSE_HIP_F16;
   PfxArgs a = {};
   a.slab = static_cast<const uint16_t*>(ex->slab_dev);
