@@ -495,7 +495,7 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
  * sparse_hip_fp8_slot_bytes(H, I) bytes in all.  H, I and Is are multiples of 64.  x [T,H], topv [T,K],
  * parts [T*K,H], shared_gate [T], shared [T,H] in that dtype.  `pow2_scales` as above, for all matrices of
  * the call.  `ws_dev`:
- * sparse_hip_fp8_moe_ffn_ws_bytes(T, K, segs->n, H, I, Is) bytes (Is = 0 without a shared expert), 16-byte
+ * sparse_hip_fp8_moe_ffn_ws_bytes(T, K, E, segs->n, H, I, Is) bytes (Is = 0 without a shared expert), 16-byte
  * aligned; calls that share one must be ordered on one stream.
  */
 size_t sparse_hip_fp8_slot_bytes(int H, int I);
@@ -505,7 +505,7 @@ size_t sparse_hip_fp8_slot_bytes(int H, int I);
  * differ in the order of their sums.  A workspace's size depends on it.  Returns the setting before.
  */
 int sparse_hip_fp8_path(int which);
-size_t sparse_hip_fp8_moe_ffn_ws_bytes(int T, int K, int num_segments, int H, int I, int Is);
+size_t sparse_hip_fp8_moe_ffn_ws_bytes(int T, int K, int num_experts, int num_segments, int H, int I, int Is);
 int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev, const void* topv_dev,
                            const int32_t* perm_dev, const int32_t* seg_offsets_dev,
                            const sparse_hip_seglist* segs, int T, int K, void* parts_dev,

@@ -118,7 +118,7 @@ SIGNATURES = {
     "sparse_hip_fp8_linear": (_i, [_vp, _vp, _vp, _i, _i, _mat, _i, _vp, _vp, _vp]),
     "sparse_hip_fp8_path": (_i, [_i]),
     "sparse_hip_fp8_slot_bytes": (_sz, [_i, _i]),
-    "sparse_hip_fp8_moe_ffn_ws_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "sparse_hip_fp8_moe_ffn_ws_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "sparse_hip_fp8_moe_ffn": (
         _i, [C.POINTER(Experts), _vp, _vp, _vp, _vp, C.POINTER(SegList), _i, _i, _vp, _mat, _mat, _mat, _vp, _i, _vp,
              _vp, _vp]),

@@ -24,7 +24,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import ops
+from . import fp8, ops
 from ._lru import LruTable
 from .context import DistEnv, Metrics, SparseContext
 from .residency import Backend, LayerResidency, ResidencyConfig
@@ -73,28 +73,43 @@ def extract_experts(experts: Any) -> Tuple[str, List[Tuple[torch.Tensor, torch.T
     raise RuntimeError("Unsupported experts container. Need fused or modulelist experts.")
 
 
+def quantized_experts(experts: Any, device: Any) -> List[Tuple[fp8.Quantized, fp8.Quantized, fp8.Quantized]]:
+    """(values, scales) of every expert's gate, up and down: a module's own where it holds 8-bit weights with
+    block scales, else quantised here, on ``device``."""
+    kind, triples = extract_experts(experts)
+    if kind == "modulelist":
+        return [tuple(fp8.module_weight(m, device) for m in (e.gate_proj, e.up_proj, e.down_proj)) for e in experts]
+    if any(w.dtype == fp8.E4M3 for w in triples[0]):
+        raise NotImplementedError("fused containers of 8-bit experts are not built: give modules with weight_scale_inv")
+    return [tuple(fp8.quantize_weight(w.to(device)) for w in t) for t in triples]
+
+
 class _Workspace:
     """Activation buffers for one (T, layer shape); shared by all layers of that shape.  The
     most recently used ``SPARSE_HIP_WORKSPACE_CACHE`` (default 8) shapes are kept."""
 
     _cache = LruTable.from_env("SPARSE_HIP_WORKSPACE_CACHE", 8)
 
-    def __init__(self, T: int, K: int, E: int, H: int, I: int, Is: int, dtype, logits_dtype, device) -> None:
+    def __init__(self, T: int, K: int, E: int, H: int, I: int, Is: int, dtype, logits_dtype, device,
+                 weight_format: str = "native") -> None:
         self.logits_dtype = logits_dtype
         self.shared_gate = torch.empty((T,), device=device, dtype=dtype)
         self.topv = torch.empty((T, K), device=device, dtype=dtype)
         self.topi = torch.empty((T, K), device=device, dtype=torch.int64)
         self.perm = ops.Permutation(T, K, E, device)
-        self.inter = torch.empty((T * K, I), device=device, dtype=dtype)
+        eight = weight_format == "fp8"       # the 8-bit products keep what they need in one block of bytes
+        self.inter = None if eight else torch.empty((T * K, I), device=device, dtype=dtype)
         self.parts = torch.empty((T * K, H), device=device, dtype=dtype)
-        self.shared_inter = torch.empty((T, Is), device=device, dtype=dtype) if Is else None
+        self.shared_inter = torch.empty((T, Is), device=device, dtype=dtype) if Is and not eight else None
+        self.fp8_ws = (torch.empty((fp8.moe_ffn_ws_bytes(T, K, E, min(E, T * K), H, I, Is),), device=device,
+                                   dtype=torch.uint8) if eight else None)
         self.shared_out = torch.empty((T, H), device=device, dtype=dtype) if Is else None
         self.segs_dev = ops.seglist_device(self.perm, min(E, T * K))
         self.route_counter = torch.zeros((1,), device=device, dtype=torch.int32)
         # small decode calls cut the shared down projection's long reduction into parts (fp32
         # sums here) that the combine step finishes; from 17 tokens on the routed experts are
         # enough work beside it and the extra reads of the combine step cost more than they save
-        self.split_parts = (ops.decode_split_parts(Is) if Is and T <= 16
+        self.split_parts = (ops.decode_split_parts(Is) if Is and T <= 16 and not eight
                             and dtype in ops.HALF_DTYPES and torch.device(device).type == "cuda" else 1)
         self.split_ws = ops.decode_split_workspace(T, H, device) if self.split_parts > 1 else None
         # host mirrors for the offloaded path (pinned, written by async D2H copies)
@@ -186,7 +201,10 @@ class _HipBackend(Backend):
     def run_segments(self, segments: Sequence[Tuple[int, int]]) -> None:
         blk, ws = self.block, self.ws
         segs = ops.seglist_host([e for e, _ in segments], [s for _, s in segments])
-        ops.grouped_swiglu(blk._experts_desc, self.x, ws.topv, ws.perm, segs, ws.inter, ws.parts)
+        if blk.weight_format == "fp8":
+            fp8.moe_ffn(blk.slab, self.x, ws.topv, ws.perm, segs=segs, parts=ws.parts, ws=ws.fp8_ws)
+        else:
+            ops.grouped_swiglu(blk._experts_desc, self.x, ws.topv, ws.perm, segs, ws.inter, ws.parts)
         self.launches += 1
 
     def fence(self):
@@ -231,6 +249,7 @@ class DistributedSparseMoeBlock(nn.Module):
         runtime_mode: str = "baseline",
         topology: Any = None,
         residency_config: Optional[ResidencyConfig] = None,
+        weight_format: str = "native",
     ) -> None:
         super().__init__()
         self.layer_idx = int(layer_idx)
@@ -292,6 +311,13 @@ class DistributedSparseMoeBlock(nn.Module):
             raise ValueError(f"cache_policy must be lru|lfu|tiered, got {self.cache_policy}")
         if self.dtype not in (torch.bfloat16, torch.float16, torch.float32):
             raise ValueError(f"dtype must be bfloat16, float16 or float32, got {self.dtype}")
+        # "native": expert weights in `dtype`; "fp8": in 8 bits with a scale per 128 x 128 block (the reference
+        # has no such path)
+        self.weight_format = str(weight_format).lower()
+        if self.weight_format not in ("native", "fp8"):
+            raise ValueError(f"weight_format must be native|fp8, got {weight_format}")
+        if self.weight_format == "fp8" and self.dtype not in ops.HALF_DTYPES:
+            raise ValueError(f"weight_format=fp8 needs bfloat16 or float16 activations, got {self.dtype}")
         self.rs_group = int(rs_group)
         self.rs_prob_to_logit_eps = float(rs_prob_to_logit_eps)
         self.prefetch_top_m = int(prefetch_top_m)
@@ -321,16 +347,27 @@ class DistributedSparseMoeBlock(nn.Module):
         self.gate_weight = mlp_block.gate.weight.detach().to(self.device, self.dtype).contiguous()
         # selection method of a DeepSeek-family gate module (the reference runs whatever gate the
         # model brings, :9503-9517): plain greedy top-k, or limited to the best expert groups
-        method = str(getattr(gate_mod, "topk_method", "greedy") or "greedy")
-        if method not in ("greedy", "group_limited_greedy"):
-            raise NotImplementedError(f"gate topk_method={method} is not built (greedy | group_limited_greedy)")
+        bias = getattr(gate_mod, "e_score_correction_bias", None)
+        method = str(getattr(gate_mod, "topk_method", None) or ("greedy" if bias is None else "noaux_tc"))
+        if method not in ("greedy", "group_limited_greedy", "noaux_tc"):
+            raise NotImplementedError(f"gate topk_method={method} is not built (greedy | group_limited_greedy | noaux_tc)")
+        if (method == "noaux_tc") != (bias is not None):
+            raise ValueError("gate topk_method=noaux_tc goes with e_score_correction_bias")
+        # a gate balanced by a bias ranks the sigmoid of the logits plus the bias, groups by their two best
+        self.gate_score = str(getattr(gate_mod, "scoring_func", None) or ("softmax" if bias is None else "sigmoid"))
+        if self.gate_score not in ops.SELECT_SCORE:
+            raise NotImplementedError(f"gate scoring_func={self.gate_score} is not built (softmax | sigmoid)")
+        self.gate_bias = None if bias is None else bias.detach().to(self.device, torch.float32).reshape(-1).contiguous()
+        self.gate_group_score = "max" if bias is None else "top2"
         self.n_group = self.topk_group = 1
-        if method == "group_limited_greedy":
+        if method != "greedy":
             self.n_group = int(getattr(gate_mod, "num_group", None) or getattr(gate_mod, "n_group", None) or 1)
             self.topk_group = int(getattr(gate_mod, "topk_group", None) or self.n_group)
             if self.topk_group >= self.n_group:
                 self.n_group = self.topk_group = 1          # every group kept: plain top-k
         self.experts_kind, expert_weights = extract_experts(mlp_block.experts)
+        if self.weight_format != "fp8" and any(w.dtype == fp8.E4M3 for w in expert_weights[0]):
+            raise ValueError("8-bit expert weights need weight_format='fp8'")
         self.num_experts = int(num_experts) if num_experts is not None else len(expert_weights)
         if self.num_experts != len(expert_weights) or self.gate_weight.shape[0] != self.num_experts:
             raise ValueError("num_experts does not match the gate / experts container")
@@ -342,10 +379,15 @@ class DistributedSparseMoeBlock(nn.Module):
         if shared_mod is not None:
             if not _is_silu(getattr(shared_mod, "act_fn", None)):
                 raise NotImplementedError("only SiLU shared experts are built")
-            # tiled content, logical [rows, cols] shape kept for argument checks
-            self.shared_weights = tuple(
-                tile_weight(t.to(self.device, self.dtype)).reshape(t.shape).contiguous()
-                for t in _mlp_weights(shared_mod))
+            if self.weight_format == "fp8":
+                self.shared_weights = tuple(
+                    fp8.Weight.from_quantized(*fp8.module_weight(m, self.device))
+                    for m in (shared_mod.gate_proj, shared_mod.up_proj, shared_mod.down_proj))
+            else:
+                # tiled content, logical [rows, cols] shape kept for argument checks
+                self.shared_weights = tuple(
+                    tile_weight(t.to(self.device, self.dtype)).reshape(t.shape).contiguous()
+                    for t in _mlp_weights(shared_mod))
             self.shared_inter_size = int(self.shared_weights[0].shape[0])
         sg = getattr(mlp_block, "shared_expert_gate", None)
         self.shared_gate_weight = (
@@ -360,8 +402,10 @@ class DistributedSparseMoeBlock(nn.Module):
         self._local_eid_set = set(self.local_expert_ids)
         self.residency: Optional[LayerResidency] = None
         self.arena: Optional[HostExpertArena] = None
+        eight = self.weight_format == "fp8"
         if self.expert_offload == "gpu":
-            self.slab = ExpertSlab.resident(expert_weights, H, I, self.dtype, self.device)
+            self.slab = (fp8.ExpertSlab.from_quantized(quantized_experts(mlp_block.experts, self.device), self.device)
+                         if eight else ExpertSlab.resident(expert_weights, H, I, self.dtype, self.device))
         else:
             cfg = residency_config if residency_config is not None else ResidencyConfig.from_env(
                 capacity=int(expert_cache), planner_mode=self.planner_mode, prefetch_top_m=int(prefetch_top_m))
@@ -370,12 +414,17 @@ class DistributedSparseMoeBlock(nn.Module):
                 cfg.cache_policy = self.cache_policy
             elif cfg.cache_policy != self.cache_policy and self.cache_policy != "lru":
                 cfg.cache_policy = self.cache_policy
-            self.arena = HostExpertArena(expert_weights, H, I, self.dtype, pin=True)
+            self.arena = (fp8.HostExpertArena(quantized_experts(mlp_block.experts, self.device), H, I, pin=True)
+                          if eight else HostExpertArena(expert_weights, H, I, self.dtype, pin=True))
             self._backend = _HipBackend(self)
             self.residency = LayerResidency(self.layer_idx, E, self.top_k, cfg, self._backend, self.metrics,
                                             expert_bytes=self.arena.expert_bytes)
-            self.slab = ExpertSlab(self.residency.num_slots, E, H, I, self.dtype, self.device)
-        self._experts_desc = ops.make_experts(self.slab.data, self.slab.expert_slot, E, H, I)
+            if eight:
+                self.slab = fp8.ExpertSlab(self.residency.num_slots, E, H, I, self.device)
+                self.slab.pow2 = self.arena.pow2
+            else:
+                self.slab = ExpertSlab(self.residency.num_slots, E, H, I, self.dtype, self.device)
+        self._experts_desc = None if eight else ops.make_experts(self.slab.data, self.slab.expert_slot, E, H, I)
         self._cache = self.residency.cache if self.residency is not None else None
         self._current_forward_batch_size = 0
         self._current_forward_seq_len = 0
@@ -400,7 +449,8 @@ class DistributedSparseMoeBlock(nn.Module):
     def _workspace(self, T: int, K: Optional[int] = None) -> _Workspace:
         return _Workspace.get(T, self.top_k if K is None else int(K), self.num_experts, self.hidden_size,
                               self.inter_size,
-                              self.shared_inter_size, self.dtype, self.logits_dtype, self.device)
+                              self.shared_inter_size, self.dtype, self.logits_dtype, self.device,
+                              *(() if self.weight_format == "native" else (self.weight_format,)))
 
     _shared_streams: dict = {}
 
@@ -446,7 +496,8 @@ class DistributedSparseMoeBlock(nn.Module):
         after_logits = after_logits or (lambda: None)
         logits = torch.empty((x.shape[0], self.num_experts), device=x.device, dtype=self.logits_dtype)
         shared_gate = ws.shared_gate if self.shared_gate_weight is not None else None
-        one_launch = self.routed_scaling_factor == 1.0 and self.n_group == 1
+        selects = self.gate_bias is not None or self.gate_score != "softmax"
+        one_launch = self.routed_scaling_factor == 1.0 and self.n_group == 1 and not selects
         if self.gate_packed is not None and x.shape[0] <= ops.ROUTE_PACKED_MAX_TOKENS and one_launch:
             # the routing launch also runs the shared expert's gate and up projections where it can
             beside = self._shared_up_wanted
@@ -465,6 +516,12 @@ class DistributedSparseMoeBlock(nn.Module):
         ops.router_logits(x, self.gate_weight, self.shared_gate_weight, self.logits_dtype, out=logits,
                           shared_gate_out=shared_gate)
         after_logits()
+        if selects:
+            ops.gate_select(logits, self.top_k, self.gate_score, self.gate_bias, self.n_group, self.topk_group,
+                            self.gate_group_score, self.norm_topk_prob, self.routed_scaling_factor, self.dtype,
+                            topv=ws.topv, topi=ws.topi)
+            ops.permute_build(ws.topi, self.num_experts, out=ws.perm)
+            return logits
         # the routed scaling factor multiplies in fp32 inside the top-k launch, before the one rounding to
         # the activation dtype, as the gate module does before the reference's cast (:9509-9513)
         ops.gate_topk(logits, self.top_k, self.norm_topk_prob, out_dtype=self.dtype, topv=ws.topv, topi=ws.topi,
@@ -624,15 +681,16 @@ class DistributedSparseMoeBlock(nn.Module):
 
         shared_gate = ws.shared_gate if self.shared_gate_weight is not None else None
         timing = self._segment_timing_on()
-        fused = (self.residency is None and self.shared_weights is not None and self.dtype in ops.HALF_DTYPES
+        eight = self.weight_format == "fp8"
+        fused = (not eight and self.residency is None and self.shared_weights is not None and self.dtype in ops.HALF_DTYPES
                  and T <= ops.DECODE_MAX_TOKENS and not timing)
         # Prefill-size batches: the shared expert needs only x and the shared gate, so it runs
         # on a second stream from the moment the logits kernel is queued, beside top-k,
         # permutation, tile map and the first routed tiles, and is joined before combine.
-        merged = (self.merged_prefill and self.residency is None and self.dtype in ops.HALF_DTYPES and x.is_cuda
+        merged = (self.merged_prefill and not eight and self.residency is None and self.dtype in ops.HALF_DTYPES and x.is_cuda
                   and T > ops.DECODE_MAX_TOKENS and not timing)
         side = (self._shared_stream() if self.shared_weights is not None and not fused and self.overlap_shared
-                and x.is_cuda and T > ops.DECODE_MAX_TOKENS and not timing and not merged else None)
+                and x.is_cuda and T > ops.DECODE_MAX_TOKENS and not timing and not merged and not eight else None)
 
         # Whether the shared expert's down projection is left as partial sums for the combine
         # step depends on the call's size and dtype only, never on where the routed experts
@@ -641,7 +699,7 @@ class DistributedSparseMoeBlock(nn.Module):
         # Calls of up to 16 tokens compute the shared expert's gate and up projections with the
         # 16-wavefront kernel, beside the routing when this call routes with the packed router,
         # alone otherwise: the same code, so the same bits, wherever it runs.
-        shared_up_alone = (self.shared_weights is not None and self.dtype in ops.HALF_DTYPES and x.is_cuda
+        shared_up_alone = (self.shared_weights is not None and not eight and self.dtype in ops.HALF_DTYPES and x.is_cuda
                            and self.route_with_shared and T <= ops.ROUTE_PACKED_MAX_TOKENS
                            and self.shared_inter_size % 32 == 0 and H % 64 == 0)
         self._shared_up_wanted = shared_up_alone and not timing
@@ -655,6 +713,12 @@ class DistributedSparseMoeBlock(nn.Module):
 
         def run_shared() -> None:
             if self.shared_weights is None or fused or merged:
+                return
+            if eight:
+                # beside the routed experts in their launches, unless those are executed or timed apart
+                if self.residency is not None or timing:
+                    fp8.moe_ffn(self.slab, x, ws.topv, ws.perm, shared=self.shared_weights, shared_gate=shared_gate,
+                                segs=_NO_SEGMENTS(), parts=ws.parts, shared_out=ws.shared_out, ws=ws.fp8_ws)
                 return
             gw, uw, dw = self.shared_weights
             if split_shared:
@@ -703,6 +767,9 @@ class DistributedSparseMoeBlock(nn.Module):
             elif merged:
                 ops.moe_ffn_prefill(self._experts_desc, x, ws.topv, ws.perm, ws.segs_dev, ws.inter, ws.parts,
                                     self.shared_weights, shared_gate, ws.shared_inter, ws.shared_out)
+            elif self.residency is None and eight:
+                fp8.moe_ffn(self.slab, x, ws.topv, ws.perm, shared=None if timing else self.shared_weights,
+                            shared_gate=shared_gate, segs=ws.segs_dev, parts=ws.parts, shared_out=ws.shared_out, ws=ws.fp8_ws)
             elif self.residency is None:
                 ops.grouped_swiglu(self._experts_desc, x, ws.topv, ws.perm, ws.segs_dev, ws.inter, ws.parts)
             else:

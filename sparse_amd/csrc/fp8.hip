@@ -23,12 +23,14 @@ static bool linear_tiles(int T, int N) {
   if (T <= kF8FewRows || path == 1) return false;
   return path == 2 || static_cast<int64_t>((T + 31) / 32) * N > 28672;
 }
-static bool ffn_tiles(int T, int K, int nseg, int H, int I, int Is) {
+// (The routed experts decide, all of them, so that a layer whose experts are executed in several calls, or apart
+// from the shared one, takes the same kernels in each.)
+static bool ffn_tiles(int T, int K, int E, int H, int I) {
   const int path = g_path.load(std::memory_order_relaxed);
   if (T <= kF8FewRows || path == 1) return false;
   // work of the rows against a fixed cost and one for the weights
-  const double h = H, rows = T * h * (static_cast<double>(nseg > 0 ? K : 0) * I + Is);
-  return path == 2 || rows > (1 << 29) + 7.0 * h * (static_cast<double>(nseg) * I + Is);
+  const double h = H;
+  return path == 2 || T * h * K * I > 7.0 * (1 << 26) + 4.0 * h * E * I;
 }
 
 static inline size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
@@ -75,7 +77,7 @@ struct FfnWs {
   void* tiles;        // many rows: the tile queues
   size_t bytes;
 };
-static FfnWs ffn_ws(void* ws, int T, int K, int nseg, int H, int I, int Is) {
+static FfnWs ffn_ws(void* ws, int T, int K, int E, int nseg, int H, int I, int Is) {
   Carve c{static_cast<uint8_t*>(ws)};
   FfnWs w = {};
   const int64_t rows = nseg > 0 ? static_cast<int64_t>(T) * K : 0;
@@ -84,7 +86,7 @@ static FfnWs ffn_ws(void* ws, int T, int K, int nseg, int H, int I, int Is) {
     w.h = take_rows(c, rows, I);
     if (Is > 0) w.sh = take_rows(c, T, Is);
   }
-  if (ffn_tiles(T, K, nseg, H, I, Is)) {
+  if (ffn_tiles(T, K, E, H, I)) {
     w.tiles = c.take(prefill_queue_ws_bytes(T, K, nseg, H, I, Is));
   } else {
     w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
@@ -175,9 +177,9 @@ size_t sparse_hip_fp8_slot_bytes(int H, int I) {
   return f8_slot(H, I).bytes;
 }
 
-size_t sparse_hip_fp8_moe_ffn_ws_bytes(int T, int K, int num_segments, int H, int I, int Is) {
-  if (T <= 0 || K <= 0 || num_segments < 0 || H <= 0 || I <= 0 || Is < 0) return 0;
-  return ffn_ws(nullptr, T, K, num_segments, H, I, Is).bytes;
+size_t sparse_hip_fp8_moe_ffn_ws_bytes(int T, int K, int num_experts, int num_segments, int H, int I, int Is) {
+  if (T <= 0 || K <= 0 || num_experts <= 0 || num_segments < 0 || H <= 0 || I <= 0 || Is < 0) return 0;
+  return ffn_ws(nullptr, T, K, num_experts, num_segments, H, I, Is).bytes;
 }
 
 int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev, const void* topv_dev,
@@ -227,11 +229,11 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   if (!routed && !shared) return SPARSE_HIP_OK;
   SP_REQUIRE(ws_dev != nullptr && aligned16(ws_dev), "%s: workspace is NULL or not 16-byte aligned", fn);
   hipStream_t st = as_stream(stream);
-  const FfnWs w = ffn_ws(ws_dev, T, K, segs->n, H, I, Is);
+  const FfnWs w = ffn_ws(ws_dev, T, K, E, segs->n, H, I, Is);
 
   // One or two tokens: rows are quantised inside the products.  More: in launches of their own, beside products
   // that stream weights; beside the tile kernel x only, which quantises the intermediate in its epilogue.
-  const bool few = T <= kF8FewRows, tiles = ffn_tiles(T, K, segs->n, H, I, Is);
+  const bool few = T <= kF8FewRows, tiles = ffn_tiles(T, K, E, H, I);
   int rc = SPARSE_HIP_OK;
   PfQueues queues = {};
   if (tiles) {

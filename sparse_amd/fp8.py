@@ -19,7 +19,7 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
-from . import _lib, ops
+from . import _lib, ops, weights
 from ._lib import Fp8Matrix, SegList
 from .ops import HALF_DTYPES, Permutation, _need, _need_half, _ptr, _same_device, call_on, dtype_code
 
@@ -275,9 +275,39 @@ class ExpertSlab:
         return ref
 
 
-def moe_ffn_ws_bytes(T: int, K: int, num_segments: int, hidden: int, inter: int, shared_inter: int = 0) -> int:
-    return int(_lib.load().sparse_hip_fp8_moe_ffn_ws_bytes(int(T), int(K), int(num_segments), int(hidden), int(inter),
-                                                           int(shared_inter)))
+class HostExpertArena(weights.HostExpertArena):
+    """All routed experts of a layer as 8-bit slots in pinned host memory, one row per expert id: an upload is
+    one copy of half the bytes of the 16-bit arena's."""
+
+    def __init__(self, experts: Sequence[Tuple[Quantized, Quantized, Quantized]], hidden: int, inter: int,
+                 pin: bool = True) -> None:
+        self.hidden, self.inter, self.dtype = int(hidden), int(inter), torch.uint8
+        self._allocate(len(experts), slot_bytes(hidden, inter), torch.uint8, pin)
+        pow2 = []
+        for e, expert in enumerate(experts):
+            pack_expert_into(self.rows[e], expert, hidden, inter)
+            pow2.append(all(are_pow2(s) for _, s in expert))
+        self.pow2 = all(pow2)
+
+
+def module_weight(linear_mod, device=None) -> Quantized:
+    """(values, scales) of a ``Linear``-like module: its own where it holds 8-bit weights with
+    ``weight_scale_inv`` (the layout of 8-bit checkpoints, one scale per 128 x 128 block), else quantised."""
+    w = linear_mod.weight.detach()
+    if w.dtype == E4M3:
+        s = getattr(linear_mod, "weight_scale_inv", None)
+        if s is None:
+            raise ValueError("an 8-bit weight needs weight_scale_inv")
+        pair = w, s.detach().to(torch.float32)
+        _check_quantized(*pair)
+        return (pair[0].to(device), pair[1].to(device)) if device is not None else pair
+    return quantize_weight(w if device is None else w.to(device))
+
+
+def moe_ffn_ws_bytes(T: int, K: int, num_experts: int, num_segments: int, hidden: int, inter: int,
+                     shared_inter: int = 0) -> int:
+    return int(_lib.load().sparse_hip_fp8_moe_ffn_ws_bytes(int(T), int(K), int(num_experts), int(num_segments),
+                                                           int(hidden), int(inter), int(shared_inter)))
 
 
 def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Permutation,
@@ -331,7 +361,7 @@ def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Perm
     if T == 0:
         return parts, shared_out
     lib = _lib.load()
-    need = lib.sparse_hip_fp8_moe_ffn_ws_bytes(T, K, segs.n, H, experts.inter, Is)
+    need = lib.sparse_hip_fp8_moe_ffn_ws_bytes(T, K, E, segs.n, H, experts.inter, Is)
     if ws is None:
         ws = x.new_empty((max(1, need),), dtype=torch.uint8)
     elif not ws.is_contiguous() or ws.numel() * ws.element_size() < need:

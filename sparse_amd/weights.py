@@ -62,8 +62,12 @@ class HostExpertArena:
     def __init__(self, experts: Sequence[ExpertWeights], hidden: int, inter: int, dtype: torch.dtype,
                  pin: bool = True) -> None:
         self.hidden, self.inter, self.dtype = hidden, inter, dtype
-        self.num_experts = len(experts)
-        numel = expert_numel(hidden, inter)
+        self._allocate(len(experts), expert_numel(hidden, inter), dtype, pin)
+        for e, w in enumerate(experts):
+            pack_expert_into(self.rows[e], tuple(t.to(dtype) for t in w), hidden, inter)
+
+    def _allocate(self, num_experts: int, numel: int, dtype: torch.dtype, pin: bool) -> None:
+        self.num_experts = num_experts
         self._pinned_ptr = None
         if pin:
             # hipHostMalloc of the exact size: torch's pinned allocator rounds every block up
@@ -75,8 +79,6 @@ class HostExpertArena:
             self.rows = torch.frombuffer(buf, dtype=torch.uint8).view(dtype).view(self.num_experts, numel)
         else:
             self.rows = torch.empty((self.num_experts, numel), dtype=dtype)
-        for e, w in enumerate(experts):
-            pack_expert_into(self.rows[e], tuple(t.to(dtype) for t in w), hidden, inter)
         self.expert_bytes = self.rows[0].numel() * self.rows.element_size()
 
     def __del__(self) -> None:

@@ -193,3 +193,31 @@ def test_moe_ffn_refusals():
     refused(call(m=(mats[0], mats[0], _lib.Fp8Matrix(P, P, 64, Is)), sh=P), "down_proj")
     refused(call(m=tuple(mats), sh=None), "shared")
     assert call(sg=segs(n=0)) == 0     # nothing to do
+
+
+def test_block_refusals():
+    from types import SimpleNamespace as NS
+
+    from sparse_amd.block import DistributedSparseMoeBlock
+    from sparse_amd.context import DistEnv, SparseContext
+    from sparse_amd.synthetic import make_mlp_block
+
+    shape = dict(family="deepseek_shared", hidden=64, num_experts=8, inter=64, shared_inter=64)
+
+    def make(gate=None, dtype=torch.bfloat16, **kw):
+        SparseContext.reset()
+        mlp = make_mlp_block(shape, dtype=dtype)
+        if gate:
+            mlp.gate = NS(weight=mlp.gate.weight, **gate)
+        return DistributedSparseMoeBlock(0, mlp, None, DistEnv(0, 1, 0, torch.device("cpu")), num_experts=8, top_k=2, dtype=dtype, **kw)
+
+    with pytest.raises(ValueError, match="weight_format must be"):
+        make(weight_format="int4")
+    with pytest.raises(ValueError, match="activations"):
+        make(dtype=torch.float32, weight_format="fp8")
+    with pytest.raises(ValueError, match="e_score_correction_bias"):
+        make(gate=dict(topk_method="noaux_tc"))
+    with pytest.raises(ValueError, match="e_score_correction_bias"):
+        make(gate=dict(topk_method="greedy", e_score_correction_bias=torch.zeros(8)))
+    with pytest.raises(NotImplementedError, match="scoring_func"):
+        make(gate=dict(scoring_func="tanh"))
