@@ -21,6 +21,18 @@ namespace sparse {
 
 constexpr int kTlRowBytes = kF8Block;               // LDS row of one k slab
 constexpr int kTlSlab = kPfBM * kTlRowBytes;
+constexpr int kTlRing = kPfStages * kTlSlab;
+
+// A tile of 32 NMI rows keeps S slabs of weight fragments in registers and S + 1 slabs of rows in LDS.  What a
+// low tile saves in accumulators and rows goes into depth: its slab is half the work or less, and four slabs
+// ahead its weights are as far away in time.
+constexpr int tl_depth(int nmi) { return nmi == 1 ? 4 : nmi == 2 ? 3 : 2; }
+// "The copies of the next slab have landed": its copies were followed by their own slab's 8 fragment loads and by
+// S - 1 slabs of NMI copies and 8 loads each.
+constexpr int tl_younger(int nmi) { return 8 + (tl_depth(nmi) - 1) * (nmi + 8); }
+constexpr int tl_wait(int vmcnt) { return 0x0F70 | (vmcnt & 15) | ((vmcnt >> 4) << 14); }
+static_assert(tl_younger(4) == 20 && tl_wait(20) == kWaitVmcnt20 && tl_younger(2) < 64 && tl_younger(1) < 64, "six bits");
+static_assert((tl_depth(1) + 1) * 32 * kTlRowBytes <= kTlRing && (tl_depth(2) + 1) * 64 * kTlRowBytes <= kTlRing, "rings fit");
 constexpr int kTlScaleBytes = kPfBM + 2 * sizeof(float);   // per slab: activation bytes, two weight scales
 static_assert(kTlSlab == kPfLdsA, "the slab geometry is that of the 16-bit kernels");
 
@@ -46,7 +58,7 @@ struct TileArgs {
 // kPow2: every weight scale is a power of two, and enters the instruction as its exponent
 template <typename F, bool kGateUp, bool kPow2>
 __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kPfStages][kTlSlab];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kTlRing];
   __shared__ float s_row[kPfBM];          // factor of a row (down), exponent of a row's scale (gate/up)
   __shared__ float s_amax[kGateUp ? 4 : 1][kPfBM];
   extern __shared__ __attribute__((aligned(16))) uint8_t s_scales[];   // [nk][128] bytes, then [nk][2] floats
@@ -54,9 +66,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int fr = lane & 15, fq = lane >> 4;
-  constexpr int kWaitVm0 = kWaitVmcnt0, kWaitVm20 = kWaitVmcnt20;
   const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-      (__attribute__((address_space(3))) uint8_t*)(&lds[0][0])));
+      (__attribute__((address_space(3))) uint8_t*)(&lds[0])));
 
   // ---- which tile (wavefront-uniform) ------------------------------------------------
   int slot, r0, M, bn;
@@ -87,8 +98,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
   const int n0 = bn * (kGateUp ? kPfBR / 2 : kPfBR);   // first output column of this tile
 
   // ---- operand addresses ------------------------------------------------------------
-  // Row r keeps chunk 2q + h at position (q + 4h) ^ f(r), f(r) = ((r >> 1) & 7) ^ ((r & 1) << 2); with
-  // r = 32 wave + 8 it + (lane >> 3), f depends on `it` through its low bit only, which flips bit 0 of the chunk.
+  // Row r keeps chunk 2q + h at position (q + 4h) ^ f(r), f(r) = ((r >> 1) & 7) ^ ((r & 1) << 2); of eight rows
+  // from 8 i on, f depends on i through its low bit only, which flips bit 0 of the chunk.
   const int l3 = lane >> 3;
   const int pos0 = (lane & 7) ^ ((l3 >> 1) ^ ((l3 & 1) << 2));
   const uint32_t chunk0 = ((pos0 & 3) << 1) | (pos0 >> 2);
@@ -102,19 +113,6 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
     if (!gather) return static_cast<uint32_t>(mm);
     uint32_t g = static_cast<uint32_t>(a.p.perm[r0 + mm]);
     return a.topk_magic != 0 ? __umulhi(g, a.topk_magic) : g;
-  };
-  uint32_t doff[4];   // byte offset of lane's piece of copy `it` inside k slab 0
-#pragma unroll
-  for (int it = 0; it < 4; ++it)
-    doff[it] = source_row(wave * 32 + it * 8 + l3) * ld + ((chunk0 ^ (it & 1)) << 4);
-  auto stage_slab = [&](int slab, int buf) {
-    const uint8_t* sb = abase + static_cast<size_t>(slab) * kF8Block;
-#pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + buf * kTlSlab + (wave * 4 + it) * 1024);
-      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(doff[it]), "s"(sb), "s"(dst)
-                   : "memory");
-    }
   };
   // The wavefront's 64 weight rows are four 16-row groups (gate/up: groups 0, 1 gate rows of 32 neurons,
   // groups 2, 3 the up rows of the same neurons); a group's slab is 2 KB, its two halves 1 KB each in lane order.
@@ -154,17 +152,16 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
   };
 
   // ---- scales to LDS, row factors ------------------------------------------------------
-  // Called once the first slabs are on their way.  Bytes are fetched eight at a time before the first is
-  // stored: one by one, each would wait a memory latency (a 16-slab tile then spent 8 of them here).
-  const uint8_t* my_scales = sbase + static_cast<size_t>(source_row(tid >> 1)) * nk;
+  // Bytes are fetched eight at a time before the first is stored: one by one, each would wait a memory latency.
   auto fill_scales = [&]() __attribute__((always_inline)) {
     const int m = tid >> 1, half = tid & 1;
+    const uint8_t* src = sbase + static_cast<size_t>(source_row(m)) * nk;
     uint8_t* dst = s_scales + (m & 15) * 8 + (m >> 4);
     float* w = reinterpret_cast<float*>(s_scales + nk * kPfBM);
     for (int kb0 = 0; kb0 < nk; kb0 += 16) {
       uint8_t v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = my_scales[min(kb0 + 2 * i + half, nk - 1)];
+      for (int i = 0; i < 8; ++i) v[i] = src[min(kb0 + 2 * i + half, nk - 1)];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (kb0 + 2 * i + half < nk) dst[(kb0 + 2 * i + half) * kPfBM] = v[i];
@@ -187,47 +184,61 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
   auto body = [&](auto nmi_c) {
     constexpr int NMI = decltype(nmi_c)::value;
     constexpr int NMT = 2 * NMI;                  // 16-row tiles
+    // While slab kt is multiplied, the rows of slab kt+S travel to the LDS buffer slab kt-1 has left and the
+    // fragments of slab kt+S to the registers the last row pair has just finished with.  Vector memory retires
+    // in order, so what has landed is known by counting.  Slabs past the end refetch the last one.
+    constexpr int S = tl_depth(NMI), kSlab = 32 * NMI * kTlRowBytes, kWait = tl_wait(tl_younger(NMI));
+    uint32_t doff[NMI];   // byte offset of lane's piece of copy `it` inside k slab 0
+#pragma unroll
+    for (int it = 0; it < NMI; ++it)
+      doff[it] = source_row((wave * NMI + it) * 8 + l3) * ld + ((chunk0 ^ ((wave * NMI + it) & 1)) << 4);
+    auto stage_slab = [&](int slab, int buf) __attribute__((always_inline)) {
+      const uint8_t* sb = abase + static_cast<size_t>(slab) * kF8Block;
+#pragma unroll
+      for (int it = 0; it < NMI; ++it) {
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + buf * kSlab + (wave * NMI + it) * 1024);
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(doff[it]), "s"(sb), "s"(dst)
+                     : "memory");
+      }
+    };
+    fill_scales();
+    i32x4 wfrag[S][2][4];   // [stage][k half][16-row group]
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int st = 0; st < S; ++st) stage_slab(min(st, nk - 1), st);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int st = 0; st < S; ++st)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, min(st, nk - 1), h);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kWait);
+    __syncthreads();
+
     vf32x4 acc[NMT][4];
 #pragma unroll
     for (int mt = 0; mt < NMT; ++mt)
 #pragma unroll
       for (int g = 0; g < 4; ++g) acc[mt][g] = vf32x4{0.f, 0.f, 0.f, 0.f};
 
-    // While slab kt is multiplied, the rows of slab kt+2 travel to the third LDS buffer and the fragments of
-    // slab kt+2 to the registers the last row pair has just finished with.  Vector memory retires in order:
-    // "the copies of slab kt+1 have landed" is the 8 fragment loads of slab kt-1, the 4 copies and the 8
-    // fragment loads of slab kt still outstanding, vmcnt(20).  Slabs past the end refetch the last one.
-    i32x4 wfrag[2][2][4];   // [stage][k half][16-row group]
-    stage_slab(0, 0);
-    stage_slab(min(1, nk - 1), 1);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, min(st, nk - 1), h);
-    __builtin_amdgcn_sched_barrier(0);
-    fill_scales();
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(kWaitVm20);
-    __syncthreads();
-
     // fragment of lane (r, q), tile mt, half h: row 16*mt + r, position (q + 4h) ^ f(r)
     const int fsw = ((fr >> 1) & 7) ^ ((fr & 1) << 2);
     const int a_row = fr * kTlRowBytes, a_x = (fq ^ fsw) << 4;
-    int cur = 0, nxt2 = 2;
+    int cur = 0, ahead = S;   // buffer of slab kt, buffer of slab kt+S
     auto slab = [&](auto stage_c, int kt) {
       constexpr int st = decltype(stage_c)::value;
       constexpr int NP = NMT / 2;                 // pairs of 16-row tiles
-      const int kt2 = min(kt + 2, nk - 1);
-      const uint8_t* la = lds[cur] + a_row;
+      const int kts = min(kt + S, nk - 1);
+      const uint8_t* la = lds + cur * kSlab + a_row;
       const uint2 sb = *reinterpret_cast<const uint2*>(s_scales + kt * kPfBM + fr * 8);
       const float2 sw = *reinterpret_cast<const float2*>(s_scales + nk * kPfBM + kt * 8);
       const float sw0 = kGateUp ? sw.x : (wave < 2 ? sw.x : sw.y), sw1 = kGateUp ? sw.y : sw0;
       i32x4 fa[2][2][2];   // [parity][tile of the pair][half]
       if (NP == 1) {       // the copies go first, so that every height issues vector memory in the counted order
-        stage_slab(kt2, nxt2);
+        stage_slab(kts, ahead);
         __builtin_amdgcn_sched_barrier(0);
       }
       auto rd = [&](int pr, i32x4 (&f)[2][2]) __attribute__((always_inline)) {
@@ -260,10 +271,10 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
             constexpr int g = decltype(g_c)::value;
             mul(std::integral_constant<int, 2 * pr>{}, g_c, fa[pr & 1][0]);
             mul(std::integral_constant<int, 2 * pr + 1>{}, g_c, fa[pr & 1][1]);
-            if constexpr (pr == NP - 1) {       // last user of group g's fragments: request those of slab kt+2
+            if constexpr (pr == NP - 1) {       // last user of group g's fragments: request those of slab kt+S
               __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, kt2, h);
+              for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, kts, h);
               __builtin_amdgcn_sched_barrier(0);
             }
           };
@@ -272,8 +283,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
           group(std::integral_constant<int, 2>{});
           group(std::integral_constant<int, 3>{});
           __builtin_amdgcn_sched_barrier(0);
-          if (NP > 1 && pr == 0) {   // the copies of slab kt+2 go out once the matrix pipe has work
-            stage_slab(kt2, nxt2);
+          if (NP > 1 && pr == 0) {   // the copies of slab kt+S go out once the matrix pipe has work
+            stage_slab(kts, ahead);
             __builtin_amdgcn_sched_barrier(0);
           }
         }
@@ -282,18 +293,23 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
       pair(std::integral_constant<int, 1>{});
       pair(std::integral_constant<int, 2>{});
       pair(std::integral_constant<int, 3>{});
-      __builtin_amdgcn_s_waitcnt(kWaitVm20);
+      __builtin_amdgcn_s_waitcnt(kWait);
       __syncthreads();
-      cur = (cur == kPfStages - 1) ? 0 : cur + 1;
-      nxt2 = (nxt2 == kPfStages - 1) ? 0 : nxt2 + 1;
+      cur = (cur == S) ? 0 : cur + 1;
+      ahead = (ahead == S) ? 0 : ahead + 1;
     };
     int kt = 0;
-    for (; kt + 2 <= nk; kt += 2) {
+    for (; kt + S <= nk; kt += S) {
       slab(std::integral_constant<int, 0>{}, kt);
       slab(std::integral_constant<int, 1>{}, kt + 1);
+      if constexpr (S > 2) slab(std::integral_constant<int, 2>{}, kt + 2);
+      if constexpr (S > 3) slab(std::integral_constant<int, 3>{}, kt + 3);
     }
     if (kt < nk) slab(std::integral_constant<int, 0>{}, kt);
-    __builtin_amdgcn_s_waitcnt(kWaitVm0);  // no copy may land in LDS after the epilogue starts to reuse it
+    if (S > 2 && kt + 1 < nk) slab(std::integral_constant<int, 1>{}, kt + 1);
+    if constexpr (S > 3)
+      if (kt + 2 < nk) slab(std::integral_constant<int, 2>{}, kt + 2);
+    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);  // no copy may land in LDS after the epilogue starts to reuse it
     __syncthreads();
 
     // ---- epilogue ----------------------------------------------------------------
@@ -318,7 +334,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
         if (fq == 0) s_amax[wave][mt * 16 + fr] = m;
       }
       __syncthreads();
-      uint8_t* st = &lds[0][0];      // 128 rows x 128 bytes, 16-byte chunks swizzled by row
+      uint8_t* st = lds;             // 128 rows x 128 bytes, 16-byte chunks swizzled by row
 #pragma unroll
       for (int mt = 0; mt < NMT; ++mt) {
         const int m = mt * 16 + fr;
@@ -347,7 +363,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
       }
     } else {
       // 16-bit rows times their factor, staged per wavefront in two 32-column passes into 16-byte stores
-      uint8_t* st = &lds[0][0] + wave * (kPfBM * 64);
+      uint8_t* st = lds + wave * (kPfBM * 64);
       uint16_t* out = static_cast<uint16_t*>(dense ? a.p.out_s : a.p.out_r);
       // whole 16-byte stores need rows that start on 16-byte boundaries
       const bool whole = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
