@@ -184,6 +184,6 @@ int f8_rows(const F8Product& p, bool gateup, bool routed, bool dense, hipStream_
 struct PfQueues;
 int f8_tile_gateup(const F8Product& p, const PfQueues& q, void* h, void* hs, void* sh, void* shs, hipStream_t st);
 int f8_tile_down(const F8Product& p, const PfQueues& q, hipStream_t st);
-int f8_tile_linear(const F8Product& p, hipStream_t st);
+int f8_tile_linear(const F8Product& p, int tile_rows, hipStream_t st);
 
 }  // namespace sparse

@@ -33,6 +33,20 @@ static bool ffn_tiles(int T, int K, int E, int H, int I) {
   return path == 2 || T * h * K * I > 7.0 * (1 << 26) + 4.0 * h * E * I;
 }
 
+// Rows per tile: the fewest of 32, 64, 128 with which the call's tiles still fit on the device together (two on a
+// compute unit).  A launch of fewer tiles than that is as long as its longest tile, and one of 32 rows takes half
+// the time of one of 128; more tiles than that cost what the weights' second reading costs.
+static int tile_rows(int64_t rows, int segments, int column_tiles) {
+  for (int r = 32; r < kPfBM; r *= 2)
+    if ((rows / r + segments) * column_tiles <= 512) return r;
+  return kPfBM;
+}
+static int ffn_tile_rows(int T, int K, int E, int H, int I) {
+  // half of the segments' last tiles are half empty; gate/up has the more tiles where it has fewer columns
+  const int nt_gu = (I + kPfBR / 2 - 1) / (kPfBR / 2), nt_dn = (H + kPfBR - 1) / kPfBR;
+  return tile_rows(static_cast<int64_t>(T) * K, E / 2, nt_gu > nt_dn ? nt_gu : nt_dn);
+}
+
 static inline size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 constexpr int kF8MaxDim = 1 << 16;      // the tile kernel keeps a scale byte per row and block in LDS
@@ -87,7 +101,7 @@ static FfnWs ffn_ws(void* ws, int T, int K, int E, int nseg, int H, int I, int I
     if (Is > 0) w.sh = take_rows(c, T, Is);
   }
   if (ffn_tiles(T, K, E, H, I)) {
-    w.tiles = c.take(prefill_queue_ws_bytes(T, K, nseg, H, I, Is));
+    w.tiles = c.take(prefill_queue_ws_bytes(T, K, nseg, H, I, Is, ffn_tile_rows(T, K, E, H, I)));
   } else {
     w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
     if (Is > 0) w.shf = static_cast<float*>(c.take(static_cast<size_t>(T) * Is * sizeof(float)));
@@ -169,7 +183,8 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   p.dtype = dtype;
   p.pow2 = pow2_scales;
   if (T <= kF8FewRows) return f8_few(p, source, false, false, true, st);
-  return linear_tiles(T, weight->rows) ? f8_tile_linear(p, st) : f8_rows(p, false, false, true, st);
+  return linear_tiles(T, weight->rows) ? f8_tile_linear(p, tile_rows(T, 0, (weight->rows + kPfBR - 1) / kPfBR), st)
+                                       : f8_rows(p, false, false, true, st);
 }
 
 size_t sparse_hip_fp8_slot_bytes(int H, int I) {
@@ -238,7 +253,8 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   PfQueues queues = {};
   if (tiles) {
     PfxMapArgs queue_args;
-    queues = prefill_queue_args(experts->expert_slot_dev, seg_offsets_dev, *segs, T, K, H, I, Is, w.tiles, &queue_args);
+    queues = prefill_queue_args(experts->expert_slot_dev, seg_offsets_dev, *segs, T, K, H, I, Is, w.tiles, &queue_args,
+                                ffn_tile_rows(T, K, E, H, I));
     rc = f8_quantize_and_queue({x_dev, T, H, w.x.values, w.x.scales}, dtype, queue_args, st);
   } else if (!few) {
     rc = f8_quantize({x_dev, T, H, w.x.values, w.x.scales}, {}, dtype, st);

@@ -49,7 +49,7 @@ struct TileArgs {
   const PfTile* map;       // NULL: dense operands only, the tile comes from the block number
   const int32_t* qhdr;
   uint32_t topk_magic;     // ceil(2^32 / topk); 0 for topk == 1
-  int32_t mt, nt;          // row and column tiles when map is NULL
+  int32_t mt, nt, rows;    // row and column tiles when map is NULL, rows per tile
   // gate/up: where the quantised rows go
   uint8_t *q_r, *qs_r, *q_s, *qs_s;
 };
@@ -86,8 +86,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
     const int end = static_cast<int>(static_cast<int64_t>(total) * (xcd + 1) / kPfXcds);
     if (first + rank >= end) return;
     bn = (first + rank) / a.mt;
-    r0 = (first + rank - bn * a.mt) * kPfBM;
-    M = min(kPfBM, a.p.T - r0);
+    r0 = (first + rank - bn * a.mt) * a.rows;
+    M = min(a.rows, a.p.T - r0);
     slot = -1;
   }
   if (M <= 0) return;
@@ -454,10 +454,11 @@ int f8_tile_down(const F8Product& p, const PfQueues& q, hipStream_t st) {
   return launch_tile<false>(a, queue_grid(q.cap_dn), st);
 }
 
-int f8_tile_linear(const F8Product& p, hipStream_t st) {
+int f8_tile_linear(const F8Product& p, int tile_rows, hipStream_t st) {
   TileArgs a = {};
   a.p = p;
-  a.mt = (p.T + kPfBM - 1) / kPfBM;
+  a.rows = tile_rows;
+  a.mt = (p.T + tile_rows - 1) / tile_rows;
   a.nt = (p.Ns + kPfBR - 1) / kPfBR;
   const int64_t total = static_cast<int64_t>(a.mt) * a.nt;
   SP_REQUIRE(total < (1ll << 30), "fp8_linear: too many tiles");

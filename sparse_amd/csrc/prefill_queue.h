@@ -19,6 +19,7 @@ struct PfxMapArgs {
   int32_t mt_shared;       // row tiles of the shared expert
   int32_t T;               // tokens (rows of the shared expert)
   int32_t cap_gu, cap_dn;  // entries in each map
+  int32_t tile_rows;       // rows per tile, kPfBM or fewer
 };
 
 // Share x of n items cut into kPfXcds contiguous shares starts here.
@@ -47,7 +48,7 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
     const int e = (a.segs.eids_dev != nullptr) ? a.segs.eids_dev[tid] : a.segs.eids[tid];
     r0 = a.seg_offsets[e];
     rows = a.seg_offsets[e + 1] - r0;
-    mt = (rows + kPfBM - 1) / kPfBM;
+    mt = (rows + a.tile_rows - 1) / a.tile_rows;
     slot = (a.segs.eids_dev != nullptr) ? a.expert_slot[e] : a.segs.slots[tid];
   }
   // inclusive scan: within the wavefronts, then over their totals
@@ -74,7 +75,7 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
         const int g = g0 + bm;
         const int x = pfx_share_of(R, g);
         const int pos = pfx_queue_base(R, S, x) + (pfx_start(S, x + 1) - pfx_start(S, x)) + (g - pfx_start(R, x));
-        if (pos < cap) map[pos] = PfTile{slot, r0 + bm * kPfBM, min(kPfBM, rows - bm * kPfBM), bn};
+        if (pos < cap) map[pos] = PfTile{slot, r0 + bm * a.tile_rows, min(a.tile_rows, rows - bm * a.tile_rows), bn};
       }
     }
     return;
@@ -107,7 +108,7 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
       local = h - pfx_start(S, x);
     }
     const int pos = pfx_queue_base(R, S, x) + local;
-    if (pos < cap) map[pos] = PfTile{-1, bm * kPfBM, min(kPfBM, a.T - bm * kPfBM), bn};
+    if (pos < cap) map[pos] = PfTile{-1, bm * a.tile_rows, min(a.tile_rows, a.T - bm * a.tile_rows), bn};
   }
   if (tid == 0) map[0] = PfTile{0, 0, 0, 0};
   if (tid < kPfXcds) {
@@ -117,19 +118,19 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
   }
 }
 
-inline int pfx_max_mtiles(int Ttok, int K, int nseg) { return (Ttok * K + kPfBM - 1) / kPfBM + nseg; }
+inline int pfx_max_mtiles(int Ttok, int K, int nseg, int tile_rows) { return (Ttok * K + tile_rows - 1) / tile_rows + nseg; }
 
 struct PfxLayout {
   int nt_gu, nt_dn, nts_gu, nts_dn, mt_shared, cap_gu, cap_dn;
 };
-inline PfxLayout pfx_layout(int Ttok, int K, int nseg, int H, int I, int Is) {
+inline PfxLayout pfx_layout(int Ttok, int K, int nseg, int H, int I, int Is, int tile_rows) {
   PfxLayout l;
   l.nt_gu = (I + kPfBR / 2 - 1) / (kPfBR / 2);
   l.nt_dn = (H + kPfBR - 1) / kPfBR;
   l.nts_gu = Is > 0 ? (Is + kPfBR / 2 - 1) / (kPfBR / 2) : 0;
   l.nts_dn = Is > 0 ? l.nt_dn : 0;
-  l.mt_shared = Is > 0 ? (Ttok + kPfBM - 1) / kPfBM : 0;
-  const int mt = nseg > 0 ? pfx_max_mtiles(Ttok, K, nseg) : 0;
+  l.mt_shared = Is > 0 ? (Ttok + tile_rows - 1) / tile_rows : 0;
+  const int mt = nseg > 0 ? pfx_max_mtiles(Ttok, K, nseg, tile_rows) : 0;
   l.cap_gu = 1 + mt * l.nt_gu + l.mt_shared * l.nts_gu;
   l.cap_dn = 1 + mt * l.nt_dn + l.mt_shared * l.nts_dn;
   return l;
@@ -137,16 +138,17 @@ inline PfxLayout pfx_layout(int Ttok, int K, int nseg, int H, int I, int Is) {
 
 constexpr size_t kPfWsHeader = 256;   // two launches x 16 ints, padded
 
-inline size_t prefill_queue_ws_bytes(int Ttok, int K, int nseg, int H, int I, int Is) {
-  const PfxLayout l = pfx_layout(Ttok, K, nseg, H, I, Is);
+inline size_t prefill_queue_ws_bytes(int Ttok, int K, int nseg, int H, int I, int Is, int tile_rows = kPfBM) {
+  const PfxLayout l = pfx_layout(Ttok, K, nseg, H, I, Is, tile_rows);
   return kPfWsHeader + (static_cast<size_t>(l.cap_gu) + l.cap_dn) * sizeof(PfTile);
 }
 
 // The arguments that build both launches' queues of a call in `tile_ws` (prefill_queue_ws_bytes), and where
 // they will be.
 inline PfQueues prefill_queue_args(const int32_t* expert_slot, const int32_t* seg_offsets, const sparse_hip_seglist& segs,
-                                   int Ttok, int K, int H, int I, int Is, void* tile_ws, PfxMapArgs* args) {
-  const PfxLayout l = pfx_layout(Ttok, K, segs.n, H, I, Is);
+                                   int Ttok, int K, int H, int I, int Is, void* tile_ws, PfxMapArgs* args,
+                                   int tile_rows = kPfBM) {
+  const PfxLayout l = pfx_layout(Ttok, K, segs.n, H, I, Is, tile_rows);
   int32_t* hdr = static_cast<int32_t*>(tile_ws);
   PfTile* map_gu = reinterpret_cast<PfTile*>(static_cast<uint8_t*>(tile_ws) + kPfWsHeader);
   PfTile* map_dn = map_gu + l.cap_gu;
@@ -165,6 +167,7 @@ inline PfQueues prefill_queue_args(const int32_t* expert_slot, const int32_t* se
   m.T = Ttok;
   m.cap_gu = l.cap_gu;
   m.cap_dn = l.cap_dn;
+  m.tile_rows = tile_rows;
   *args = m;
   return PfQueues{hdr, map_gu, map_dn, l.cap_gu, l.cap_dn};
 }

@@ -6,7 +6,7 @@
 
 namespace sparse {
 
-constexpr int kPfBM = 128;        // rows per tile
+constexpr int kPfBM = 128;        // rows per tile at most
 constexpr int kPfBR = 256;        // weight rows per tile
 constexpr int kPfBK = 64;         // k slab
 constexpr int kPfThreads = 256;
