@@ -10,18 +10,19 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 // Which kernels serve more than kF8FewRows rows: 0 by size, 1 the streaming ones, 2 the tiles.
 static std::atomic<int> g_path{0};
 
-// The streaming kernel reads the weights once for every 32 rows, the tile kernel once or twice in all, but it
-// starts slowly (10 us for its first tile, then 1.2 us a 128-wide slab while few tiles are there to overlap)
-// and reads weights that are used once at 4.5 TB/s where the streaming kernel reaches 6.  Measured on both
-// sides of the border, streaming / tiles:
-//   linear  2048 x 5632: 128 rows 21 / 29 us, 256 rows 34 / 29;  4096 x 4096: 128 rows 30 / 48, 256 rows 53 / 49
-//   experts 60 of 1408 x 2048, 4 a token, shared 5632: 64 tokens 108 / 126 us, 128 tokens 149 / 137
-//           16 of 704 x 1024, 3 a token: 256 tokens 38 / 41 us, 384 tokens 47 / 42
-//           8 of 704 x 2048, 2 a token, shared 1408: 128 tokens 38 / 42 us, 192 tokens 48 / 42
-static bool linear_tiles(int T, int N) {
+// The streaming kernel reads the weights once for every 32 rows; the tile kernel reads them once or twice in all,
+// but starts slowly (7 us, then 0.45 us a 128-wide slab while few tiles are there to overlap) and reads weights
+// that are used once at 4.5 TB/s where the streaming kernel reaches 6.  Measured on both sides of the border,
+// streaming / tiles:
+//   linear  2048 x 5632: 64 rows 13.3 / 14.3 us, 128 rows 21 / 14.8;  4096 x 4096: 64 rows 17 / 21, 128 rows 29 / 22
+//           1000 x 1418: 333 rows 11.8 / 12.5, 512 rows 15.1 / 12.7;  512 x 1024: 333 rows 8.3 / 8.8, 512 rows 9.6 / 9.0
+//   experts 60 of 1408 x 2048, 4 a token, shared 5632: 64 tokens 109 / 115 us, 96 tokens 131 / 121
+//           16 of 704 x 1024, 3 a token: 64 tokens 20.7 / 22.1, 128 tokens 25.8 / 22.9
+//           8 of 704 x 2048, 2 a token, shared 1408: 48 tokens 23.8 / 24.7, 96 tokens 32 / 25.4
+static bool linear_tiles(int T, int K, int N) {
   const int path = g_path.load(std::memory_order_relaxed);
   if (T <= kF8FewRows || path == 1) return false;
-  return path == 2 || static_cast<int64_t>((T + 31) / 32) * N > 28672;
+  return path == 2 || static_cast<double>((T + 31) / 32) * N > 10000.0 + 6.0e6 / K;
 }
 // (The routed experts decide, all of them, so that a layer whose experts are executed in several calls, or apart
 // from the shared one, takes the same kernels in each.)
@@ -30,7 +31,7 @@ static bool ffn_tiles(int T, int K, int E, int H, int I) {
   if (T <= kF8FewRows || path == 1) return false;
   // work of the rows against a fixed cost and one for the weights
   const double h = H;
-  return path == 2 || T * h * K * I > 7.0 * (1 << 26) + 4.0 * h * E * I;
+  return path == 2 || T * (h * K * I + 2.0e6) > 2.4e8 + 4.4 * h * E * I;
 }
 
 // Rows per tile: the fewest of 32, 64, 128 with which the call's tiles still fit on the device together (two on a
@@ -183,7 +184,7 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   p.dtype = dtype;
   p.pow2 = pow2_scales;
   if (T <= kF8FewRows) return f8_few(p, source, false, false, true, st);
-  return linear_tiles(T, weight->rows) ? f8_tile_linear(p, tile_rows(T, 0, (weight->rows + kPfBR - 1) / kPfBR), st)
+  return linear_tiles(T, weight->cols, weight->rows) ? f8_tile_linear(p, tile_rows(T, 0, (weight->rows + kPfBR - 1) / kPfBR), st)
                                        : f8_rows(p, false, false, true, st);
 }
 
