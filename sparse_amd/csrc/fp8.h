@@ -43,6 +43,13 @@ __device__ __forceinline__ float f8_row16_max(float v) {
   v = fmaxf(v, dpp_move<0x128, 0xf>(0.f, v));
   return v;
 }
+// ... over the 8 lanes of half a row.
+__device__ __forceinline__ float f8_row8_max(float v) {
+  v = fmaxf(v, dpp_move<0xb1, 0xf>(0.f, v));    // quad_perm 1,0,3,2
+  v = fmaxf(v, dpp_move<0x4e, 0xf>(0.f, v));    // quad_perm 2,3,0,1
+  v = fmaxf(v, dpp_move<0x141, 0xf>(0.f, v));   // row_half_mirror
+  return v;
+}
 // The magnitude that counts towards amax: NaN and infinities do not (they become NaN in 8 bits).
 __device__ __forceinline__ float f8_magnitude(float v) {
   const float a = fabsf(v);

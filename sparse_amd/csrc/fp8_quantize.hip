@@ -5,7 +5,8 @@
 namespace sparse {
 
 constexpr int kQzThreads = 256;
-constexpr int kQzLane = 8;                       // values per lane: 16 lanes make a run
+constexpr int kQzLane = 16;                      // values per lane: 8 lanes make a run
+constexpr int kQzLanes = kF8Block / kQzLane;     // lanes per run
 constexpr int kQzRuns = kQzThreads * kQzLane / kF8Block;
 
 struct QuantizeArgs {
@@ -21,22 +22,24 @@ template <typename T, bool kVec>
 __device__ __forceinline__ void quantize_block(const QuantizeArgs& a, uint32_t block) {
   const int which = block >= a.first_blocks;
   if (which) block -= a.first_blocks;
-  const int64_t run = static_cast<int64_t>(block) * kQzRuns + (threadIdx.x >> 4);
-  if (run >= a.runs[which]) return;              // 16 lanes leave together
+  const int64_t run = static_cast<int64_t>(block) * kQzRuns + threadIdx.x / kQzLanes;
+  if (run >= a.runs[which]) return;              // a run's lanes leave together
   const int K = a.K[which], nb = a.nb[which];
   // (a row's number fits 32 bits; so does almost every run's, and the short division is several times faster)
   const int64_t t = run < (1ll << 32) ? static_cast<uint32_t>(run) / static_cast<uint32_t>(nb) : run / nb;
-  const int k = static_cast<int>(run - t * nb) * kF8Block + (threadIdx.x & 15) * kQzLane;
+  const int k = static_cast<int>(run - t * nb) * kF8Block + (threadIdx.x % kQzLanes) * kQzLane;
   const T* row = static_cast<const T*>(a.x[which]) + t * K;
   float v[kQzLane];
   if (kVec) {
-    // a multiple of 8: a lane's eight values are all inside the row or all behind it
-    typedef T vec __attribute__((ext_vector_type(kQzLane)));
-    vec u = {};
-    if (k < K) u = *reinterpret_cast<const vec*>(row + k);
+    // a multiple of 8: eight of a lane's values are all inside the row or all behind it
+    typedef T vec __attribute__((ext_vector_type(8)));
+    vec u[2] = {};
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      if (k + 8 * c < K) u[c] = *reinterpret_cast<const vec*>(row + k + 8 * c);
 #pragma unroll
     for (int j = 0; j < kQzLane; ++j) {
-      const T e = u[j];
+      const T e = u[j >> 3][j & 7];
       v[j] = Elem<T>::load(&e);
     }
   } else {
@@ -46,14 +49,14 @@ __device__ __forceinline__ void quantize_block(const QuantizeArgs& a, uint32_t b
   float m = 0.f;
 #pragma unroll
   for (int j = 0; j < kQzLane; ++j) m = fmaxf(m, f8_magnitude(v[j]));
-  m = f8_row16_max(m);
+  m = f8_row8_max(m);
   const int s = f8_exponent(m);
   const float inv = f8_inverse(s);
-  uint2 q;
-  q.x = f8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-  q.y = f8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-  *reinterpret_cast<uint2*>(a.values[which] + t * nb * kF8Block + k) = q;
-  if ((threadIdx.x & 15) == 0) a.scales[which][run] = static_cast<uint8_t>(s + kF8Bias);
+  uint32_t q[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) q[j] = f8_pack4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+  *reinterpret_cast<uint4*>(a.values[which] + t * nb * kF8Block + k) = make_uint4(q[0], q[1], q[2], q[3]);
+  if (threadIdx.x % kQzLanes == 0) a.scales[which][run] = static_cast<uint8_t>(s + kF8Bias);
 }
 
 template <typename T, bool kVec>
@@ -83,7 +86,7 @@ static int quantize_as(const F8Quantize& a, const F8Quantize& b, const PfxMapArg
     q.values[i] = static_cast<uint8_t*>(m.values);
     q.scales[i] = static_cast<uint8_t*>(m.scales);
     blocks[i] = (q.runs[i] + kQzRuns - 1) / kQzRuns;
-    vec = vec && m.K % kQzLane == 0 && (reinterpret_cast<uintptr_t>(m.x) & 15) == 0;
+    vec = vec && m.K % 8 == 0 && (reinterpret_cast<uintptr_t>(m.x) & 15) == 0;
   }
   SP_REQUIRE(blocks[0] + blocks[1] < (1ll << 31) - (1 << 20), "fp8_quantize: too many rows");
   if (blocks[0] + blocks[1] == 0) return SPARSE_HIP_OK;

@@ -44,7 +44,7 @@ class Rows:
     __slots__ = ("data", "scales", "cols", "dtype")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, cols: int, dtype: torch.dtype) -> None:
-        self.data, self.scales, self.cols, self.dtype = data, scales, int(cols), dtype
+        self.data, self.scales, self.cols, self.dtype = data, scales, cols, dtype
 
     @property
     def values(self) -> torch.Tensor:
@@ -193,7 +193,8 @@ def linear(x: Union[torch.Tensor, Rows], weight: Weight, out: Optional[torch.Ten
         out = src.new_empty((T, weight.rows), dtype=dtype)
     else:
         _need(out, "out", dtype, (T, weight.rows))
-    _same_device(index, weight.data, out)
+        _same_device(index, out)
+    _same_device(index, weight.data)
     lib = _lib.load()
     if rows:
         rc = call_on(index, lib.sparse_hip_fp8_linear, None, src.data_ptr(), x.scales.data_ptr(), dtype_code(dtype), T,

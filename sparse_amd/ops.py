@@ -17,13 +17,13 @@ from ._lru import LruTable
 from ._lib import BF16, F16, F32, DECODE_MAX_TOKENS, Experts, SegList
 
 
+_DTYPE_CODES = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
+
+
 def dtype_code(dtype: torch.dtype) -> int:
-    if dtype == torch.bfloat16:
-        return BF16
-    if dtype == torch.float16:
-        return F16
-    if dtype == torch.float32:
-        return F32
+    code = _DTYPE_CODES.get(dtype)
+    if code is not None:
+        return code
     raise ValueError(f"unsupported dtype {dtype}: the MoE kernels take bfloat16, float16 or float32")
 
 
@@ -55,14 +55,16 @@ def _need(t: torch.Tensor, name: str, dtype=None, shape=None) -> None:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-# the stream handle without building a Stream object around it (0.1 instead of 1.1 us)
+# the stream handle without building a Stream object around it (0.1 instead of 1.1 us), the current device
+# without asking whether the runtime is up (device tensors are at hand)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def call_on(index: int, fn, *args) -> int:
     """``fn(*args, stream)`` with device ``index`` current, on its current stream."""
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         return fn(*args, _raw_stream(index))
     with torch.cuda.device(index):
         return fn(*args, _raw_stream(index))
@@ -152,19 +154,23 @@ def gate_select(logits: torch.Tensor, k: int, score: str = "softmax", bias: Opti
         raise ValueError(f"group_score must be max|top2, got {group_score}")
     T, E = logits.shape
     k = int(k)
+    if k < 1:
+        raise ValueError(f"k must be at least 1, got {k}")
     odt = out_dtype or logits.dtype
     index = logits.get_device()
     if bias is not None:
         _need(bias, "bias", torch.float32, (E,))
+        _same_device(index, bias)
     if topv is None:
-        topv = logits.new_empty((T, max(0, k)), dtype=odt)
+        topv = logits.new_empty((T, k), dtype=odt)
     else:
         _need(topv, "topv", odt, (T, k))
+        _same_device(index, topv)
     if topi is None:
-        topi = logits.new_empty((T, max(0, k)), dtype=torch.int64)
+        topi = logits.new_empty((T, k), dtype=torch.int64)
     else:
         _need(topi, "topi", torch.int64, (T, k))
-    _same_device(index, bias, topv, topi)
+        _same_device(index, topi)
     rc = call_on(index, _lib.load().sparse_hip_gate_select, logits.data_ptr(), dtype_code(logits.dtype), _ptr(bias), T, E, k,
                  SELECT_SCORE[score], n_group, topk_group, SELECT_GROUP[group_score], bool(renorm), scale, dtype_code(odt),
                  topv.data_ptr(), topi.data_ptr())
