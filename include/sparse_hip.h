@@ -490,8 +490,8 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
  * and, unless shared_down_w is NULL, shared[t] likewise on the shared expert's matrices over all tokens,
  * times sigmoid(shared_gate[t]) when shared_gate_dev is not NULL.  Rows of segments that are not in `segs`
  * are left untouched; segs->n == 0: the shared expert alone.
- * `experts` describes the slab as for 16-bit weights, with dtype that of the activations (bf16 or fp16); a
- * slot holds gate, up and down as matrices above and behind them their scales in the same order,
+ * `experts` describes the slab as for 16-bit weights, with dtype that of the activations (bf16 or fp16), and
+ * expert_slot_dev may be NULL: expert e is in slot e.  A slot holds gate, up and down as matrices above and behind them their scales in the same order,
  * sparse_hip_fp8_slot_bytes(H, I) bytes in all.  H, I and Is are multiples of 64.  x [T,H], topv [T,K],
  * parts [T*K,H], shared_gate [T], shared [T,H] in that dtype.  `pow2_scales` as above, for all matrices of
  * the call.  `ws_dev`:

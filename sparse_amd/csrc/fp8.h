@@ -177,6 +177,66 @@ struct F8Product {
   int32_t pow2;                                     // every weight scale is a power of two
   sparse_hip_seglist segs;
 };
+
+// Which 16 output columns of which matrix a workgroup of the streaming kernels owns, and for which rows.
+struct F8Where {
+  const uint8_t *w0, *w1;      // the tile's panels
+  const float *s0, *s1;        // and their scales
+  int nb, K, N, n0, r0, M;
+  bool dense;
+};
+// At the start of a kernel every load waits a microsecond, and the compiler would place each behind the wait for
+// the one before.  Naming values to an empty statement has them loaded together: the kernel's arguments, then
+// the segment count with the expert, then slot with offsets.
+__device__ __forceinline__ bool f8_where(const F8Product& a, int block, int tiles_r, int tiles_s, F8Where& w) {
+  int tile;
+  w.dense = block < tiles_s;
+  if (w.dense) {
+    asm volatile("" ::"s"(a.w0), "s"(a.w1), "s"(a.s0), "s"(a.s1), "s"(a.Ks), "s"(a.Ns), "s"(a.T), "s"(a.act_s));
+    tile = block;
+    w.K = a.Ks;
+    w.N = a.Ns;
+    w.r0 = 0;
+    w.M = a.T;
+    w.w0 = a.w0;
+    w.w1 = a.w1;
+    w.s0 = a.s0;
+    w.s1 = a.s1;
+  } else {
+    const int b = block - tiles_s, si = b / tiles_r;
+    tile = b - si * tiles_r;
+    asm volatile("" ::"s"(a.segs.eids_dev), "s"(a.segs.count_dev), "s"(a.segs.n), "s"(a.expert_slot), "s"(a.seg_offsets),
+                 "s"(a.slab), "s"(a.slot_stride), "s"(a.off0), "s"(a.soff0), "s"(a.Kr), "s"(a.Nr), "s"(a.act_r), "s"(a.perm));
+    int eid, slot_id;
+    if (a.segs.eids_dev != nullptr) {
+      const int count = a.segs.count_dev[0];
+      eid = a.segs.eids_dev[si];
+      asm volatile("" ::"s"(count), "s"(eid));
+      if (si >= min(count, a.segs.n)) return false;
+      slot_id = a.expert_slot != nullptr ? a.expert_slot[eid] : eid;
+    } else {
+      eid = a.segs.eids[si];
+      slot_id = a.segs.slots[si];
+    }
+    w.r0 = a.seg_offsets[eid];
+    w.M = a.seg_offsets[eid + 1] - w.r0;
+    w.K = a.Kr;
+    w.N = a.Nr;
+    const uint8_t* slot = a.slab + static_cast<uint64_t>(slot_id) * a.slot_stride;
+    w.w0 = slot + a.off0;
+    w.w1 = slot + a.off1;
+    w.s0 = reinterpret_cast<const float*>(slot + a.soff0);
+    w.s1 = reinterpret_cast<const float*>(slot + a.soff1);
+  }
+  w.n0 = tile * 16;
+  w.nb = (w.K + kF8Block - 1) / kF8Block;
+  const size_t panel = static_cast<size_t>(tile) * w.nb * kF8TileBytes, scales = static_cast<size_t>(w.n0 / kF8Block) * w.nb;
+  w.w0 += panel;
+  w.w1 += panel;
+  w.s0 += scales;
+  w.s1 += scales;
+  return true;
+}
 // Two rows at most: gate/up (SwiGLU of two products, fp32 out) or a single product, of rows that are
 // quantised on the way in (from the 16-bit type, from fp32) or were before.
 constexpr int kF8FewRows = 2;

@@ -224,7 +224,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
     SP_REQUIRE(topv_dev && perm_dev && seg_offsets_dev && parts_dev, "%s: NULL pointer", fn);
     SP_REQUIRE(aligned16(parts_dev), "%s: parts must be 16-byte aligned", fn);
     if (segs->eids_dev != nullptr) {
-      SP_REQUIRE(segs->count_dev != nullptr && experts->expert_slot_dev != nullptr, "%s: a device segment list needs a count and expert_slot_dev", fn);
+      SP_REQUIRE(segs->count_dev != nullptr, "%s: a device segment list needs a count", fn);
     } else {
       for (int i = 0; i < segs->n; ++i)
         SP_REQUIRE(segs->eids[i] >= 0 && segs->eids[i] < E && segs->slots[i] >= 0, "%s: segment %d names expert %d in slot %d", fn, i,

@@ -104,64 +104,23 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
   __shared__ __attribute__((aligned(16))) uint8_t lds[kStage > kSums ? kStage : kSums];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, q = lane >> 4;
-  const bool dense = static_cast<int>(blockIdx.x) < tiles_s;
-
-  const uint8_t *w0, *w1;
-  const float *s0, *s1;
-  int K, N, tile, M, r0 = 0;
-  if (dense) {
-    tile = blockIdx.x;
-    K = a.Ks;
-    N = a.Ns;
-    M = a.T;
-    w0 = a.w0;
-    w1 = a.w1;
-    s0 = a.s0;
-    s1 = a.s1;
-  } else {
-    const int b = blockIdx.x - tiles_s, si = b / tiles_r;
-    tile = b - si * tiles_r;
-    int eid, slot_id;
-    if (a.segs.eids_dev != nullptr) {
-      if (si >= min(a.segs.count_dev[0], a.segs.n)) return;
-      eid = a.segs.eids_dev[si];
-      slot_id = a.expert_slot[eid];
-    } else {
-      eid = a.segs.eids[si];
-      slot_id = a.segs.slots[si];
-    }
-    K = a.Kr;
-    N = a.Nr;
-    r0 = a.seg_offsets[eid];
-    M = a.seg_offsets[eid + 1] - r0;
-    const uint8_t* slot = a.slab + static_cast<uint64_t>(slot_id) * a.slot_stride;
-    w0 = slot + a.off0;
-    w1 = slot + a.off1;
-    s0 = reinterpret_cast<const float*>(slot + a.soff0);
-    s1 = reinterpret_cast<const float*>(slot + a.soff1);
-  }
-  M = min(M, kF8FewRows);                   // (the ids of a token are distinct: a segment has T rows at most)
-  if (M <= 0) return;
-  const int nb = (K + kF8Block - 1) / kF8Block;
-  const int n0 = tile * 16;
+  F8Where own;
+  if (!f8_where(a, blockIdx.x, tiles_r, tiles_s, own)) return;
+  const bool dense = own.dense;
+  const int nb = own.nb, K = own.K, N = own.N, n0 = own.n0, r0 = own.r0;
   const uint8_t* wp[NM];
   const float* sp[NM];
 #pragma unroll
   for (int mi = 0; mi < NM; ++mi) {
-    wp[mi] = (mi ? w1 : w0) + static_cast<size_t>(tile) * nb * kF8TileBytes + lane * 16;
-    sp[mi] = (mi ? s1 : s0) + static_cast<size_t>(n0 / kF8Block) * nb;
+    wp[mi] = (mi ? own.w1 : own.w0) + lane * 16;
+    sp[mi] = mi ? own.s1 : own.s0;
   }
+  const int M = min(own.M, kF8FewRows);      // (the ids of a token are distinct: a segment has T rows at most)
+  if (M <= 0) return;
 
   vf32x4 acc[NM];
 #pragma unroll
   for (int mi = 0; mi < NM; ++mi) acc[mi] = vf32x4{0.f, 0.f, 0.f, 0.f};
-
-  // The factor of the row whose sum this lane stores at the end, asked for now.
-  float factor = 1.f;
-  if (!kGateUp && wave == 0 && r < M) {
-    if (!dense) factor = F::from_bits(static_cast<const uint16_t*>(a.topv)[a.perm[r0 + r]]);
-    else if (a.gate_s != nullptr) factor = F::from_bits(static_cast<const uint16_t*>(a.gate_s)[r0 + r]);
-  }
 
   // ---- the chunks --------------------------------------------------------------------------
   // Two register stages in turn: while a chunk is multiplied the next one's loads are in flight.  Loads
@@ -183,14 +142,20 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
         // read once per launch: a non-temporal load leaves the caches to the activations
         st.w[i][mi][0] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(p));
         st.w[i][mi][1] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(p + 1024));
-        st.ws[i][mi] = sp[mi][kb];
       }
     }
+  };
+  auto load_scales = [&](Stage& st, int chunk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < KW; ++i)
+#pragma unroll
+      for (int mi = 0; mi < NM; ++mi) st.ws[i][mi] = sp[mi][min(chunk * KC + wave + i * kFwWaves, nb - 1)];
   };
   auto load_rows = [&](Stage& st, int chunk) __attribute__((always_inline)) {   // (a second row that is not there repeats the first)
     const int m = min(my_m, M - 1), kb = min(chunk * KC + my_kb, nb - 1);
     size_t row = r0 + m;
-    if (!dense && a.gather) row = static_cast<uint32_t>(a.perm[r0 + m]) / static_cast<uint32_t>(a.topk);
+    if (!dense && a.gather)                      // (one token: every row is its)
+      row = a.T == 1 ? 0 : static_cast<uint32_t>(a.perm[r0 + m]) / static_cast<uint32_t>(a.topk);
     st.src.load(dense ? a.act_s : a.act_r, dense ? a.act_ss : a.act_rs, row, K, nb, kb, gl * 8, vec != 0);
   };
   auto use = [&](const Stage& st, int chunk, uint8_t* buf) __attribute__((always_inline)) {
@@ -232,23 +197,36 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
   __builtin_amdgcn_sched_barrier(0);
   load_weights(s1_, 1);
   __builtin_amdgcn_sched_barrier(0);
+  load_scales(s0_, 0);
+  load_scales(s1_, 1);
+  // The factor of the row whose sum this lane stores at the end, asked for once the loads of
+  // the first chunks are on their way.
+  float factor = 1.f;
+  if (!kGateUp && wave == 0 && r < M) {
+    if (!dense) factor = F::from_bits(static_cast<const uint16_t*>(a.topv)[a.perm[r0 + r]]);
+    else if (a.gate_s != nullptr) factor = F::from_bits(static_cast<const uint16_t*>(a.gate_s)[r0 + r]);
+  }
+  __builtin_amdgcn_sched_barrier(0);
   int c = 0;
   for (; c + 4 <= chunks; c += 2) {      // (no branch in here: the waits count what is in flight)
     use(s0_, c, buf0);
     __builtin_amdgcn_sched_barrier(0);
     load_rows(s0_, c + 2);
     load_weights(s0_, c + 2);
+    load_scales(s0_, c + 2);
     __builtin_amdgcn_sched_barrier(0);
     use(s1_, c + 1, buf1);
     __builtin_amdgcn_sched_barrier(0);
     load_rows(s1_, c + 3);
     load_weights(s1_, c + 3);
+    load_scales(s1_, c + 3);
     __builtin_amdgcn_sched_barrier(0);
   }
   use(s0_, c, buf0);                     // one to three chunks are left
   if (c + 2 < chunks) {
     load_rows(s0_, c + 2);
     load_weights(s0_, c + 2);
+    load_scales(s0_, c + 2);
   }
   if (c + 1 < chunks) use(s1_, c + 1, buf1);
   if (c + 2 < chunks) use(s0_, c + 2, buf0);

@@ -23,73 +23,21 @@ __global__ __launch_bounds__(kRwThreads) void f8_rows_kernel(const F8Product a, 
   __shared__ vf32x4 red[kRwWaves][NTmax * NM][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, q = lane >> 4;
-  const bool dense = static_cast<int>(blockIdx.x) < tiles_s;
-
-  const uint8_t *w0, *w1;
-  const float *s0, *s1;
-  int K, N, tile, M, r0 = 0;
-  if (dense) {
-    tile = blockIdx.x;
-    K = a.Ks;
-    N = a.Ns;
-    M = a.T;
-    w0 = a.w0;
-    w1 = a.w1;
-    s0 = a.s0;
-    s1 = a.s1;
-  } else {
-    const int b = blockIdx.x - tiles_s, si = b / tiles_r;
-    tile = b - si * tiles_r;
-    int eid, slot_id;
-    if (a.segs.eids_dev != nullptr) {
-      if (si >= min(a.segs.count_dev[0], a.segs.n)) return;
-      eid = a.segs.eids_dev[si];
-      slot_id = a.expert_slot[eid];
-    } else {
-      eid = a.segs.eids[si];
-      slot_id = a.segs.slots[si];
-    }
-    K = a.Kr;
-    N = a.Nr;
-    r0 = a.seg_offsets[eid];
-    M = a.seg_offsets[eid + 1] - r0;
-    const uint8_t* slot = a.slab + static_cast<uint64_t>(slot_id) * a.slot_stride;
-    w0 = slot + a.off0;
-    w1 = slot + a.off1;
-    s0 = reinterpret_cast<const float*>(slot + a.soff0);
-    s1 = reinterpret_cast<const float*>(slot + a.soff1);
-  }
-  const int m0 = blockIdx.y * 16 * NTmax;
-  M = min(M - m0, 16 * NTmax);
-  if (M <= 0) return;
-  r0 += m0;
-  const int nb = (K + kF8Block - 1) / kF8Block;
-  const int n0 = tile * 16;
+  F8Where own;
+  if (!f8_where(a, blockIdx.x, tiles_r, tiles_s, own)) return;
+  const bool dense = own.dense;
+  const int nb = own.nb, N = own.N, n0 = own.n0;
   const uint8_t* wp[NM];
   const float* sp[NM];
 #pragma unroll
   for (int mi = 0; mi < NM; ++mi) {
-    wp[mi] = (mi ? w1 : w0) + static_cast<size_t>(tile) * nb * kF8TileBytes + lane * 16;
-    sp[mi] = (mi ? s1 : s0) + static_cast<size_t>(n0 / kF8Block) * nb;
+    wp[mi] = (mi ? own.w1 : own.w0) + lane * 16;
+    sp[mi] = mi ? own.s1 : own.s0;
   }
+  const int m0 = blockIdx.y * 16 * NTmax, M = min(own.M - m0, 16 * NTmax), r0 = own.r0 + m0;
+  if (M <= 0) return;
   auto body = [&](auto nt_c) __attribute__((always_inline)) {
   constexpr int NT = decltype(nt_c)::value;
-  const uint8_t *xp[NT], *xs[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int m = min(nt * 16 + r, M - 1);       // rows past the end repeat the last and are not stored
-    size_t row = r0 + m;
-    if (!dense && a.gather) row = static_cast<uint32_t>(a.perm[r0 + m]) / static_cast<uint32_t>(a.topk);
-    xp[nt] = (dense ? a.act_s : a.act_r) + row * nb * kF8Block + q * 32;
-    xs[nt] = (dense ? a.act_ss : a.act_rs) + row * nb;
-  }
-  const int my_m = wave * 16 + r;                // wavefront nt stores row group nt
-  float factor = 1.f;
-  if (!kGateUp && wave < NT && my_m < M) {
-    if (!dense) factor = F::from_bits(static_cast<const uint16_t*>(a.topv)[a.perm[r0 + my_m]]);
-    else if (a.gate_s != nullptr) factor = F::from_bits(static_cast<const uint16_t*>(a.gate_s)[r0 + my_m]);
-  }
-
   vf32x4 acc[NM][NT];
 #pragma unroll
   for (int mi = 0; mi < NM; ++mi)
@@ -101,15 +49,23 @@ __global__ __launch_bounds__(kRwThreads) void f8_rows_kernel(const F8Product a, 
     int xs[NT];
     float ws[NM];
   };
-  auto load = [&](Stage& st, int i) __attribute__((always_inline)) {   // the wavefront's block number i (past the end: the last)
+  auto load_weights = [&](Stage& st, int i) __attribute__((always_inline)) {   // the wavefront's block number i (past the end: the last)
     const int kb = min(wave + i * kRwWaves, nb - 1);
 #pragma unroll
     for (int mi = 0; mi < NM; ++mi) {
       const uint8_t* p = wp[mi] + static_cast<size_t>(kb) * kF8TileBytes;
       st.w[mi][0] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(p));
       st.w[mi][1] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(p + 1024));
-      st.ws[mi] = sp[mi][kb];
     }
+  };
+  auto load_scales = [&](Stage& st, int i) __attribute__((always_inline)) {
+    const int kb = min(wave + i * kRwWaves, nb - 1);
+#pragma unroll
+    for (int mi = 0; mi < NM; ++mi) st.ws[mi] = sp[mi][kb];
+  };
+  const uint8_t *xp[NT], *xs[NT];
+  auto load_rows = [&](Stage& st, int i) __attribute__((always_inline)) {
+    const int kb = min(wave + i * kRwWaves, nb - 1);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const uint8_t* p = xp[nt] + kb * kF8Block;
@@ -117,6 +73,11 @@ __global__ __launch_bounds__(kRwThreads) void f8_rows_kernel(const F8Product a, 
       st.x[nt][1] = *reinterpret_cast<const i32x4*>(p + 16);
       st.xs[nt] = xs[nt][kb];
     }
+  };
+  auto load = [&](Stage& st, int i) __attribute__((always_inline)) {
+    load_weights(st, i);
+    load_rows(st, i);
+    load_scales(st, i);
   };
   auto use = [&](const Stage& st) __attribute__((always_inline)) {
     if constexpr (kGateUp) {
@@ -145,10 +106,29 @@ __global__ __launch_bounds__(kRwThreads) void f8_rows_kernel(const F8Product a, 
     }
   };
   const int n = (nb - wave + kRwWaves - 1) / kRwWaves;     // blocks of this wavefront
+  // The first weights go out before anything that waits for the permutation.
   Stage a0, a1;
-  load(a0, 0);
+  load_weights(a0, 0);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int m = min(nt * 16 + r, M - 1);       // rows past the end repeat the last and are not stored
+    size_t row = r0 + m;
+    if (!dense && a.gather) row = static_cast<uint32_t>(a.perm[r0 + m]) / static_cast<uint32_t>(a.topk);
+    xp[nt] = (dense ? a.act_s : a.act_r) + row * nb * kF8Block + q * 32;
+    xs[nt] = (dense ? a.act_ss : a.act_rs) + row * nb;
+  }
+  load_rows(a0, 0);
+  load_scales(a0, 0);
   __builtin_amdgcn_sched_barrier(0);
   load(a1, 1);
+  __builtin_amdgcn_sched_barrier(0);
+  const int my_m = wave * 16 + r;                // wavefront nt stores row group nt
+  float factor = 1.f;
+  if (!kGateUp && wave < NT && my_m < M) {
+    if (!dense) factor = F::from_bits(static_cast<const uint16_t*>(a.topv)[a.perm[r0 + my_m]]);
+    else if (a.gate_s != nullptr) factor = F::from_bits(static_cast<const uint16_t*>(a.gate_s)[r0 + my_m]);
+  }
   __builtin_amdgcn_sched_barrier(0);
   int c = 0;
   for (; c + 4 <= n; c += 2) {           // (no branch in here: the waits count what is in flight)

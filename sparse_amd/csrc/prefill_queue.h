@@ -49,7 +49,7 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
     r0 = a.seg_offsets[e];
     rows = a.seg_offsets[e + 1] - r0;
     mt = (rows + a.tile_rows - 1) / a.tile_rows;
-    slot = (a.segs.eids_dev != nullptr) ? a.expert_slot[e] : a.segs.slots[tid];
+    slot = (a.segs.eids_dev != nullptr) ? (a.expert_slot != nullptr ? a.expert_slot[e] : e) : a.segs.slots[tid];
   }
   // inclusive scan: within the wavefronts, then over their totals
   int scan = mt;

@@ -235,7 +235,7 @@ def pack_expert_into(dst: torch.Tensor, expert: Tuple[Quantized, Quantized, Quan
 
 
 class ExpertSlab:
-    """8-bit experts of one layer in HBM, one slot each, and the device-side expert -> slot table."""
+    """8-bit experts of one layer in HBM, one slot each."""
 
     def __init__(self, num_slots: int, num_experts: int, hidden: int, inter: int, device) -> None:
         if hidden % 64 or inter % 64 or hidden <= 0 or inter <= 0:
@@ -246,7 +246,8 @@ class ExpertSlab:
         self.data = torch.empty((self.num_slots, self.expert_bytes), dtype=torch.uint8, device=device)
         self._refs: dict = {}
         self.pow2 = False       # whether every scale of the slots in use is a power of two
-        self.expert_slot = torch.arange(self.num_experts, dtype=torch.int32, device=device)
+        # device segment lists read the slots here; None: expert e is in slot e (host lists name their slots)
+        self.expert_slot: Optional[torch.Tensor] = None
 
     @classmethod
     def from_quantized(cls, experts: Sequence[Tuple[Quantized, Quantized, Quantized]], device=None) -> "ExpertSlab":
@@ -270,7 +271,7 @@ class ExpertSlab:
         """The slab as the C entry takes it, for activations of ``dtype``; built once per dtype."""
         ref = self._refs.get(dtype)
         if ref is None:
-            ref = C.byref(_lib.Experts(self.data.data_ptr(), self.expert_bytes, self.expert_slot.data_ptr(),
+            ref = C.byref(_lib.Experts(self.data.data_ptr(), self.expert_bytes, _ptr(self.expert_slot),
                                        self.num_experts, self.hidden, self.inter, dtype_code(dtype)))
             self._refs[dtype] = ref
         return ref
