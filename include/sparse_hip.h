@@ -476,7 +476,7 @@ int sparse_hip_fp8_quantize(const void* x_dev, int dtype, int T, int K, void* va
  * quantised as above into the workspace (sparse_hip_fp8_linear_ws_bytes(T, cols) bytes, 16-byte aligned),
  * or x_dev is NULL and xq_dev / xs_dev hold the rows' values and scales (no workspace).  `pow2_scales`: the
  * caller says that every scale of the weight is a power of two between 2^-126 and 2^127, which calls of many
- * rows make use of; 0 is right for any scales.
+ * rows make use of; 0 is right for any scales.  Up to 2^28 rows and 2^16 columns.
  */
 size_t sparse_hip_fp8_linear_ws_bytes(int T, int K);
 int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_dev, int dtype, int T,
@@ -490,19 +490,21 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
  * and, unless shared_down_w is NULL, shared[t] likewise on the shared expert's matrices over all tokens,
  * times sigmoid(shared_gate[t]) when shared_gate_dev is not NULL.  Rows of segments that are not in `segs`
  * are left untouched; segs->n == 0: the shared expert alone.
+ * An expert is listed once, and a token's K experts differ.
  * `experts` describes the slab as for 16-bit weights, with dtype that of the activations (bf16 or fp16), and
- * expert_slot_dev may be NULL: expert e is in slot e.  A slot holds gate, up and down as matrices above and behind them their scales in the same order,
- * sparse_hip_fp8_slot_bytes(H, I) bytes in all.  H, I and Is are multiples of 64.  x [T,H], topv [T,K],
+ * expert_slot_dev may be NULL: expert e is in slot e.  A slot holds gate, up and down as matrices above and
+ * behind them their scales in the same order, sparse_hip_fp8_slot_bytes(H, I) bytes in all.  H, I and Is are multiples of 64.  x [T,H], topv [T,K],
  * parts [T*K,H], shared_gate [T], shared [T,H] in that dtype.  `pow2_scales` as above, for all matrices of
  * the call.  `ws_dev`:
- * sparse_hip_fp8_moe_ffn_ws_bytes(T, K, E, segs->n, H, I, Is) bytes (Is = 0 without a shared expert), 16-byte
- * aligned; calls that share one must be ordered on one stream.
+ * sparse_hip_fp8_moe_ffn_ws_bytes(T, K, E, segs->n, H, I, Is) bytes (Is = 0 without a shared expert; 0 for sizes
+ * that the call refuses), 16-byte aligned; calls that share one must be ordered on one stream.
  */
 size_t sparse_hip_fp8_slot_bytes(int H, int I);
 /*
  * Measurement aid: which kernels the 8-bit products of more than two rows take, for the whole process.  0 (the
  * default): by size; 1: those that stream weights past the rows; 2: tiles.  Both are right at any size; they
- * differ in the order of their sums.  A workspace's size depends on it.  Returns the setting before.
+ * differ in the order of their sums.  A workspace's size depends on it: not to be changed between asking for the
+ * size and the call.  Returns the setting before.
  */
 int sparse_hip_fp8_path(int which);
 size_t sparse_hip_fp8_moe_ffn_ws_bytes(int T, int K, int num_experts, int num_segments, int H, int I, int Is);

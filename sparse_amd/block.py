@@ -384,6 +384,8 @@ class DistributedSparseMoeBlock(nn.Module):
                     fp8.Weight.from_quantized(*fp8.module_weight(m, self.device))
                     for m in (shared_mod.gate_proj, shared_mod.up_proj, shared_mod.down_proj))
             else:
+                if any(w.dtype == fp8.E4M3 for w in _mlp_weights(shared_mod)):
+                    raise ValueError("8-bit shared-expert weights need weight_format='fp8'")
                 # tiled content, logical [rows, cols] shape kept for argument checks
                 self.shared_weights = tuple(
                     tile_weight(t.to(self.device, self.dtype)).reshape(t.shape).contiguous()

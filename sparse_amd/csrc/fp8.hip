@@ -10,6 +10,11 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 // Which kernels serve more than kF8FewRows rows: 0 by size, 1 the streaming ones, 2 the tiles.
 static std::atomic<int> g_path{0};
 
+constexpr int kF8MaxDim = 1 << 16;          // the tile kernel keeps a scale byte per row and block in LDS
+constexpr int kF8MaxOut = 1 << 28;          // columns of a product
+constexpr int64_t kF8MaxRows = 1ll << 28;   // flat rows: the division by topk is a 32-bit multiply
+constexpr int kF8StreamRows = 1 << 20;      // the streaming kernel's grid has a row of workgroups for every 32 rows
+
 // The streaming kernel reads the weights once for every 32 rows; the tile kernel reads them once or twice in all,
 // but starts slowly (7 us, then 0.45 us a 128-wide slab while few tiles are there to overlap) and reads weights
 // that are used once at 4.5 TB/s where the streaming kernel reaches 6.  Measured on both sides of the border,
@@ -22,7 +27,7 @@ static std::atomic<int> g_path{0};
 static bool linear_tiles(int T, int K, int N) {
   const int path = g_path.load(std::memory_order_relaxed);
   if (T <= kF8FewRows || path == 1) return false;
-  return path == 2 || static_cast<double>((T + 31) / 32) * N > 10000.0 + 6.0e6 / K;
+  return path == 2 || T > kF8StreamRows || static_cast<double>((T + 31) / 32) * N > 10000.0 + 6.0e6 / K;
 }
 // (The routed experts decide, all of them, so that a layer whose experts are executed in several calls, or apart
 // from the shared one, takes the same kernels in each.)
@@ -31,7 +36,7 @@ static bool ffn_tiles(int T, int K, int E, int H, int I) {
   if (T <= kF8FewRows || path == 1) return false;
   // work of the rows against a fixed cost and one for the weights
   const double h = H;
-  return path == 2 || T * (h * K * I + 2.0e6) > 2.4e8 + 4.4 * h * E * I;
+  return path == 2 || T > kF8StreamRows || T * (h * K * I + 2.0e6) > 2.4e8 + 4.4 * h * E * I;
 }
 
 // Rows per tile: the fewest of 32, 64, 128 with which the call's tiles still fit on the device together (two on a
@@ -49,9 +54,6 @@ static int ffn_tile_rows(int T, int K, int E, int H, int I) {
 }
 
 static inline size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
-
-constexpr int kF8MaxDim = 1 << 16;      // the tile kernel keeps a scale byte per row and block in LDS
-constexpr int64_t kF8MaxRows = 1ll << 28;   // flat rows: the division by topk is a 32-bit multiply
 
 // A workspace handed out front to back in 256-byte steps; with a null base it only counts.
 struct Carve {
@@ -147,8 +149,8 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
                           const sparse_hip_fp8_matrix* weight, int pow2_scales, void* out_dev, void* ws_dev, void* stream) {
   SP_REQUIRE(is_16bit(dtype), "fp8_linear: activations must be bf16 or fp16, got dtype %d", dtype);
   SP_REQUIRE(weight != nullptr, "fp8_linear: NULL weight");
-  SP_REQUIRE(weight->rows >= 1 && weight->rows <= kF8MaxDim && weight->cols >= 1 && weight->cols <= kF8MaxDim,
-             "fp8_linear: weight is [%d,%d], each side must be in [1,%d]", weight->rows, weight->cols, kF8MaxDim);
+  SP_REQUIRE(weight->rows >= 1 && weight->rows <= kF8MaxOut && weight->cols >= 1 && weight->cols <= kF8MaxDim,
+             "fp8_linear: weight is [%d,%d], must be in [1,%d] x [1,%d]", weight->rows, weight->cols, kF8MaxOut, kF8MaxDim);
   int rc = check_matrix("fp8_linear", "weight", weight, weight->rows, weight->cols);
   if (rc != SPARSE_HIP_OK) return rc;
   SP_REQUIRE(T >= 0, "fp8_linear: T=%d", T);
@@ -184,8 +186,8 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   p.dtype = dtype;
   p.pow2 = pow2_scales;
   if (T <= kF8FewRows) return f8_few(p, source, false, false, true, st);
-  return linear_tiles(T, weight->cols, weight->rows) ? f8_tile_linear(p, tile_rows(T, 0, (weight->rows + kPfBR - 1) / kPfBR), st)
-                                       : f8_rows(p, false, false, true, st);
+  if (!linear_tiles(T, weight->cols, weight->rows)) return f8_rows(p, false, false, true, st);
+  return f8_tile_linear(p, tile_rows(T, 0, (weight->rows + kPfBR - 1) / kPfBR), st);
 }
 
 size_t sparse_hip_fp8_slot_bytes(int H, int I) {
@@ -194,7 +196,9 @@ size_t sparse_hip_fp8_slot_bytes(int H, int I) {
 }
 
 size_t sparse_hip_fp8_moe_ffn_ws_bytes(int T, int K, int num_experts, int num_segments, int H, int I, int Is) {
-  if (T <= 0 || K <= 0 || num_experts <= 0 || num_segments < 0 || H <= 0 || I <= 0 || Is < 0) return 0;
+  if (T <= 0 || K <= 0 || K > SPARSE_HIP_MAX_TOPK || static_cast<int64_t>(T) * K >= kF8MaxRows) return 0;
+  if (num_experts <= 0 || num_experts > SPARSE_HIP_MAX_EXPERTS || num_segments < 0 || num_segments > SPARSE_HIP_MAX_EXPERTS) return 0;
+  if (H <= 0 || H > kF8MaxDim || I <= 0 || I > kF8MaxDim || Is < 0 || Is > kF8MaxDim) return 0;
   return ffn_ws(nullptr, T, K, num_experts, num_segments, H, I, Is).bytes;
 }
 
@@ -226,9 +230,13 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
     if (segs->eids_dev != nullptr) {
       SP_REQUIRE(segs->count_dev != nullptr, "%s: a device segment list needs a count", fn);
     } else {
-      for (int i = 0; i < segs->n; ++i)
+      bool seen[SPARSE_HIP_MAX_EXPERTS] = {};     // (the workspace has room for each segment's tiles once)
+      for (int i = 0; i < segs->n; ++i) {
         SP_REQUIRE(segs->eids[i] >= 0 && segs->eids[i] < E && segs->slots[i] >= 0, "%s: segment %d names expert %d in slot %d", fn, i,
                    static_cast<int>(segs->eids[i]), static_cast<int>(segs->slots[i]));
+        SP_REQUIRE(!seen[segs->eids[i]], "%s: expert %d is listed twice", fn, static_cast<int>(segs->eids[i]));
+        seen[segs->eids[i]] = true;
+      }
     }
   }
   int Is = 0;

@@ -39,7 +39,8 @@ def padded(n: int) -> int:
 
 # ------------------------------------------------------------------------------- rows
 class Rows:
-    """Quantised rows: ``data [T, padded(K)]`` (zeros behind column K) and ``scales [T, blocks(K)]``."""
+    """Quantised rows as ``quantize`` makes them: ``data [T, padded(K)]`` (zeros behind column K) and
+    ``scales [T, blocks(K)]``; ``dtype`` is that of the rows they were made of."""
 
     __slots__ = ("data", "scales", "cols", "dtype")
 
@@ -235,7 +236,8 @@ def pack_expert_into(dst: torch.Tensor, expert: Tuple[Quantized, Quantized, Quan
 
 
 class ExpertSlab:
-    """8-bit experts of one layer in HBM, one slot each."""
+    """8-bit experts of one layer in HBM, one slot each.  Host segment lists name the slots of their experts;
+    with a device list expert e is in slot e."""
 
     def __init__(self, num_slots: int, num_experts: int, hidden: int, inter: int, device) -> None:
         if hidden % 64 or inter % 64 or hidden <= 0 or inter <= 0:
@@ -246,8 +248,6 @@ class ExpertSlab:
         self.data = torch.empty((self.num_slots, self.expert_bytes), dtype=torch.uint8, device=device)
         self._refs: dict = {}
         self.pow2 = False       # whether every scale of the slots in use is a power of two
-        # device segment lists read the slots here; None: expert e is in slot e (host lists name their slots)
-        self.expert_slot: Optional[torch.Tensor] = None
 
     @classmethod
     def from_quantized(cls, experts: Sequence[Tuple[Quantized, Quantized, Quantized]], device=None) -> "ExpertSlab":
@@ -271,8 +271,8 @@ class ExpertSlab:
         """The slab as the C entry takes it, for activations of ``dtype``; built once per dtype."""
         ref = self._refs.get(dtype)
         if ref is None:
-            ref = C.byref(_lib.Experts(self.data.data_ptr(), self.expert_bytes, _ptr(self.expert_slot),
-                                       self.num_experts, self.hidden, self.inter, dtype_code(dtype)))
+            ref = C.byref(_lib.Experts(self.data.data_ptr(), self.expert_bytes, None, self.num_experts, self.hidden,
+                                       self.inter, dtype_code(dtype)))
             self._refs[dtype] = ref
         return ref
 
@@ -335,6 +335,11 @@ def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Perm
         raise ValueError(f"the permutation does not belong to {T} tokens x {K} over {E} experts")
     if segs is None:
         segs = ops.seglist_device(perm, min(E, T * K))
+    if segs.eids_dev:
+        if experts.num_slots < E:
+            raise ValueError(f"a device segment list needs a slot for each of the {E} experts, the slab has {experts.num_slots}")
+    elif any(not 0 <= s < experts.num_slots for s in segs.slots[:segs.n]):
+        raise ValueError(f"the segment list names slots outside the slab's {experts.num_slots}")
     if parts is None:
         parts = x.new_empty((T * K, H))
     else:

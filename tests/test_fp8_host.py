@@ -163,6 +163,8 @@ def test_moe_ffn_refusals():
         s.count_dev = None
         if n > 0:
             s.eids[0], s.slots[0] = eid, slot
+        if n == 2:
+            s.eids[1], s.slots[1] = 1 - eid, 1
         return s
 
     def call(E=4, h=H, i=I, dt=1, stride=stride, slab=P, sg=None, T=3, K=2, x=P, topv=P, parts=P, m=(None,) * 3, sh=None, ws=P):
@@ -221,3 +223,46 @@ def test_block_refusals():
         make(gate=dict(topk_method="greedy", e_score_correction_bias=torch.zeros(8)))
     with pytest.raises(NotImplementedError, match="scoring_func"):
         make(gate=dict(scoring_func="tanh"))
+
+
+def test_an_expert_is_listed_once():
+    lib = _lib.load()
+    P = 4096
+    s = _lib.SegList()
+    s.n = 3
+    for i, e in enumerate((2, 0, 2)):
+        s.eids[i], s.slots[i] = e, i
+    ex = _lib.Experts(P, fp8.slot_bytes(128, 64), None, 4, 128, 64, 1)
+    refused(lib.sparse_hip_fp8_moe_ffn(C.byref(ex), P, P, P, P, C.byref(s), 3, 2, P, None, None, None, None, 0, None, P, None),
+            "expert 2 is listed twice")
+
+
+def test_workspace_of_refused_sizes():
+    f = _lib.load().sparse_hip_fp8_moe_ffn_ws_bytes
+    good = dict(T=8, K=2, E=8, n=8, H=128, I=64, Is=64)
+    assert f(*good.values()) > 0
+    for name, v in dict(T=1 << 28, K=17, E=257, n=257, H=1 << 17, I=1 << 17, Is=1 << 17).items():
+        assert f(*{**good, name: v}.values()) == 0, name
+    assert f(*{**good, "T": 0}.values()) == 0
+
+
+def test_linear_of_a_vocabulary_is_taken():
+    """More than 2^16 output columns pass the checks (and no rows are nothing to do)."""
+    lib = _lib.load()
+    m = _lib.Fp8Matrix(4096, 4096, 200000, 64)
+    assert lib.sparse_hip_fp8_linear(4096, None, None, 1, 0, C.byref(m), 0, None, None, None) == 0
+    m = _lib.Fp8Matrix(4096, 4096, (1 << 28) + 1, 64)
+    refused(lib.sparse_hip_fp8_linear(4096, None, None, 1, 1, C.byref(m), 0, 4096, None, None), "must be in")
+
+
+def test_native_block_refuses_an_8_bit_shared_expert():
+    from sparse_amd.block import DistributedSparseMoeBlock
+    from sparse_amd.context import DistEnv, SparseContext
+    from sparse_amd.synthetic import make_mlp_block
+
+    SparseContext.reset()
+    mlp = make_mlp_block(dict(family="deepseek_shared", hidden=64, num_experts=8, inter=64, shared_inter=64), dtype=torch.bfloat16)
+    shared = getattr(mlp, "shared_expert", None) or mlp.shared_experts
+    shared.down_proj.weight = torch.nn.Parameter(shared.down_proj.weight.detach().to(torch.float8_e4m3fn), requires_grad=False)
+    with pytest.raises(ValueError, match="weight_format='fp8'"):
+        DistributedSparseMoeBlock(0, mlp, None, DistEnv(0, 1, 0, torch.device("cpu")), num_experts=8, top_k=2, dtype=torch.bfloat16)

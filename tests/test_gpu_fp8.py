@@ -376,3 +376,42 @@ def test_linear_long_rows(path, device, T):
     x = rand_rows(T, K, torch.bfloat16)
     want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s), grouped(T))
     within(fp8.linear(x.to(device), fp8.Weight.from_quantized(q.to(device), s.to(device))), want, bound, torch.bfloat16)
+
+
+@pytest.mark.parametrize("T", [1, 5, 150])
+def test_linear_of_many_columns(path, device, T):
+    """More than 2^16 columns, as an output projection has, and not a multiple of 16."""
+    K, N = 72, (1 << 16) + 43
+    q, s = rand_weight(N, K)
+    x = rand_rows(T, K, torch.bfloat16)
+    got = fp8.linear(x.to(device), fp8.Weight.from_quantized(q.to(device), s.to(device)))
+    for a, b in ((0, 128), ((1 << 16) - 128, N)):          # the first block, the last before the border and those behind
+        want, bound = ref_fp8.product(ref_fp8.rows(x), (q[a:b], s[a // 128:-(-b // 128)]), grouped(T))
+        within(got[:, a:b], want, bound, torch.bfloat16)
+
+
+def test_linear_of_many_rows(device):
+    """More rows than the streaming kernel's grid reaches, of a product small enough to be given to it."""
+    T, K, N = (1 << 21) + 5, 2, 3
+    q, s = rand_weight(N, K)
+    x = rand_rows(64, K, torch.bfloat16)
+    w = fp8.Weight.from_quantized(q.to(device), s.to(device))
+    big = x.to(device).repeat(-(-T // 64), 1)[:T].contiguous()
+    got = fp8.linear(big, w)
+    want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s), True)
+    for at in (0, 1 << 20, (T - 64) // 64 * 64):
+        within(got[at:at + 64], want, bound, torch.bfloat16)
+    assert torch.equal(got, got[:64].repeat(-(-T // 64), 1)[:T])
+
+
+def test_slots_outside_the_slab_are_refused(device):
+    c = make_case(4, 128, 4, 64, 2, 0, False, torch.bfloat16, seed=3)
+    d = on_gpu(c, device)
+    perm = ops.permute_build(c["topi"].to(device), 4)
+    few = fp8.ExpertSlab(2, 4, 128, 64, device)
+    topv = c["topv"].to(device)
+    with pytest.raises(ValueError, match="a slot for each"):
+        fp8.moe_ffn(few, d["x"], topv, perm)
+    for slot in (2, -1):
+        with pytest.raises(ValueError, match="slots outside"):
+            fp8.moe_ffn(few, d["x"], topv, perm, segs=ops.seglist_host([1, 3], [0, slot]))
