@@ -187,7 +187,7 @@ struct F8Where {
 };
 // At the start of a kernel every load waits a microsecond, and the compiler would place each behind the wait for
 // the one before.  Naming values to an empty statement has them loaded together: the kernel's arguments, then
-// the segment count with the expert, then slot with offsets.
+// the segment count with the expert, then slot with offsets (one token's experts: 19.0 -> 18.6 us).
 __device__ __forceinline__ bool f8_where(const F8Product& a, int block, int tiles_r, int tiles_s, F8Where& w) {
   int tile;
   w.dense = block < tiles_s;
@@ -246,8 +246,8 @@ int f8_few(const F8Product& p, int source, bool gateup, bool routed, bool dense,
 // The same of more rows, 8-bit ones.
 int f8_rows(const F8Product& p, bool gateup, bool routed, bool dense, hipStream_t st);
 
-// The same for many rows, 16-bit formats: 128 x 256 tiles.  gate/up writes quantised rows; routed and dense
-// tiles come from one set of queues.
+// The same of many rows: 128 x 256 tiles.  gate/up writes quantised rows; routed and dense tiles come from one set
+// of queues.
 struct PfQueues;
 int f8_tile_gateup(const F8Product& p, const PfQueues& q, void* h, void* hs, void* sh, void* shs, hipStream_t st);
 int f8_tile_down(const F8Product& p, const PfQueues& q, hipStream_t st);

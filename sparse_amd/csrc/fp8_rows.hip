@@ -1,12 +1,24 @@
-// Block-scaled 8-bit matrix products of a few dozen rows that are 8-bit already: weights and rows both go
-// straight from memory to registers.
+// Block-scaled 8-bit matrix products of three to a few dozen rows that are 8-bit already: weights and rows both
+// go straight from memory to registers.
 //
-// A workgroup owns 16 output columns of two matrices (gate and up of one expert), or 16 NM of one, and up to
-// 16 NT rows of a segment.  Its four wavefronts deal the 128-wide k blocks among themselves; two register
-// stages of KW blocks each are in flight per wavefront.  Rows are read from L2 by every workgroup of their
-// segment, in the matrix instruction's own layout: no LDS and no barrier before the wavefronts' sums meet.
-// With more than eight rows this beats quantising inside the kernel (fp8_few.hip), where every workgroup
-// repeats the work for all of its rows: gate/up of 32 tokens over 60 experts of 1408 x 2048, 91 us there.
+//   y[m, n] = sum over blocks b of 2^e(m, b) s(n, b) sum over k in b of x[m, k] w[n, k]
+//
+// What bounds it is the weights' way from HBM.  A workgroup owns 16 output columns of two matrices (gate and up
+// of one expert) or of one, and up to 16 NTmax rows of a segment.  Its four wavefronts deal the 128-wide k blocks
+// among themselves, one block a register stage, two stages in flight: that leaves registers for four to five
+// wavefronts on a SIMD, whose loads together keep HBM busy (two blocks a stage: down of 8 tokens 15.6 us instead
+// of 14.4; two column groups a workgroup: 23).  Rows are read from L2 by every workgroup of their segment, in the
+// matrix instruction's own layout: no LDS and no barrier before the wavefronts' sums meet.  Quantising the rows
+// in here instead of in a launch before (fp8_few.hip does) repeats that work in every workgroup: 24.4 + 14.4 us
+// become 30.4 + 33.1.
+//
+// Gate and up are products of the values widened to bf16, added in fp32, as their result is rounded to 8 bits next
+// and the 8-bit instruction's cut-off would move values across rounding borders; the matrix cycles are hidden
+// behind the loads.  Down and single products, rounded to 16 bits, take the 8-bit instruction with the rows'
+// scales as its operand.
+//
+// 8 tokens of 4 among 60 experts of 1408 x 2048 and a shared one of 5632: gate/up 170 MB in 24.8 us (6.9 TB/s),
+// down 85 MB in 14.5 us (5.9 TB/s).  333 rows of 1000 by 1418 weight rows, the border to the tile kernel: 9.3 us.
 #include <type_traits>
 
 #include "fp8.h"

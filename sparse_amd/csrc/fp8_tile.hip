@@ -1,17 +1,31 @@
 // Block-scaled 8-bit matrix products of many rows: the tile kernel.
 //
-// A workgroup of four wavefronts computes 128 rows x 256 weight rows (gate/up: 128 gate rows and the 128 up
+//   y[m, n] = sum over blocks b of 2^e(m, b) s(n, b) sum over k in b of x[m, k] w[n, k]
+//
+// A workgroup of four wavefronts computes up to 128 rows x 256 weight rows (gate/up: 128 gate rows and the 128 up
 // rows of the same neurons) over 128-wide k slabs.  An 8-bit slab row is 128 bytes, as a 64-wide slab row of
 // the 16-bit kernels is, so the movement of data is theirs: activation rows, gathered through the
-// permutation, go to a three-buffer LDS ring by direct global -> LDS copies with 16-byte chunks swizzled by
-// row; weight fragments come straight from the tiled layout into two alternating register sets; everything
-// is requested two slabs ahead and vector memory is awaited by count.  A slab is one 16x16x128 matrix
+// permutation, go to an LDS ring by direct global -> LDS copies with 16-byte chunks swizzled by row; weight
+// fragments come straight from the tiled layout into alternating register sets; everything is requested two
+// to four slabs ahead (tl_depth) and vector memory is awaited by count.  A slab is one 16x16x128 matrix
 // instruction per 16 x 16 tile where the 16-bit kernels have two of half the rate: the same bytes feed
 // twice the arithmetic.
 //
 // Scales: the activations' E8M0 bytes of the whole tile are laid out in LDS once, the eight bytes that a
 // lane's eight row tiles need for a slab side by side, and enter the instruction as its own operand.  The
-// weights' fp32 scales multiply the slab's sum on its way into the accumulator.
+// weights' fp32 scales multiply the slab's sum on its way into the accumulator, or, where all are powers of two,
+// enter the instruction as exponents (4096 rows of 2048 by 5632 weight rows: 65 -> 57 us).
+//
+// Gate/up ends in the quantiser: a tile's 128 neurons are one run of the intermediate, its largest magnitude is
+// found across the four wavefronts in LDS and 8-bit rows with their scales leave, a quarter of the bytes of fp32
+// ones and a launch less.
+//
+// What bounds it: two workgroups share a compute unit; in the steady loop their matrix instructions fill half of
+// the cycles (16 slabs of 128 rows: 27 us of both, 13.7 at the instruction's peak), and the 4.5 us before a
+// tile's first slab and 4 us behind its last are covered by the other workgroup only.  4096 rows of 2048 by 5632
+// weight rows: 51 us, 1.86 PFLOP/s (a library 8-bit product of that size: 51 us).  4096 tokens, 6 of 64 experts
+// of 1408 x 2048, shared 2816: gate/up 378 GFLOP in 194 to 221 us, down 189 GFLOP in 123 to 136.  Lower tiles for
+// a fuller last round lose: 96 rows 54 us, 64 rows 63.
 #include <type_traits>
 
 #include "fp8.h"
@@ -213,7 +227,6 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
       for (int g = 0; g < 4; ++g)
 #pragma unroll
         for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, min(st, nk - 1), h);
-    __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(kWait);
     __syncthreads();

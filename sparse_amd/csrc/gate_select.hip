@@ -9,9 +9,10 @@
 // The ranking runs in 32 bits all the same, on values known to 2^-19 + 2^-22 |r|, and every comparison that
 // decides something is checked: the gap between two neighbours of the ranking, the last chosen and the first
 // not chosen among them, and between any two groups, is larger than both errors, or the token starts over in
-// 64 bits (about one token in a hundred of 256 random logits; equal 16-bit logits without a bias always do).  32-bit maxima cross
-// the lanes in one instruction a step where 64-bit ones take a dozen: one token of 256 experts in 8 groups
-// 8.7 -> 5.4 us, 4096 tokens 17.1 -> 12.5 us.  What is left is latency: 4 MB of logits are read in a
+// 64 bits (about one token in a hundred of 256 random logits; equal 16-bit logits without a bias always do).
+// 32-bit maxima cross the lanes in one instruction a step where 64-bit ones take a dozen: one token of 256
+// experts in 8 groups 8.7 -> 5.4 us, 4096 tokens 17.1 -> 12.5 us.  What is left is the latency of the K + 1
+// maxima, one behind the other, of the groups and of the exponentials in 64 bits: 4 MB of logits are read in a
 // microsecond.
 #include "common.h"
 
@@ -70,8 +71,8 @@ __device__ __forceinline__ bool select_by(const SelectArgs& a, V (&r)[NV], V* s_
   constexpr bool kExact = sizeof(V) == 8;
   constexpr V kLow = -INFINITY;
   // twice what a 32-bit value may be off
-  const auto slack = [](V v) { return static_cast<V>(3.814697e-6f) + static_cast<V>(4.76837e-7f) * (v < 0 ? -v : v); };
   const auto size = [](V v) { return v < 0 ? -v : v; };
+  const auto slack = [&](V v) { return static_cast<V>(3.814697e-6f) + static_cast<V>(4.76837e-7f) * size(v); };
   bool clear = true;
   int id[NV];
 #pragma unroll
@@ -263,10 +264,13 @@ extern "C" int sparse_hip_gate_select(const void* logits_dev, int logits_dtype, 
   SP_REQUIRE(E >= 1 && E <= SPARSE_HIP_MAX_EXPERTS, "gate_select: E=%d outside [1,%d]", E, SPARSE_HIP_MAX_EXPERTS);
   SP_REQUIRE(K >= 1 && K <= SPARSE_HIP_MAX_TOPK && K <= E, "gate_select: K=%d outside [1,min(%d,E=%d)]", K, SPARSE_HIP_MAX_TOPK, E);
   SP_REQUIRE(score == SPARSE_HIP_SCORE_SOFTMAX || score == SPARSE_HIP_SCORE_SIGMOID, "gate_select: unknown score %d", score);
-  SP_REQUIRE(group_score == SPARSE_HIP_GROUP_MAX || group_score == SPARSE_HIP_GROUP_TOP2, "gate_select: unknown group score %d", group_score);
-  SP_REQUIRE(n_group >= 1 && n_group <= kSelMaxGroups && E % n_group == 0, "gate_select: n_group=%d must divide E=%d and be at most %d", n_group, E, kSelMaxGroups);
+  SP_REQUIRE(group_score == SPARSE_HIP_GROUP_MAX || group_score == SPARSE_HIP_GROUP_TOP2,
+             "gate_select: unknown group score %d", group_score);
+  SP_REQUIRE(n_group >= 1 && n_group <= kSelMaxGroups && E % n_group == 0,
+             "gate_select: n_group=%d must divide E=%d and be at most %d", n_group, E, kSelMaxGroups);
   SP_REQUIRE(topk_group >= 1 && topk_group <= n_group, "gate_select: topk_group=%d outside [1,%d]", topk_group, n_group);
-  SP_REQUIRE(K <= topk_group * (E / n_group), "gate_select: K=%d exceeds the %d experts of %d groups", K, topk_group * (E / n_group), topk_group);
+  SP_REQUIRE(K <= topk_group * (E / n_group), "gate_select: K=%d exceeds the %d experts of %d groups", K,
+             topk_group * (E / n_group), topk_group);
   SP_REQUIRE(T >= 0, "gate_select: T=%d", T);
   if (T == 0) return SPARSE_HIP_OK;
   SP_REQUIRE(logits_dev && topv_dev && topi_dev, "gate_select: NULL pointer");

@@ -34,10 +34,11 @@ __device__ __forceinline__ int pfx_share_of(int n, int i) {
 // of the routed ones (the shared expert's down tiles are the long ones, so they go first).
 __device__ __forceinline__ int pfx_queue_base(int R, int S, int x) { return 1 + pfx_start(S, x) + pfx_start(R, x); }
 
-// One workgroup of 256 threads, number b of nt_gu + nt_dn + 2, of the queue build.  Workgroups [0, nt_gu) and [nt_gu, nt_gu + nt_dn): one per routed column tile of the two launches --
-// segment s -> its row-tile count, scan, then thread s writes the entries of (segment s, this column
-// tile, row tile 0 ..), routed order (segment, column tile, row tile).  The two last workgroups write
-// the shared expert's entries (column tile, row tile) and the queue headers of their launch.
+// One workgroup of 256 threads, number b of nt_gu + nt_dn + 2, of the queue build.  Workgroups [0, nt_gu) and
+// [nt_gu, nt_gu + nt_dn): one per routed column tile of the two launches -- segment s -> its row-tile count, scan,
+// then thread s writes the entries of (segment s, this column tile, row tile 0 ..), routed order (segment, column
+// tile, row tile).  The two last workgroups write the shared expert's entries (column tile, row tile) and the queue
+// headers of their launch.
 __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const int b) {
   static_assert(SPARSE_HIP_MAX_EXPERTS <= 256, "one thread per segment");
   const int tid = threadIdx.x;
