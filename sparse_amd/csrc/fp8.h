@@ -178,26 +178,45 @@ struct F8Product {
   sparse_hip_seglist segs;
 };
 
+// Lists that an earlier launch wrote, read with scalar loads.
+typedef const __attribute__((address_space(4))) int32_t* f8_list;
+
 // Which 16 output columns of which matrix a workgroup of the streaming kernels owns, and for which rows.
 struct F8Where {
   const uint8_t *w0, *w1;      // the tile's panels
   const float *s0, *s1;        // and their scales
-  int nb, K, N, n0, r0, M;
+  const uint8_t *act, *acts;   // the rows' values and scales
+  const int32_t* perm;         // gathered rows: flat row -> token * topk + slot; else NULL
+  f8_list range;               // routed: the segment's first row and the one behind its last
+  int topk, T, nb, K, N, n0;
   bool dense;
+  __device__ __forceinline__ int first_row() const { return dense ? 0 : range[0]; }
+  __device__ __forceinline__ int rows() const { return dense ? T : range[1] - range[0]; }
 };
-// At the start of a kernel every load waits a microsecond, and the compiler would place each behind the wait for
-// the one before.  Naming values to an empty statement has them loaded together: the kernel's arguments, then
-// the segment count with the expert, then slot with offsets (one token's experts: 19.0 -> 18.6 us).
+// At the start of a kernel every load takes up to a microsecond, and the compiler places each behind the wait for the
+// one before.  Passing values through an empty statement has them loaded together and kept: the kernel's arguments,
+// then the segment count with the expert, then (where the slots are in a list) the slot.  The segment's rows
+// are asked for later: the weights' addresses do not need them.
 __device__ __forceinline__ bool f8_where(const F8Product& a, int block, int tiles_r, int tiles_s, F8Where& w) {
-  int tile;
+  const int32_t *slots = a.expert_slot, *eids = a.segs.eids_dev, *counts = a.segs.count_dev;
+  uint64_t stride = a.slot_stride, off0 = a.off0, off1 = a.off1, soff0 = a.soff0, soff1 = a.soff1;
+  int n = a.segs.n, gather = a.gather, Kr = a.Kr, Nr = a.Nr;
+  w.K = a.Ks;
+  w.N = a.Ns;
+  w.topk = a.topk;
+  w.T = a.T;
+  w.range = reinterpret_cast<f8_list>(reinterpret_cast<uintptr_t>(a.seg_offsets));
+  asm volatile("" : "+s"(tiles_r), "+s"(tiles_s), "+s"(stride), "+s"(off0), "+s"(off1), "+s"(soff0), "+s"(soff1), "+s"(w.range),
+               "+s"(slots), "+s"(eids), "+s"(counts), "+s"(n), "+s"(gather), "+s"(Kr), "+s"(Nr)
+               : "s"(a.slab), "s"(a.w0), "s"(a.w1), "s"(a.s0), "s"(a.s1), "s"(a.act_r), "s"(a.act_rs), "s"(a.act_s), "s"(a.act_ss),
+                 "s"(a.perm));
+  asm volatile("" : "+s"(w.K), "+s"(w.N), "+s"(w.topk), "+s"(w.T));
   w.dense = block < tiles_s;
+  int tile = block;
   if (w.dense) {
-    asm volatile("" ::"s"(a.w0), "s"(a.w1), "s"(a.s0), "s"(a.s1), "s"(a.Ks), "s"(a.Ns), "s"(a.T), "s"(a.act_s));
-    tile = block;
-    w.K = a.Ks;
-    w.N = a.Ns;
-    w.r0 = 0;
-    w.M = a.T;
+    w.act = a.act_s;
+    w.acts = a.act_ss;
+    w.perm = nullptr;
     w.w0 = a.w0;
     w.w1 = a.w1;
     w.s0 = a.s0;
@@ -205,28 +224,28 @@ __device__ __forceinline__ bool f8_where(const F8Product& a, int block, int tile
   } else {
     const int b = block - tiles_s, si = b / tiles_r;
     tile = b - si * tiles_r;
-    asm volatile("" ::"s"(a.segs.eids_dev), "s"(a.segs.count_dev), "s"(a.segs.n), "s"(a.expert_slot), "s"(a.seg_offsets),
-                 "s"(a.slab), "s"(a.slot_stride), "s"(a.off0), "s"(a.soff0), "s"(a.Kr), "s"(a.Nr), "s"(a.act_r), "s"(a.perm));
     int eid, slot_id;
-    if (a.segs.eids_dev != nullptr) {
-      const int count = a.segs.count_dev[0];
-      eid = a.segs.eids_dev[si];
-      asm volatile("" ::"s"(count), "s"(eid));
-      if (si >= min(count, a.segs.n)) return false;
-      slot_id = a.expert_slot != nullptr ? a.expert_slot[eid] : eid;
+    if (eids != nullptr) {
+      int count = reinterpret_cast<f8_list>(reinterpret_cast<uintptr_t>(counts))[0];
+      eid = reinterpret_cast<f8_list>(reinterpret_cast<uintptr_t>(eids))[si];
+      asm volatile("" : "+s"(count), "+s"(eid));
+      if (si >= min(count, n)) return false;
+      slot_id = slots != nullptr ? reinterpret_cast<f8_list>(reinterpret_cast<uintptr_t>(slots))[eid] : eid;
     } else {
-      eid = a.segs.eids[si];
-      slot_id = a.segs.slots[si];
+      eid = __builtin_amdgcn_readfirstlane(a.segs.eids[si]);
+      slot_id = __builtin_amdgcn_readfirstlane(a.segs.slots[si]);
     }
-    w.r0 = a.seg_offsets[eid];
-    w.M = a.seg_offsets[eid + 1] - w.r0;
-    w.K = a.Kr;
-    w.N = a.Nr;
-    const uint8_t* slot = a.slab + static_cast<uint64_t>(slot_id) * a.slot_stride;
-    w.w0 = slot + a.off0;
-    w.w1 = slot + a.off1;
-    w.s0 = reinterpret_cast<const float*>(slot + a.soff0);
-    w.s1 = reinterpret_cast<const float*>(slot + a.soff1);
+    w.range += eid;
+    w.K = Kr;
+    w.N = Nr;
+    w.act = a.act_r;
+    w.acts = a.act_rs;
+    w.perm = gather ? a.perm : nullptr;
+    const uint8_t* slot = a.slab + static_cast<uint64_t>(slot_id) * stride;
+    w.w0 = slot + off0;
+    w.w1 = slot + off1;
+    w.s0 = reinterpret_cast<const float*>(slot + soff0);
+    w.s1 = reinterpret_cast<const float*>(slot + soff1);
   }
   w.n0 = tile * 16;
   w.nb = (w.K + kF8Block - 1) / kF8Block;

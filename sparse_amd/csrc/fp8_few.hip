@@ -47,15 +47,16 @@ __device__ __forceinline__ u32x4 fw_round(const float (&v)[8], float& scale) {
   return __builtin_bit_cast(u32x4, f8_widen8(f8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
                                              f8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)));
 }
-template <typename F, int kSrc>
+// kVec: rows of the 16-bit type start on 16-byte boundaries and hold a multiple of 8 values
+template <typename F, int kSrc, bool kVec>
 struct Source;
-template <typename F>
-struct Source<F, kSrc16> {
+template <typename F, bool kVec>
+struct Source<F, kSrc16, kVec> {
   u32x4 v;
-  __device__ __forceinline__ void load(const uint8_t* base, const uint8_t*, size_t row, int K, int, int kb, int at, bool vec) {
+  __device__ __forceinline__ void load(const uint8_t* base, const uint8_t*, size_t row, int K, int, int kb, int at) {
     const int k = kb * kF8Block + at;
     const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + row * K + k;
-    if (vec) {
+    if (kVec) {
       v = k < K ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
     } else {
       uint32_t e[8];
@@ -72,10 +73,10 @@ struct Source<F, kSrc16> {
     return fw_round(f, scale);
   }
 };
-template <typename F>
-struct Source<F, kSrc32> {
+template <typename F, bool kVec>
+struct Source<F, kSrc32, kVec> {
   vf32x4 a, b;
-  __device__ __forceinline__ void load(const uint8_t* base, const uint8_t*, size_t row, int K, int, int kb, int at, bool) {
+  __device__ __forceinline__ void load(const uint8_t* base, const uint8_t*, size_t row, int K, int, int kb, int at) {
     const int k = kb * kF8Block + at;    // K a multiple of 64
     const float* p = reinterpret_cast<const float*>(base) + row * K + k;
     a = b = vf32x4{0.f, 0.f, 0.f, 0.f};
@@ -89,11 +90,11 @@ struct Source<F, kSrc32> {
     return fw_round(f, scale);
   }
 };
-template <typename F>
-struct Source<F, kSrc8> {
+template <typename F, bool kVec>
+struct Source<F, kSrc8, kVec> {
   uint2 v;
   uint8_t e;
-  __device__ __forceinline__ void load(const uint8_t* base, const uint8_t* scales, size_t row, int, int nb, int kb, int at, bool) {
+  __device__ __forceinline__ void load(const uint8_t* base, const uint8_t* scales, size_t row, int, int nb, int kb, int at) {
     v = *reinterpret_cast<const uint2*>(base + (row * nb + kb) * kF8Block + at);
     e = scales[row * nb + kb];
   }
@@ -103,9 +104,10 @@ struct Source<F, kSrc8> {
   }
 };
 
-// kGateUp: NM = 2 matrices, gate and up, fp32 SwiGLU out.  Otherwise one.
-template <typename F, bool kGateUp, int NM, int kSrc>
-__global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, int tiles_r, int tiles_s, int vec) {
+// kGateUp: two matrices, gate and up, fp32 SwiGLU out.  Otherwise one.
+template <typename F, bool kGateUp, int kSrc, bool kVec>
+__global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, int tiles_r, int tiles_s) {
+  constexpr int NM = kGateUp ? 2 : 1;
   constexpr int kStage = 2 * kF8FewRows * kFwStride, kSums = kFwWaves * NM * 64 * static_cast<int>(sizeof(vf32x4));
   __shared__ __attribute__((aligned(16))) uint8_t lds[kStage > kSums ? kStage : kSums];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
   F8Where own;
   if (!f8_where(a, blockIdx.x, tiles_r, tiles_s, own)) return;
   const bool dense = own.dense;
-  const int nb = own.nb, K = own.K, N = own.N, n0 = own.n0, r0 = own.r0;
+  const int nb = own.nb, K = own.K, N = own.N, n0 = own.n0;
   const uint8_t* wp[NM];
   const float* sp[NM];
 #pragma unroll
@@ -121,8 +123,6 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
     wp[mi] = (mi ? own.w1 : own.w0) + lane * 16;
     sp[mi] = mi ? own.s1 : own.s0;
   }
-  const int M = min(own.M, kF8FewRows);      // (the ids of a token are distinct: a segment has T rows at most)
-  if (M <= 0) return;
 
   vf32x4 acc[NM];
 #pragma unroll
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
   struct Stage {
     i32x4 w[KW][NM][2];
     float ws[KW][NM];
-    Source<F, kSrc> src;
+    Source<F, kSrc, kVec> src;
   };
   auto load_weights = [&](Stage& st, int chunk) __attribute__((always_inline)) {
 #pragma unroll
@@ -157,12 +157,17 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
 #pragma unroll
       for (int mi = 0; mi < NM; ++mi) st.ws[i][mi] = sp[mi][min(chunk * KC + wave + i * kFwWaves, nb - 1)];
   };
-  auto load_rows = [&](Stage& st, int chunk) __attribute__((always_inline)) {   // (a second row that is not there repeats the first)
-    const int m = min(my_m, M - 1), kb = min(chunk * KC + my_kb, nb - 1);
-    size_t row = r0 + m;
-    if (!dense && a.gather)                      // (one token: every row is its)
-      row = a.T == 1 ? 0 : static_cast<uint32_t>(a.perm[r0 + m]) / static_cast<uint32_t>(a.topk);
-    st.src.load(dense ? a.act_s : a.act_r, dense ? a.act_ss : a.act_rs, row, K, nb, kb, gl * 8, vec != 0);
+  // ---- the first weights go out before anything that waits for the segment's rows ------------
+  Stage s0_, s1_;
+  load_weights(s0_, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  const int r0 = own.first_row(), M = min(own.rows(), kF8FewRows);   // (the ids of a token are distinct: a segment has T rows at most)
+  if (M <= 0) return;
+  // (a second row that is not there repeats the first; of one token every row is its)
+  size_t my_row = r0 + min(my_m, M - 1);
+  if (own.perm != nullptr) my_row = own.T == 1 ? 0 : static_cast<uint32_t>(own.perm[my_row]) / static_cast<uint32_t>(own.topk);
+  auto load_rows = [&](Stage& st, int chunk) __attribute__((always_inline)) {
+    st.src.load(own.act, own.acts, my_row, K, nb, min(chunk * KC + my_kb, nb - 1), gl * 8);
   };
   auto use = [&](const Stage& st, int chunk, uint8_t* buf) __attribute__((always_inline)) {
     const int c0 = chunk * KC;
@@ -195,9 +200,6 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
   };
   const int chunks = (nb + KC - 1) / KC;
   uint8_t *const buf0 = lds, *const buf1 = lds + kF8FewRows * kFwStride;
-  Stage s0_, s1_;
-  load_weights(s0_, 0);
-  __builtin_amdgcn_sched_barrier(0);
   load_rows(s0_, 0);
   load_rows(s1_, 1);
   __builtin_amdgcn_sched_barrier(0);
@@ -264,28 +266,28 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
   }
 }
 
-template <typename F, bool kGateUp, int NM, int kSrc>
-static int launch_few(const F8Product& p, int tiles_r, int tiles_s, int vec, hipStream_t st) {
+template <typename F, bool kGateUp, int kSrc, bool kVec>
+static int launch_few(const F8Product& p, int tiles_r, int tiles_s, hipStream_t st) {
   const int64_t grid = tiles_s + static_cast<int64_t>(tiles_r) * p.segs.n;
   if (grid == 0) return SPARSE_HIP_OK;
   SP_REQUIRE(grid < (1ll << 31), "fp8 product: grid too large");
   SP_REQUIRE(p.T <= kF8FewRows, "fp8 product: %d rows", p.T);
-  hipLaunchKernelGGL((f8_few_kernel<F, kGateUp, NM, kSrc>), dim3(static_cast<unsigned>(grid)),
-                     dim3(kFwThreads), 0, st, p, tiles_r, tiles_s, vec);
+  hipLaunchKernelGGL((f8_few_kernel<F, kGateUp, kSrc, kVec>), dim3(static_cast<unsigned>(grid)), dim3(kFwThreads), 0, st, p,
+                     tiles_r, tiles_s);
   SP_LAUNCH_CHECK("f8_few_kernel");
   return SPARSE_HIP_OK;
 }
 
 template <typename F>
 static int few_as(const F8Product& p, int source, bool gateup, bool routed, bool dense, hipStream_t st) {
-  const int groups_r = routed ? (p.Nr + 15) / 16 : 0, groups_s = dense ? (p.Ns + 15) / 16 : 0;
+  const int tr = routed ? (p.Nr + 15) / 16 : 0, ts = dense ? (p.Ns + 15) / 16 : 0;
+  if (source == kF8From32) return launch_few<F, false, kSrc32, true>(p, tr, ts, st);
+  if (source == kF8From8) return launch_few<F, false, kSrc8, true>(p, tr, ts, st);
   // 16-byte loads of the rows need aligned rows of a multiple of eight values
   const int K = dense ? p.Ks : p.Kr;
-  const int vec = K % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.act_s) | reinterpret_cast<uintptr_t>(p.act_r)) & 15) == 0;
-  if (gateup) return launch_few<F, true, 2, kSrc16>(p, groups_r, groups_s, vec, st);
-  if (source == kF8From16) return launch_few<F, false, 1, kSrc16>(p, groups_r, groups_s, vec, st);
-  if (source == kF8From32) return launch_few<F, false, 1, kSrc32>(p, groups_r, groups_s, vec, st);
-  return launch_few<F, false, 1, kSrc8>(p, groups_r, groups_s, vec, st);
+  const bool vec = K % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.act_s) | reinterpret_cast<uintptr_t>(p.act_r)) & 15) == 0;
+  if (gateup) return vec ? launch_few<F, true, kSrc16, true>(p, tr, ts, st) : launch_few<F, true, kSrc16, false>(p, tr, ts, st);
+  return vec ? launch_few<F, false, kSrc16, true>(p, tr, ts, st) : launch_few<F, false, kSrc16, false>(p, tr, ts, st);
 }
 
 int f8_few(const F8Product& p, int source, bool gateup, bool routed, bool dense, hipStream_t st) {

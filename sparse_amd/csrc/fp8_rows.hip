@@ -46,8 +46,8 @@ __global__ __launch_bounds__(kRwThreads) void f8_rows_kernel(const F8Product a, 
     wp[mi] = (mi ? own.w1 : own.w0) + lane * 16;
     sp[mi] = mi ? own.s1 : own.s0;
   }
-  const int m0 = blockIdx.y * 16 * NTmax, M = min(own.M - m0, 16 * NTmax), r0 = own.r0 + m0;
-  if (M <= 0) return;
+  const int m0 = blockIdx.y * 16 * NTmax, M = min(own.rows() - m0, 16 * NTmax), r0 = own.first_row() + m0;
+  if ((NTmax > 1 || blockIdx.y > 0) && M <= 0) return;
   auto body = [&](auto nt_c) __attribute__((always_inline)) {
   constexpr int NT = decltype(nt_c)::value;
   vf32x4 acc[NM][NT];
@@ -118,17 +118,17 @@ __global__ __launch_bounds__(kRwThreads) void f8_rows_kernel(const F8Product a, 
     }
   };
   const int n = (nb - wave + kRwWaves - 1) / kRwWaves;     // blocks of this wavefront
-  // The first weights go out before anything that waits for the permutation.
+  // The first weights go out before anything that waits for the segment's rows.
   Stage a0, a1;
   load_weights(a0, 0);
   __builtin_amdgcn_sched_barrier(0);
+  if (M <= 0) return;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int m = min(nt * 16 + r, M - 1);       // rows past the end repeat the last and are not stored
-    size_t row = r0 + m;
-    if (!dense && a.gather) row = static_cast<uint32_t>(a.perm[r0 + m]) / static_cast<uint32_t>(a.topk);
-    xp[nt] = (dense ? a.act_s : a.act_r) + row * nb * kF8Block + q * 32;
-    xs[nt] = (dense ? a.act_ss : a.act_rs) + row * nb;
+    size_t row = r0 + min(nt * 16 + r, M - 1);   // rows past the end repeat the last and are not stored
+    if (own.perm != nullptr) row = static_cast<uint32_t>(own.perm[row]) / static_cast<uint32_t>(own.topk);
+    xp[nt] = own.act + row * nb * kF8Block + q * 32;
+    xs[nt] = own.acts + row * nb;
   }
   load_rows(a0, 0);
   load_scales(a0, 0);
