@@ -269,7 +269,9 @@ int f8_rows(const F8Product& p, bool gateup, bool routed, bool dense, hipStream_
 // of queues.
 struct PfQueues;
 int f8_tile_gateup(const F8Product& p, const PfQueues& q, void* h, void* hs, void* sh, void* shs, hipStream_t st);
-int f8_tile_down(const F8Product& p, const PfQueues& q, hipStream_t st);
+// (tiles of 32 rows are 128 columns wide in down and linear)
+int f8_tile_columns(int tile_rows);
+int f8_tile_down(const F8Product& p, const PfQueues& q, int tile_rows, hipStream_t st);
 int f8_tile_linear(const F8Product& p, int tile_rows, hipStream_t st);
 
 }  // namespace sparse

@@ -16,18 +16,19 @@ constexpr int64_t kF8MaxRows = 1ll << 28;   // flat rows: the division by topk i
 constexpr int kF8StreamRows = 1 << 20;      // the streaming kernel's grid has a row of workgroups for every 32 rows
 
 // The streaming kernel reads the weights once for every 32 rows; the tile kernel reads them once or twice in all,
-// but starts slowly (7 us, then 0.45 us a 128-wide slab while few tiles are there to overlap) and reads weights
-// that are used once at 4.5 TB/s where the streaming kernel reaches 6.  Measured on both sides of the border,
-// streaming / tiles:
-//   linear  2048 x 5632: 64 rows 13.3 / 14.3 us, 128 rows 21 / 14.8;  4096 x 4096: 64 rows 17 / 21, 128 rows 29 / 22
-//           1000 x 1418: 333 rows 11.8 / 12.5, 512 rows 15.1 / 12.7;  512 x 1024: 333 rows 8.3 / 8.8, 512 rows 9.6 / 9.0
-//   experts 60 of 1408 x 2048, 4 a token, shared 5632: 64 tokens 109 / 115 us, 96 tokens 131 / 121
-//           16 of 704 x 1024, 3 a token: 64 tokens 20.7 / 22.1, 128 tokens 25.8 / 22.9
-//           8 of 704 x 2048, 2 a token, shared 1408: 48 tokens 23.8 / 24.7, 96 tokens 32 / 25.4
-static bool linear_tiles(int T, int K, int N) {
+// but starts slowly (5 us, then 0.25 us a 128-wide slab while few tiles are there to overlap).  Measured on both
+// sides of the border, streaming / tiles:
+//   linear  2048 x 5632: 32 rows 10.4 / 11.2 us, 64 rows 13.3 / 11.5;  4096 x 4096: 48 rows 14.8 / 15.4, 64 rows 17.1 / 15.4
+//           1000 x 1418: 192 rows 9.2 / 9.7, 333 rows 11.9 / 10.2;  512 x 1024: 192 rows 7.3 / 7.6, 333 rows 8.6 / 7.7
+//           5632 x 2048: 64 rows 12.3 / 18.4, 192 rows 26.7 / 19.7;  256 x 256: 512 rows 6.3 / 7.0, 1024 rows 7.5 / 7.1
+//   experts 60 of 1408 x 2048, 4 a token, shared 5632: 32 tokens 81.8 / 96.2 us, 64 tokens 113 / 102
+//           16 of 704 x 1024, 3 a token: 48 tokens 19.5 / 20.5, 96 tokens 23.5 / 21.4
+//           8 of 704 x 2048, 2 a token, shared 1408: 48 tokens 22.8 / 23.3, 64 tokens 25.8 / 23.4
+//           64 of 256 x 512, 6 a token: 16 tokens 15.2 / 17.5, 48 tokens 20.4 / 18.0
+static bool linear_tiles(int T, int N) {
   const int path = g_path.load(std::memory_order_relaxed);
   if (T <= kF8FewRows || path == 1) return false;
-  return path == 2 || T > kF8StreamRows || static_cast<double>((T + 31) / 32) * N > 10000.0 + 6.0e6 / K;
+  return path == 2 || T > kF8StreamRows || static_cast<int64_t>(T) * N > 256000;
 }
 // (The routed experts decide, all of them, so that a layer whose experts are executed in several calls, or apart
 // from the shared one, takes the same kernels in each.)
@@ -35,13 +36,14 @@ static bool ffn_tiles(int T, int K, int E, int H, int I) {
   const int path = g_path.load(std::memory_order_relaxed);
   if (T <= kF8FewRows || path == 1) return false;
   // work of the rows against a fixed cost and one for the weights
-  const double h = H;
-  return path == 2 || T > kF8StreamRows || T * (h * K * I + 2.0e6) > 2.4e8 + 4.4 * h * E * I;
+  const double size = static_cast<double>(H) * I;
+  return path == 2 || T > kF8StreamRows || static_cast<double>(T) * K * (size + 1.0e6) > 2.2e8 + 3.6 * size * E;
 }
 
-// Rows per tile: the fewest of 32, 64, 128 with which the call's tiles still fit on the device together (two on a
-// compute unit).  A launch of fewer tiles than that is as long as its longest tile, and one of 32 rows takes half
-// the time of one of 128; more tiles than that cost what the weights' second reading costs.
+// Rows per tile: the fewest of 32, 64, 128 with which the call's tiles (of 256 columns) still fit on the device
+// together, two on a compute unit.  A launch of fewer tiles than that is as long as its longest tile, and one of 32
+// rows takes half the time of one of 128; more tiles than that cost what the weights' second reading costs.  Tiles
+// of 32 rows are then cut to 128 columns (f8_tile_columns).
 static int tile_rows(int64_t rows, int segments, int column_tiles) {
   for (int r = 32; r < kPfBM; r *= 2)
     if ((rows / r + segments) * column_tiles <= 512) return r;
@@ -104,7 +106,8 @@ static FfnWs ffn_ws(void* ws, int T, int K, int E, int nseg, int H, int I, int I
     if (Is > 0) w.sh = take_rows(c, T, Is);
   }
   if (ffn_tiles(T, K, E, H, I)) {
-    w.tiles = c.take(prefill_queue_ws_bytes(T, K, nseg, H, I, Is, ffn_tile_rows(T, K, E, H, I)));
+    const int rows_per_tile = ffn_tile_rows(T, K, E, H, I);
+    w.tiles = c.take(prefill_queue_ws_bytes(T, K, nseg, H, I, Is, rows_per_tile, f8_tile_columns(rows_per_tile)));
   } else {
     w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
     if (Is > 0) w.shf = static_cast<float*>(c.take(static_cast<size_t>(T) * Is * sizeof(float)));
@@ -186,7 +189,7 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
   p.dtype = dtype;
   p.pow2 = pow2_scales;
   if (T <= kF8FewRows) return f8_few(p, source, false, false, true, st);
-  if (!linear_tiles(T, weight->cols, weight->rows)) return f8_rows(p, false, false, true, st);
+  if (!linear_tiles(T, weight->rows)) return f8_rows(p, false, false, true, st);
   return f8_tile_linear(p, tile_rows(T, 0, (weight->rows + kPfBR - 1) / kPfBR), st);
 }
 
@@ -258,12 +261,13 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   // One or two tokens: rows are quantised inside the products.  More: in launches of their own, beside products
   // that stream weights; beside the tile kernel x only, which quantises the intermediate in its epilogue.
   const bool few = T <= kF8FewRows, tiles = ffn_tiles(T, K, E, H, I);
+  const int rows_per_tile = tiles ? ffn_tile_rows(T, K, E, H, I) : 0;
   int rc = SPARSE_HIP_OK;
   PfQueues queues = {};
   if (tiles) {
     PfxMapArgs queue_args;
     queues = prefill_queue_args(experts->expert_slot_dev, seg_offsets_dev, *segs, T, K, H, I, Is, w.tiles, &queue_args,
-                                ffn_tile_rows(T, K, E, H, I));
+                                rows_per_tile, f8_tile_columns(rows_per_tile));
     rc = f8_quantize_and_queue({x_dev, T, H, w.x.values, w.x.scales}, dtype, queue_args, st);
   } else if (!few) {
     rc = f8_quantize({x_dev, T, H, w.x.values, w.x.scales}, {}, dtype, st);
@@ -331,7 +335,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
     p.Ks = Is;
     p.Ns = H;
   }
-  if (tiles) return f8_tile_down(p, queues, st);
+  if (tiles) return f8_tile_down(p, queues, rows_per_tile, st);
   return few ? f8_few(p, kF8From32, false, routed, shared, st) : f8_rows(p, false, routed, shared, st);
 }
 

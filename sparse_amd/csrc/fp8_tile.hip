@@ -40,13 +40,19 @@ constexpr int kTlRing = kPfStages * kTlSlab;
 // A tile of 32 NMI rows keeps S slabs of weight fragments in registers and S + 1 slabs of rows in LDS.  What a
 // low tile saves in accumulators and rows goes into depth: its slab is half the work or less, and four slabs
 // ahead its weights are as far away in time.
-constexpr int tl_depth(int nmi) { return nmi == 1 ? 4 : nmi == 2 ? 3 : 2; }
-// "The copies of the next slab have landed": its copies were followed by their own slab's 8 fragment loads and by
-// S - 1 slabs of NMI copies and 8 loads each.
-constexpr int tl_younger(int nmi) { return 8 + (tl_depth(nmi) - 1) * (nmi + 8); }
+constexpr int tl_depth(int nmi, bool narrow) { return narrow ? 6 : nmi == 1 ? 4 : nmi == 2 ? 3 : 2; }
+// "The copies of the next slab have landed": its copies were followed by their own slab's 2 NG fragment loads and by
+// S - 1 slabs of NMI copies and 2 NG loads each.
+constexpr int tl_younger(int nmi, bool narrow) {
+  const int loads = narrow ? 4 : 8;
+  return loads + (tl_depth(nmi, narrow) - 1) * (nmi + loads);
+}
 constexpr int tl_wait(int vmcnt) { return 0x0F70 | (vmcnt & 15) | ((vmcnt >> 4) << 14); }
-static_assert(tl_younger(4) == 20 && tl_wait(20) == kWaitVmcnt20 && tl_younger(2) < 64 && tl_younger(1) < 64, "six bits");
-static_assert((tl_depth(1) + 1) * 32 * kTlRowBytes <= kTlRing && (tl_depth(2) + 1) * 64 * kTlRowBytes <= kTlRing, "rings fit");
+static_assert(tl_younger(4, false) == 20 && tl_wait(20) == kWaitVmcnt20, "the count of the 16-bit kernels");
+static_assert(tl_younger(2, false) < 64 && tl_younger(1, false) < 64 && tl_younger(1, true) < 64, "six bits");
+static_assert((tl_depth(1, false) + 1) * 32 * kTlRowBytes <= kTlRing && (tl_depth(2, false) + 1) * 64 * kTlRowBytes <= kTlRing, "rings fit");
+constexpr int kTlNarrowRows = 32;
+constexpr int kTlNarrowRing = (tl_depth(1, true) + 1) * kTlNarrowRows * kTlRowBytes;
 constexpr int kTlScaleBytes = kPfBM + 2 * sizeof(float);   // per slab: activation bytes, two weight scales
 static_assert(kTlSlab == kPfLdsA, "the slab geometry is that of the 16-bit kernels");
 
@@ -70,9 +76,13 @@ struct TileArgs {
 
 // F: the 16-bit format of outputs, route weights and gate logits
 // kPow2: every weight scale is a power of two, and enters the instruction as its exponent
-template <typename F, bool kGateUp, bool kPow2>
-__global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kTlRing];
+// kNarrow: tiles of 32 rows by 128, three workgroups to a compute unit instead of two (not for gate/up)
+template <typename F, bool kGateUp, bool kPow2, bool kNarrow>
+__global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(const TileArgs a) {
+  constexpr int NG = kNarrow ? 2 : 4;                         // 16-row groups of weights per wavefront
+  constexpr int kRows = kNarrow ? kTlNarrowRows : kPfBM;
+  static_assert(!(kNarrow && kGateUp), "gate/up tiles are wide: their 128 neurons are one run of the quantiser");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kNarrow ? kTlNarrowRing : kTlRing];
   __shared__ float s_row[kPfBM];          // factor of a row (down), exponent of a row's scale (gate/up)
   __shared__ float s_amax[kGateUp ? 4 : 1][kPfBM];
   extern __shared__ __attribute__((aligned(16))) uint8_t s_scales[];   // [nk][128] bytes, then [nk][2] floats
@@ -109,7 +119,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
   const int Kdim = dense ? a.p.Ks : a.p.Kr, N = dense ? a.p.Ns : a.p.Nr;
   const int nk = (Kdim + kF8Block - 1) / kF8Block;
   const uint32_t ld = static_cast<uint32_t>(nk) * kF8Block;
-  const int n0 = bn * (kGateUp ? kPfBR / 2 : kPfBR);   // first output column of this tile
+  const int n0 = bn * (kGateUp ? kPfBR / 2 : 64 * NG);   // first output column of this tile
 
   // ---- operand addresses ------------------------------------------------------------
   // Row r keeps chunk 2q + h at position (q + 4h) ^ f(r), f(r) = ((r >> 1) & 7) ^ ((r & 1) << 2); of eight rows
@@ -130,7 +140,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
   };
   // The wavefront's 64 weight rows are four 16-row groups (gate/up: groups 0, 1 gate rows of 32 neurons,
   // groups 2, 3 the up rows of the same neurons); a group's slab is 2 KB, its two halves 1 KB each in lane order.
-  const uint8_t* wbase[4];
+  const uint8_t* wbase[NG];
   const float *ws0, *ws1;      // the scales of the tile's two 128-row blocks (gate/up: of gate and of up)
   const uint32_t woff = lane * 16;
   {
@@ -150,9 +160,9 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
     }
     const int last16 = ((N + 15) & ~15) - 16;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
+    for (int g = 0; g < NG; ++g) {
       const uint8_t* base = (kGateUp && g >= 2) ? w1 : w0;
-      const int n = min(kGateUp ? (n0 + wave * 32 + (g & 1) * 16) : (n0 + wave * 64 + g * 16), last16);
+      const int n = min(kGateUp ? (n0 + wave * 32 + (g & 1) * 16) : (n0 + wave * 16 * NG + g * 16), last16);
       wbase[g] = uniform_ptr(base + static_cast<size_t>(n >> 4) * nk * kF8TileBytes);
     }
     const int nblk = (N + kF8Block - 1) / kF8Block, b0 = n0 / kF8Block;
@@ -168,17 +178,18 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
   // ---- scales to LDS, row factors ------------------------------------------------------
   // Bytes are fetched eight at a time before the first is stored: one by one, each would wait a memory latency.
   auto fill_scales = [&]() __attribute__((always_inline)) {
-    const int m = tid >> 1, half = tid & 1;
+    constexpr int kShare = kPfThreads / kRows;    // threads of a row
+    const int m = tid / kShare, part = tid % kShare;
     const uint8_t* src = sbase + static_cast<size_t>(source_row(m)) * nk;
     uint8_t* dst = s_scales + (m & 15) * 8 + (m >> 4);
     float* w = reinterpret_cast<float*>(s_scales + nk * kPfBM);
-    for (int kb0 = 0; kb0 < nk; kb0 += 16) {
+    for (int kb0 = part; kb0 < nk; kb0 += 8 * kShare) {
       uint8_t v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = src[min(kb0 + 2 * i + half, nk - 1)];
+      for (int i = 0; i < 8; ++i) v[i] = src[min(kb0 + kShare * i, nk - 1)];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (kb0 + 2 * i + half < nk) dst[(kb0 + 2 * i + half) * kPfBM] = v[i];
+        if (kb0 + kShare * i < nk) dst[(kb0 + kShare * i) * kPfBM] = v[i];
     }
     for (int i = tid; i < 2 * nk; i += kPfThreads) w[i] = ((i & 1) ? ws1 : ws0)[i >> 1];
     // down: factor of each row, the route weight or the sigmoid of the shared expert's gate
@@ -201,7 +212,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
     // While slab kt is multiplied, the rows of slab kt+S travel to the LDS buffer slab kt-1 has left and the
     // fragments of slab kt+S to the registers the last row pair has just finished with.  Vector memory retires
     // in order, so what has landed is known by counting.  Slabs past the end refetch the last one.
-    constexpr int S = tl_depth(NMI), kSlab = 32 * NMI * kTlRowBytes, kWait = tl_wait(tl_younger(NMI));
+    constexpr int S = tl_depth(NMI, kNarrow), kSlab = 32 * NMI * kTlRowBytes, kWait = tl_wait(tl_younger(NMI, kNarrow));
     uint32_t doff[NMI];   // byte offset of lane's piece of copy `it` inside k slab 0
 #pragma unroll
     for (int it = 0; it < NMI; ++it)
@@ -216,7 +227,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
       }
     };
     fill_scales();
-    i32x4 wfrag[S][2][4];   // [stage][k half][16-row group]
+    i32x4 wfrag[S][2][NG];   // [stage][k half][16-row group]
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int st = 0; st < S; ++st) stage_slab(min(st, nk - 1), st);
@@ -224,18 +235,18 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
 #pragma unroll
     for (int st = 0; st < S; ++st)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, min(st, nk - 1), h);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(kWait);
     __syncthreads();
 
-    vf32x4 acc[NMT][4];
+    vf32x4 acc[NMT][NG];
 #pragma unroll
     for (int mt = 0; mt < NMT; ++mt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) acc[mt][g] = vf32x4{0.f, 0.f, 0.f, 0.f};
+      for (int g = 0; g < NG; ++g) acc[mt][g] = vf32x4{0.f, 0.f, 0.f, 0.f};
 
     // fragment of lane (r, q), tile mt, half h: row 16*mt + r, position (q + 4h) ^ f(r)
     const int fsw = ((fr >> 1) & 7) ^ ((fr & 1) << 2);
@@ -248,7 +259,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
       const uint8_t* la = lds + cur * kSlab + a_row;
       const uint2 sb = *reinterpret_cast<const uint2*>(s_scales + kt * kPfBM + fr * 8);
       const float2 sw = *reinterpret_cast<const float2*>(s_scales + nk * kPfBM + kt * 8);
-      const float sw0 = kGateUp ? sw.x : (wave < 2 ? sw.x : sw.y), sw1 = kGateUp ? sw.y : sw0;
+      const float sw0 = kGateUp || kNarrow || wave < 2 ? sw.x : sw.y, sw1 = kGateUp ? sw.y : sw0;
       i32x4 fa[2][2][2];   // [parity][tile of the pair][half]
       if (NP == 1) {       // the copies go first, so that every height issues vector memory in the counted order
         stage_slab(kts, ahead);
@@ -293,8 +304,10 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
           };
           group(std::integral_constant<int, 0>{});
           group(std::integral_constant<int, 1>{});
-          group(std::integral_constant<int, 2>{});
-          group(std::integral_constant<int, 3>{});
+          if constexpr (NG > 2) {
+            group(std::integral_constant<int, 2>{});
+            group(std::integral_constant<int, 3>{});
+          }
           __builtin_amdgcn_sched_barrier(0);
           if (NP > 1 && pr == 0) {   // the copies of slab kt+S go out once the matrix pipe has work
             stage_slab(kts, ahead);
@@ -317,11 +330,17 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
       slab(std::integral_constant<int, 1>{}, kt + 1);
       if constexpr (S > 2) slab(std::integral_constant<int, 2>{}, kt + 2);
       if constexpr (S > 3) slab(std::integral_constant<int, 3>{}, kt + 3);
+      if constexpr (S > 4) slab(std::integral_constant<int, 4>{}, kt + 4);
+      if constexpr (S > 5) slab(std::integral_constant<int, 5>{}, kt + 5);
     }
     if (kt < nk) slab(std::integral_constant<int, 0>{}, kt);
     if (S > 2 && kt + 1 < nk) slab(std::integral_constant<int, 1>{}, kt + 1);
     if constexpr (S > 3)
       if (kt + 2 < nk) slab(std::integral_constant<int, 2>{}, kt + 2);
+    if constexpr (S > 4)
+      if (kt + 3 < nk) slab(std::integral_constant<int, 3>{}, kt + 3);
+    if constexpr (S > 5)
+      if (kt + 4 < nk) slab(std::integral_constant<int, 4>{}, kt + 4);
     __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);  // no copy may land in LDS after the epilogue starts to reuse it
     __syncthreads();
 
@@ -376,12 +395,12 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
       }
     } else {
       // 16-bit rows times their factor, staged per wavefront in two 32-column passes into 16-byte stores
-      uint8_t* st = lds + wave * (kPfBM * 64);
+      uint8_t* st = lds + wave * (kRows * 64);
       uint16_t* out = static_cast<uint16_t*>(dense ? a.p.out_s : a.p.out_r);
       // whole 16-byte stores need rows that start on 16-byte boundaries
       const bool whole = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
-      for (int pass = 0; pass < 2; ++pass) {
+      for (int pass = 0; pass < NG / 2; ++pass) {
         if (pass) __syncthreads();  // staging rows are reused
 #pragma unroll
         for (int mt = 0; mt < NMT; ++mt) {
@@ -398,7 +417,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
           }
         }
         __syncthreads();
-        const int ncol0 = n0 + wave * 64 + pass * 32;
+        const int ncol0 = n0 + wave * 16 * NG + pass * 32;
 #pragma unroll
         for (int it = 0; it < 2 * NMI; ++it) {
           const int m = it * 16 + (lane >> 2), q = lane & 3;
@@ -418,7 +437,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
       }
     }
   };
-  switch ((M + 31) >> 5) {
+  if constexpr (kNarrow) body(std::integral_constant<int, 1>{});
+  else switch ((M + 31) >> 5) {
     case 1: body(std::integral_constant<int, 1>{}); break;
     case 2: body(std::integral_constant<int, 2>{}); break;
     case 3: body(std::integral_constant<int, 3>{}); break;
@@ -426,13 +446,13 @@ __global__ __launch_bounds__(kPfThreads, 2) void f8_tile_kernel(const TileArgs a
   }
 }
 
-template <bool kGateUp>
+template <bool kGateUp, bool kNarrow>
 static int launch_tile(const TileArgs& a, int64_t grid, hipStream_t st) {
   SP_REQUIRE(grid < (1ll << 31), "fp8 product: grid too large");
   const int Kmax = a.p.Ks > a.p.Kr ? a.p.Ks : a.p.Kr;
   const unsigned dyn = static_cast<unsigned>(f8_blocks(Kmax)) * kTlScaleBytes;
 #define SP_TILE_LAUNCH(F, P) \
-  hipLaunchKernelGGL((f8_tile_kernel<F, kGateUp, P>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a)
+  hipLaunchKernelGGL((f8_tile_kernel<F, kGateUp, P, kNarrow>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a)
   if (a.p.dtype == SPARSE_HIP_F16) {
     if (a.p.pow2) SP_TILE_LAUNCH(Fp16, true); else SP_TILE_LAUNCH(Fp16, false);
   } else {
@@ -456,15 +476,18 @@ int f8_tile_gateup(const F8Product& p, const PfQueues& q, void* h, void* hs, voi
   a.qs_r = static_cast<uint8_t*>(hs);
   a.q_s = static_cast<uint8_t*>(sh);
   a.qs_s = static_cast<uint8_t*>(shs);
-  return launch_tile<true>(a, queue_grid(q.cap_gu), st);
+  return launch_tile<true, false>(a, queue_grid(q.cap_gu), st);
 }
 
-int f8_tile_down(const F8Product& p, const PfQueues& q, hipStream_t st) {
+int f8_tile_columns(int tile_rows) { return tile_rows <= kTlNarrowRows ? kPfBR / 2 : kPfBR; }
+
+int f8_tile_down(const F8Product& p, const PfQueues& q, int tile_rows, hipStream_t st) {
   TileArgs a = {};
   a.p = p;
   a.map = q.map_dn;
   a.qhdr = q.hdr + 16;
-  return launch_tile<false>(a, queue_grid(q.cap_dn), st);
+  return tile_rows <= kTlNarrowRows ? launch_tile<false, true>(a, queue_grid(q.cap_dn), st)
+                                    : launch_tile<false, false>(a, queue_grid(q.cap_dn), st);
 }
 
 int f8_tile_linear(const F8Product& p, int tile_rows, hipStream_t st) {
@@ -472,10 +495,12 @@ int f8_tile_linear(const F8Product& p, int tile_rows, hipStream_t st) {
   a.p = p;
   a.rows = tile_rows;
   a.mt = (p.T + tile_rows - 1) / tile_rows;
-  a.nt = (p.Ns + kPfBR - 1) / kPfBR;
+  const int columns = f8_tile_columns(tile_rows);
+  a.nt = (p.Ns + columns - 1) / columns;
   const int64_t total = static_cast<int64_t>(a.mt) * a.nt;
   SP_REQUIRE(total < (1ll << 30), "fp8_linear: too many tiles");
-  return launch_tile<false>(a, (total + kPfXcds - 1) / kPfXcds * kPfXcds, st);
+  const int64_t grid = (total + kPfXcds - 1) / kPfXcds * kPfXcds;
+  return tile_rows <= kTlNarrowRows ? launch_tile<false, true>(a, grid, st) : launch_tile<false, false>(a, grid, st);
 }
 
 }  // namespace sparse

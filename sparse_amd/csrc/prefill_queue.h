@@ -124,10 +124,10 @@ inline int pfx_max_mtiles(int Ttok, int K, int nseg, int tile_rows) { return (Tt
 struct PfxLayout {
   int nt_gu, nt_dn, nts_gu, nts_dn, mt_shared, cap_gu, cap_dn;
 };
-inline PfxLayout pfx_layout(int Ttok, int K, int nseg, int H, int I, int Is, int tile_rows) {
+inline PfxLayout pfx_layout(int Ttok, int K, int nseg, int H, int I, int Is, int tile_rows, int down_columns) {
   PfxLayout l;
   l.nt_gu = (I + kPfBR / 2 - 1) / (kPfBR / 2);
-  l.nt_dn = (H + kPfBR - 1) / kPfBR;
+  l.nt_dn = (H + down_columns - 1) / down_columns;
   l.nts_gu = Is > 0 ? (Is + kPfBR / 2 - 1) / (kPfBR / 2) : 0;
   l.nts_dn = Is > 0 ? l.nt_dn : 0;
   l.mt_shared = Is > 0 ? (Ttok + tile_rows - 1) / tile_rows : 0;
@@ -139,8 +139,9 @@ inline PfxLayout pfx_layout(int Ttok, int K, int nseg, int H, int I, int Is, int
 
 constexpr size_t kPfWsHeader = 256;   // two launches x 16 ints, padded
 
-inline size_t prefill_queue_ws_bytes(int Ttok, int K, int nseg, int H, int I, int Is, int tile_rows = kPfBM) {
-  const PfxLayout l = pfx_layout(Ttok, K, nseg, H, I, Is, tile_rows);
+inline size_t prefill_queue_ws_bytes(int Ttok, int K, int nseg, int H, int I, int Is, int tile_rows = kPfBM,
+                                     int down_columns = kPfBR) {
+  const PfxLayout l = pfx_layout(Ttok, K, nseg, H, I, Is, tile_rows, down_columns);
   return kPfWsHeader + (static_cast<size_t>(l.cap_gu) + l.cap_dn) * sizeof(PfTile);
 }
 
@@ -148,8 +149,8 @@ inline size_t prefill_queue_ws_bytes(int Ttok, int K, int nseg, int H, int I, in
 // they will be.
 inline PfQueues prefill_queue_args(const int32_t* expert_slot, const int32_t* seg_offsets, const sparse_hip_seglist& segs,
                                    int Ttok, int K, int H, int I, int Is, void* tile_ws, PfxMapArgs* args,
-                                   int tile_rows = kPfBM) {
-  const PfxLayout l = pfx_layout(Ttok, K, segs.n, H, I, Is, tile_rows);
+                                   int tile_rows = kPfBM, int down_columns = kPfBR) {
+  const PfxLayout l = pfx_layout(Ttok, K, segs.n, H, I, Is, tile_rows, down_columns);
   int32_t* hdr = static_cast<int32_t*>(tile_ws);
   PfTile* map_gu = reinterpret_cast<PfTile*>(static_cast<uint8_t*>(tile_ws) + kPfWsHeader);
   PfTile* map_dn = map_gu + l.cap_gu;
