@@ -259,6 +259,10 @@ __device__ __forceinline__ bool f8_where(const F8Product& a, int block, int tile
 // Two rows at most: gate/up (SwiGLU of two products, fp32 out) or a single product, of rows that are
 // quantised on the way in (from the 16-bit type, from fp32) or were before.
 constexpr int kF8FewRows = 2;
+// From this many blocks of 128 on, workgroups of 8 wavefronts instead of 4 stream a single matrix past up to 16 rows:
+// its 16-column workgroups do not fill the device, and the depth of a wavefront's share is the call's time.  One row of
+// 5632 by 2048 weight rows 7.2 -> 5.7 us, of 4096 by 4096 6.6 -> 5.9; of 2048 by 5632, 16 blocks, 5.5 -> 5.9.
+constexpr int kF8LongBlocks = 20;
 enum { kF8From16 = 0, kF8From32 = 1, kF8From8 = 2 };
 int f8_few(const F8Product& p, int source, bool gateup, bool routed, bool dense, hipStream_t st);
 

@@ -3,8 +3,9 @@
 //
 //   y[m, n] = sum over blocks b of 2^e(m, b) s(n, b) sum over k in b of q[m, k] w[n, k],  q, e: the quantiser's
 //
-// A workgroup owns 16 output columns (weight rows) of two matrices (gate and up of one expert) or of one.  Its four
-// wavefronts deal the 128-wide k blocks among themselves, a chunk of 4 KW blocks at a time; each wavefront requests
+// A workgroup owns 16 output columns (weight rows) of two matrices (gate and up of one expert) or of one.  Its
+// wavefronts, four or, for a single matrix of long rows, eight (kF8LongBlocks), deal the 128-wide k blocks among
+// themselves, a chunk of KW blocks each at a time; each wavefront requests
 // its weights of a chunk (2 KB a block, straight from the tiled layout into registers) two chunks ahead, and while
 // they travel the workgroup quantises its rows of the chunk: 16 lanes hold a run of 128, find its largest
 // magnitude, round to 8 bits and put the rounded values down as bf16, which holds them exactly, with the run's
@@ -26,15 +27,8 @@
 
 namespace sparse {
 
-constexpr int kFwThreads = 256;
-constexpr int kFwWaves = kFwThreads / 64;
 constexpr int kSrc16 = kF8From16, kSrc32 = kF8From32, kSrc8 = kF8From8;
-
 constexpr int KW = 2;                             // blocks of a chunk per wavefront
-constexpr int KC = kFwWaves * KW;                 // blocks of a chunk
-constexpr int kFwValues = KC * kF8Block * 2;      // LDS row of a chunk: values, scales
-constexpr int kFwStride = kFwValues + KC * 4;
-static_assert(kFwThreads / 16 == kF8FewRows * KC, "one run of a chunk for each 16 lanes");
 
 // Eight values of a run, one sixteenth of it, on their way to LDS.
 __device__ __forceinline__ u32x4 fw_round(const float (&v)[8], float& scale) {
@@ -104,10 +98,14 @@ struct Source<F, kSrc8, kVec> {
   }
 };
 
-// kGateUp: two matrices, gate and up, fp32 SwiGLU out.  Otherwise one.
-template <typename F, bool kGateUp, int kSrc, bool kVec>
-__global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, int tiles_r, int tiles_s) {
+// kGateUp: two matrices, gate and up, fp32 SwiGLU out.  Otherwise one.  kFwWaves: wavefronts of a workgroup.
+template <typename F, bool kGateUp, int kSrc, bool kVec, int kFwWaves>
+__global__ __launch_bounds__(kFwWaves * 64) void f8_few_kernel(const F8Product a, int tiles_r, int tiles_s) {
   constexpr int NM = kGateUp ? 2 : 1;
+  constexpr int KC = kFwWaves * KW;                 // blocks of a chunk
+  constexpr int kFwValues = KC * kF8Block * 2;      // LDS row of a chunk: values, scales
+  constexpr int kFwStride = kFwValues + KC * 4;
+  static_assert(kFwWaves * 4 == kF8FewRows * KC, "one run of a chunk for each 16 lanes");
   constexpr int kStage = 2 * kF8FewRows * kFwStride, kSums = kFwWaves * NM * 64 * static_cast<int>(sizeof(vf32x4));
   __shared__ __attribute__((aligned(16))) uint8_t lds[kStage > kSums ? kStage : kSums];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -266,13 +264,13 @@ __global__ __launch_bounds__(kFwThreads) void f8_few_kernel(const F8Product a, i
   }
 }
 
-template <typename F, bool kGateUp, int kSrc, bool kVec>
+template <typename F, bool kGateUp, int kSrc, bool kVec, int W = 4>
 static int launch_few(const F8Product& p, int tiles_r, int tiles_s, hipStream_t st) {
   const int64_t grid = tiles_s + static_cast<int64_t>(tiles_r) * p.segs.n;
   if (grid == 0) return SPARSE_HIP_OK;
   SP_REQUIRE(grid < (1ll << 31), "fp8 product: grid too large");
   SP_REQUIRE(p.T <= kF8FewRows, "fp8 product: %d rows", p.T);
-  hipLaunchKernelGGL((f8_few_kernel<F, kGateUp, kSrc, kVec>), dim3(static_cast<unsigned>(grid)), dim3(kFwThreads), 0, st, p,
+  hipLaunchKernelGGL((f8_few_kernel<F, kGateUp, kSrc, kVec, W>), dim3(static_cast<unsigned>(grid)), dim3(W * 64), 0, st, p,
                      tiles_r, tiles_s);
   SP_LAUNCH_CHECK("f8_few_kernel");
   return SPARSE_HIP_OK;
@@ -282,11 +280,14 @@ template <typename F>
 static int few_as(const F8Product& p, int source, bool gateup, bool routed, bool dense, hipStream_t st) {
   const int tr = routed ? (p.Nr + 15) / 16 : 0, ts = dense ? (p.Ns + 15) / 16 : 0;
   if (source == kF8From32) return launch_few<F, false, kSrc32, true>(p, tr, ts, st);
-  if (source == kF8From8) return launch_few<F, false, kSrc8, true>(p, tr, ts, st);
+  const bool wide = !routed && f8_blocks(p.Ks) > kF8LongBlocks;
+  if (source == kF8From8)
+    return wide ? launch_few<F, false, kSrc8, true, 8>(p, tr, ts, st) : launch_few<F, false, kSrc8, true>(p, tr, ts, st);
   // 16-byte loads of the rows need aligned rows of a multiple of eight values
   const int K = dense ? p.Ks : p.Kr;
   const bool vec = K % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.act_s) | reinterpret_cast<uintptr_t>(p.act_r)) & 15) == 0;
   if (gateup) return vec ? launch_few<F, true, kSrc16, true>(p, tr, ts, st) : launch_few<F, true, kSrc16, false>(p, tr, ts, st);
+  if (wide) return vec ? launch_few<F, false, kSrc16, true, 8>(p, tr, ts, st) : launch_few<F, false, kSrc16, false, 8>(p, tr, ts, st);
   return vec ? launch_few<F, false, kSrc16, true>(p, tr, ts, st) : launch_few<F, false, kSrc16, false>(p, tr, ts, st);
 }
 

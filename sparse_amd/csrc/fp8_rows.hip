@@ -4,8 +4,8 @@
 //   y[m, n] = sum over blocks b of 2^e(m, b) s(n, b) sum over k in b of x[m, k] w[n, k]
 //
 // What bounds it is the weights' way from HBM.  A workgroup owns 16 output columns of two matrices (gate and up
-// of one expert) or of one, and up to 16 NTmax rows of a segment.  Its four wavefronts deal the 128-wide k blocks
-// among themselves, one block a register stage, two stages in flight: that leaves registers for four to five
+// of one expert) or of one, and up to 16 NTmax rows of a segment.  Its wavefronts, four or, for a single matrix of
+// long rows, eight (kF8LongBlocks), deal the 128-wide k blocks among themselves, one block a register stage, two stages in flight: that leaves registers for four to five
 // wavefronts on a SIMD, whose loads together keep HBM busy (two blocks a stage: down of 8 tokens 15.6 us instead
 // of 14.4; two column groups a workgroup: 23).  Rows are read from L2 by every workgroup of their segment, in the
 // matrix instruction's own layout: no LDS and no barrier before the wavefronts' sums meet.  Quantising the rows
@@ -25,12 +25,10 @@
 
 namespace sparse {
 
-constexpr int kRwThreads = 256;
-constexpr int kRwWaves = kRwThreads / 64;
-
 // NTmax: 16-row groups at most; a segment takes the form of the groups it has.
-template <typename F, bool kGateUp, int NTmax>
-__global__ __launch_bounds__(kRwThreads) void f8_rows_kernel(const F8Product a, int tiles_r, int tiles_s) {
+// kRwWaves: wavefronts of a workgroup
+template <typename F, bool kGateUp, int NTmax, int kRwWaves>
+__global__ __launch_bounds__(kRwWaves * 64) void f8_rows_kernel(const F8Product a, int tiles_r, int tiles_s) {
   constexpr int NM = kGateUp ? 2 : 1;
   __shared__ vf32x4 red[kRwWaves][NTmax * NM][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -188,14 +186,14 @@ __global__ __launch_bounds__(kRwThreads) void f8_rows_kernel(const F8Product a, 
   else body(std::integral_constant<int, NTmax>{});
 }
 
-template <typename F, bool kGateUp, int NT>
+template <typename F, bool kGateUp, int NT, int W>
 static int launch_rows(const F8Product& p, int tiles_r, int tiles_s, hipStream_t st) {
   const int64_t grid = tiles_s + static_cast<int64_t>(tiles_r) * p.segs.n;
   const int64_t groups = (p.T + 16 * NT - 1) / (16 * NT);
   if (grid == 0) return SPARSE_HIP_OK;
   SP_REQUIRE(grid < (1ll << 31) && groups < 65536, "fp8 product: grid too large");
-  hipLaunchKernelGGL((f8_rows_kernel<F, kGateUp, NT>), dim3(static_cast<unsigned>(grid), static_cast<unsigned>(groups)),
-                     dim3(kRwThreads), 0, st, p, tiles_r, tiles_s);
+  hipLaunchKernelGGL((f8_rows_kernel<F, kGateUp, NT, W>), dim3(static_cast<unsigned>(grid), static_cast<unsigned>(groups)),
+                     dim3(W * 64), 0, st, p, tiles_r, tiles_s);
   SP_LAUNCH_CHECK("f8_rows_kernel");
   return SPARSE_HIP_OK;
 }
@@ -203,9 +201,10 @@ static int launch_rows(const F8Product& p, int tiles_r, int tiles_s, hipStream_t
 template <typename F>
 static int rows_as(const F8Product& p, bool gateup, bool routed, bool dense, hipStream_t st) {
   const int groups_r = routed ? (p.Nr + 15) / 16 : 0, groups_s = dense ? (p.Ns + 15) / 16 : 0;
-  if (p.T <= 16)
-    return gateup ? launch_rows<F, true, 1>(p, groups_r, groups_s, st) : launch_rows<F, false, 1>(p, groups_r, groups_s, st);
-  return gateup ? launch_rows<F, true, 2>(p, groups_r, groups_s, st) : launch_rows<F, false, 2>(p, groups_r, groups_s, st);
+  if (gateup) return p.T <= 16 ? launch_rows<F, true, 1, 4>(p, groups_r, groups_s, st) : launch_rows<F, true, 2, 4>(p, groups_r, groups_s, st);
+  if (p.T > 16) return launch_rows<F, false, 2, 4>(p, groups_r, groups_s, st);
+  return !routed && f8_blocks(p.Ks) > kF8LongBlocks ? launch_rows<F, false, 1, 8>(p, groups_r, groups_s, st)
+                                                    : launch_rows<F, false, 1, 4>(p, groups_r, groups_s, st);
 }
 
 int f8_rows(const F8Product& p, bool gateup, bool routed, bool dense, hipStream_t st) {

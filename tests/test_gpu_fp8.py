@@ -415,3 +415,17 @@ def test_slots_outside_the_slab_are_refused(device):
     for slot in (2, -1):
         with pytest.raises(ValueError, match="slots outside"):
             fp8.moe_ffn(few, d["x"], topv, perm, segs=ops.seglist_host([1, 3], [0, slot]))
+
+
+@pytest.mark.parametrize("K", [2560, 2561, 5632])
+@pytest.mark.parametrize("T", [1, 2, 9, 16, 17])
+def test_linear_on_both_sides_of_the_long_rows(device, T, K):
+    """20, 21 and 44 blocks: a few rows take more wavefronts from the second on; given as 16-bit rows and as 8-bit ones."""
+    N = 83
+    q, s = rand_weight(N, K)
+    x = rand_rows(T, K, torch.bfloat16)
+    w = fp8.Weight.from_quantized(q.to(device), s.to(device))
+    want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s), grouped(T))
+    got = fp8.linear(x.to(device), w)
+    within(got, want, bound, torch.bfloat16)
+    assert torch.equal(fp8.linear(fp8.quantize(x.to(device)), w), got)
