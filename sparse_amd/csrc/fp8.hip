@@ -55,6 +55,14 @@ static int ffn_tile_rows(int T, int K, int E, int H, int I) {
   return tile_rows(static_cast<int64_t>(T) * K, E / 2, nt_gu > nt_dn ? nt_gu : nt_dn);
 }
 
+// Rows of the shared expert's gate/up tiles: higher ones, beside routed tiles that leave less room.  128 tokens, 4 of 60
+// experts of 1408 x 2048 and a shared one of 5632: 176 tiles of 32 rows behind 600 routed ones 122 us, 88 of 64 109.
+static int ffn_shared_rows(int T, int K, int E, int I, int Is, int rows) {
+  const int64_t routed = (static_cast<int64_t>(T) * K / rows + E / 2) * ((I + kPfBR / 2 - 1) / (kPfBR / 2));
+  while (rows < kPfBM && routed + static_cast<int64_t>((T + rows - 1) / rows) * ((Is + kPfBR / 2 - 1) / (kPfBR / 2)) > 512) rows *= 2;
+  return rows;
+}
+
 static inline size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 // A workspace handed out front to back in 256-byte steps; with a null base it only counts.
@@ -107,7 +115,8 @@ static FfnWs ffn_ws(void* ws, int T, int K, int E, int nseg, int H, int I, int I
   }
   if (ffn_tiles(T, K, E, H, I)) {
     const int rows_per_tile = ffn_tile_rows(T, K, E, H, I);
-    w.tiles = c.take(prefill_queue_ws_bytes(T, K, nseg, H, I, Is, rows_per_tile, f8_tile_columns(rows_per_tile)));
+    w.tiles = c.take(prefill_queue_ws_bytes(T, K, nseg, H, I, Is, rows_per_tile, f8_tile_columns(rows_per_tile),
+                                            ffn_shared_rows(T, K, E, I, Is, rows_per_tile)));
   } else {
     w.hf = static_cast<float*>(c.take(static_cast<size_t>(rows) * I * sizeof(float)));
     if (Is > 0) w.shf = static_cast<float*>(c.take(static_cast<size_t>(T) * Is * sizeof(float)));
@@ -267,7 +276,8 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   if (tiles) {
     PfxMapArgs queue_args;
     queues = prefill_queue_args(experts->expert_slot_dev, seg_offsets_dev, *segs, T, K, H, I, Is, w.tiles, &queue_args,
-                                rows_per_tile, f8_tile_columns(rows_per_tile));
+                                rows_per_tile, f8_tile_columns(rows_per_tile),
+                                ffn_shared_rows(T, K, E, I, Is, rows_per_tile));
     rc = f8_quantize_and_queue({x_dev, T, H, w.x.values, w.x.scales}, dtype, queue_args, st);
   } else if (!few) {
     rc = f8_quantize({x_dev, T, H, w.x.values, w.x.scales}, {}, dtype, st);

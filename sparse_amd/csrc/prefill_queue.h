@@ -16,10 +16,11 @@ struct PfxMapArgs {
   PfTile* map_dn;
   int32_t nt_gu, nt_dn;    // column tiles of a routed expert
   int32_t nts_gu, nts_dn;  // column tiles of the shared expert (0: none)
-  int32_t mt_shared;       // row tiles of the shared expert
+  int32_t mts_gu, mts_dn;  // row tiles of the shared expert
   int32_t T;               // tokens (rows of the shared expert)
   int32_t cap_gu, cap_dn;  // entries in each map
   int32_t tile_rows;       // rows per tile, kPfBM or fewer
+  int32_t shared_rows;     // ... of the shared expert's gate/up tiles
 };
 
 // Share x of n items cut into kPfXcds contiguous shares starts here.
@@ -69,7 +70,7 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
     PfTile* map = which == 0 ? a.map_gu : a.map_dn;
     const int nt = which == 0 ? a.nt_gu : a.nt_dn;
     const int cap = which == 0 ? a.cap_gu : a.cap_dn;
-    const int R = total_mt * nt, S = a.mt_shared * (which == 0 ? a.nts_gu : a.nts_dn);
+    const int R = total_mt * nt, S = which == 0 ? a.mts_gu * a.nts_gu : a.mts_dn * a.nts_dn;
     if (mt > 0) {
       const int g0 = (scan - mt) * nt + bn * mt;
       for (int bm = 0; bm < mt; ++bm) {
@@ -85,7 +86,8 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
   PfTile* map = which == 0 ? a.map_gu : a.map_dn;
   const int nt = which == 0 ? a.nt_gu : a.nt_dn;
   const int cap = which == 0 ? a.cap_gu : a.cap_dn;
-  const int R = total_mt * nt, S = a.mt_shared * (which == 0 ? a.nts_gu : a.nts_dn);
+  const int mts = which == 0 ? a.mts_gu : a.mts_dn, rows_s = which == 0 ? a.shared_rows : a.tile_rows;
+  const int R = total_mt * nt, S = mts * (which == 0 ? a.nts_gu : a.nts_dn);
   // The shared expert's tiles.  Where the tile grid divides evenly, XCD x takes a block of it -- a quarter
   // of the row tiles by half of the column tiles -- and walks the block down its rows first, so that the
   // 64 workgroups an XCD runs at a time cover about 8 x 8 tiles: each activation row tile and each weight
@@ -93,8 +95,8 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
   // the whole activation matrix, four times its L2, once per column tile.)  Otherwise: contiguous shares
   // of the (column tile, row tile) order.
   const int nts = which == 0 ? a.nts_gu : a.nts_dn;
-  const bool blocked = a.mt_shared % 4 == 0 && nts % 2 == 0 && nts > 0;
-  const int RG = a.mt_shared / 4, per_xcd = S / kPfXcds;
+  const bool blocked = mts % 4 == 0 && nts % 2 == 0 && nts > 0;
+  const int RG = mts / 4, per_xcd = S / kPfXcds;
   for (int h = tid; h < S; h += 256) {
     int bn, bm, x, local;
     if (blocked) {
@@ -103,13 +105,13 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
       bm = (x & 3) * RG + local % RG;
       bn = (x >> 2) * (nts / 2) + local / RG;
     } else {
-      bn = h / a.mt_shared;
-      bm = h - bn * a.mt_shared;
+      bn = h / mts;
+      bm = h - bn * mts;
       x = pfx_share_of(S, h);
       local = h - pfx_start(S, x);
     }
     const int pos = pfx_queue_base(R, S, x) + local;
-    if (pos < cap) map[pos] = PfTile{-1, bm * a.tile_rows, min(a.tile_rows, a.T - bm * a.tile_rows), bn};
+    if (pos < cap) map[pos] = PfTile{-1, bm * rows_s, min(rows_s, a.T - bm * rows_s), bn};
   }
   if (tid == 0) map[0] = PfTile{0, 0, 0, 0};
   if (tid < kPfXcds) {
@@ -122,26 +124,27 @@ __device__ __forceinline__ void prefill_queue_block(const PfxMapArgs& a, const i
 inline int pfx_max_mtiles(int Ttok, int K, int nseg, int tile_rows) { return (Ttok * K + tile_rows - 1) / tile_rows + nseg; }
 
 struct PfxLayout {
-  int nt_gu, nt_dn, nts_gu, nts_dn, mt_shared, cap_gu, cap_dn;
+  int nt_gu, nt_dn, nts_gu, nts_dn, mts_gu, mts_dn, cap_gu, cap_dn;
 };
-inline PfxLayout pfx_layout(int Ttok, int K, int nseg, int H, int I, int Is, int tile_rows, int down_columns) {
+inline PfxLayout pfx_layout(int Ttok, int K, int nseg, int H, int I, int Is, int tile_rows, int down_columns, int shared_rows) {
   PfxLayout l;
   l.nt_gu = (I + kPfBR / 2 - 1) / (kPfBR / 2);
   l.nt_dn = (H + down_columns - 1) / down_columns;
   l.nts_gu = Is > 0 ? (Is + kPfBR / 2 - 1) / (kPfBR / 2) : 0;
   l.nts_dn = Is > 0 ? l.nt_dn : 0;
-  l.mt_shared = Is > 0 ? (Ttok + tile_rows - 1) / tile_rows : 0;
+  l.mts_gu = Is > 0 ? (Ttok + shared_rows - 1) / shared_rows : 0;
+  l.mts_dn = Is > 0 ? (Ttok + tile_rows - 1) / tile_rows : 0;
   const int mt = nseg > 0 ? pfx_max_mtiles(Ttok, K, nseg, tile_rows) : 0;
-  l.cap_gu = 1 + mt * l.nt_gu + l.mt_shared * l.nts_gu;
-  l.cap_dn = 1 + mt * l.nt_dn + l.mt_shared * l.nts_dn;
+  l.cap_gu = 1 + mt * l.nt_gu + l.mts_gu * l.nts_gu;
+  l.cap_dn = 1 + mt * l.nt_dn + l.mts_dn * l.nts_dn;
   return l;
 }
 
 constexpr size_t kPfWsHeader = 256;   // two launches x 16 ints, padded
 
 inline size_t prefill_queue_ws_bytes(int Ttok, int K, int nseg, int H, int I, int Is, int tile_rows = kPfBM,
-                                     int down_columns = kPfBR) {
-  const PfxLayout l = pfx_layout(Ttok, K, nseg, H, I, Is, tile_rows, down_columns);
+                                     int down_columns = kPfBR, int shared_rows = kPfBM) {
+  const PfxLayout l = pfx_layout(Ttok, K, nseg, H, I, Is, tile_rows, down_columns, shared_rows);
   return kPfWsHeader + (static_cast<size_t>(l.cap_gu) + l.cap_dn) * sizeof(PfTile);
 }
 
@@ -149,8 +152,8 @@ inline size_t prefill_queue_ws_bytes(int Ttok, int K, int nseg, int H, int I, in
 // they will be.
 inline PfQueues prefill_queue_args(const int32_t* expert_slot, const int32_t* seg_offsets, const sparse_hip_seglist& segs,
                                    int Ttok, int K, int H, int I, int Is, void* tile_ws, PfxMapArgs* args,
-                                   int tile_rows = kPfBM, int down_columns = kPfBR) {
-  const PfxLayout l = pfx_layout(Ttok, K, segs.n, H, I, Is, tile_rows, down_columns);
+                                   int tile_rows = kPfBM, int down_columns = kPfBR, int shared_rows = kPfBM) {
+  const PfxLayout l = pfx_layout(Ttok, K, segs.n, H, I, Is, tile_rows, down_columns, shared_rows);
   int32_t* hdr = static_cast<int32_t*>(tile_ws);
   PfTile* map_gu = reinterpret_cast<PfTile*>(static_cast<uint8_t*>(tile_ws) + kPfWsHeader);
   PfTile* map_dn = map_gu + l.cap_gu;
@@ -165,11 +168,13 @@ inline PfQueues prefill_queue_args(const int32_t* expert_slot, const int32_t* se
   m.nt_dn = l.nt_dn;
   m.nts_gu = l.nts_gu;
   m.nts_dn = l.nts_dn;
-  m.mt_shared = l.mt_shared;
+  m.mts_gu = l.mts_gu;
+  m.mts_dn = l.mts_dn;
   m.T = Ttok;
   m.cap_gu = l.cap_gu;
   m.cap_dn = l.cap_dn;
   m.tile_rows = tile_rows;
+  m.shared_rows = shared_rows;
   *args = m;
   return PfQueues{hdr, map_gu, map_dn, l.cap_gu, l.cap_dn};
 }

@@ -429,3 +429,17 @@ def test_linear_on_both_sides_of_the_long_rows(device, T, K):
     got = fp8.linear(x.to(device), w)
     within(got, want, bound, torch.bfloat16)
     assert torch.equal(fp8.linear(fp8.quantize(x.to(device)), w), got)
+
+
+def test_shared_tiles_higher_than_routed_ones(device):
+    """So many routed tiles that the shared expert's gate/up takes tiles of 64 rows beside routed ones of 32."""
+    c = make_case(120, 64, 60, 1408, 4, 640, True, torch.bfloat16, seed=21)
+    d = on_gpu(c, device)
+    old = _lib.load().sparse_hip_fp8_path(2)
+    try:
+        parts, shared = fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"], shared=d["sh"], shared_gate=d["sg"])
+    finally:
+        _lib.load().sparse_hip_fp8_path(old)
+    want, bound, wsh, bsh = oracle(c, "tiles")
+    within(parts, want, bound, torch.bfloat16)
+    within(shared, wsh, bsh, torch.bfloat16)
