@@ -17,8 +17,8 @@
 // behind the loads.  Down and single products, rounded to 16 bits, take the 8-bit instruction with the rows'
 // scales as its operand.
 //
-// 8 tokens of 4 among 60 experts of 1408 x 2048 and a shared one of 5632: gate/up 170 MB in 24.8 us (6.9 TB/s),
-// down 85 MB in 14.5 us (5.9 TB/s).  333 rows of 1000 by 1418 weight rows, the border to the tile kernel: 9.3 us.
+// 8 tokens of 4 among 60 experts of 1408 x 2048 and a shared one of 5632: gate/up 170 MB in 24.4 us (7.0 TB/s),
+// down 85 MB in 14 us (6.1 TB/s).  From some 64 rows on the tile kernel is faster (fp8.hip has both sides).
 #include <type_traits>
 
 #include "fp8.h"
