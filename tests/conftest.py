@@ -20,3 +20,16 @@ def device():
     if not torch.cuda.is_available():
         pytest.skip("no GPU visible")
     return torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _no_garbage_left():
+    """Blocks are reference cycles that hold captured graphs, so their device memory is given back when the collector
+    next runs: at the end of each module rather than inside a later test that watches the free memory."""
+    yield
+    torch = sys.modules.get("torch")
+    if torch is not None and torch.cuda.is_available() and torch.cuda.is_initialized():
+        import gc
+
+        gc.collect()
+        torch.cuda.synchronize()
