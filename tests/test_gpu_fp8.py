@@ -443,3 +443,37 @@ def test_shared_tiles_higher_than_routed_ones(device):
     want, bound, wsh, bsh = oracle(c, "tiles")
     within(parts, want, bound, torch.bfloat16)
     within(shared, wsh, bsh, torch.bfloat16)
+
+
+def test_linear_long_rows_in_high_tiles(device):
+    """The longest rows again, in tiles of 128 rows: their scales take most of what LDS the slabs leave."""
+    T, K, N = 2048, 65536, 4352
+    q, s = rand_weight(256, K)
+    x = rand_rows(16, K, torch.bfloat16)
+    w = fp8.Weight.from_quantized(q.to(device).repeat(N // 256, 1), s.to(device).repeat(N // 256, 1))
+    got = fp8.linear(x.to(device).repeat(T // 16, 1), w).view(T // 16, 16, N // 256, 256)
+    assert torch.equal(got, got[:1, :, :1].expand_as(got))
+    want, bound = ref_fp8.product(ref_fp8.rows(x), (q[:16], s[:1]), True)
+    within(got[0, :, 0, :16], want, bound, torch.bfloat16)
+
+
+def test_experts_without_tokens(device):
+    c = make_case(4, 128, 4, 64, 2, 64, False, torch.bfloat16, seed=5)
+    d = on_gpu(c, device)
+    perm = ops.Permutation(0, 2, 4, device)          # (permute_build itself takes one token and more)
+    parts, shared = fp8.moe_ffn(d["slab"], d["x"][:0], d["topv"][:0], perm, shared=d["sh"])
+    assert parts.shape == (0, 128) and shared.shape == (0, 128)
+
+
+def test_arguments_that_are_refused(device):
+    q, s = rand_weight(32, 64)
+    w = fp8.Weight.from_quantized(q.to(device), s.to(device))
+    x = rand_rows(4, 64, torch.bfloat16).to(device)
+    for bad in (x.t().contiguous().t(), x.float(), x[:, :32].contiguous(), x.cpu(), x[0]):
+        with pytest.raises(ValueError):
+            fp8.linear(bad, w)
+    for out in (torch.empty(4, 32, device=device), torch.empty(4, 33, device=device, dtype=x.dtype)):
+        with pytest.raises(ValueError):
+            fp8.linear(x, w, out)
+    with pytest.raises(ValueError):
+        fp8.quantize(x.t())
