@@ -10,6 +10,8 @@
 // decides something is checked: the gap between two neighbours of the ranking, the last chosen and the first
 // not chosen among them, and between any two groups, is larger than both errors, or the token starts over in
 // 64 bits (about one token in a hundred of 256 random logits; equal 16-bit logits without a bias always do).
+// A group's sum of two is as far off as its two terms together, however small it is itself: where large biases
+// of both signs cancel in it, the 32-bit sum may be rounding alone.
 // 32-bit maxima cross the lanes in one instruction a step where 64-bit ones take a dozen: one token of 256
 // experts in 8 groups 8.7 -> 5.4 us, 4096 tokens 17.1 -> 12.5 us.  What is left is the latency of the K + 1
 // maxima, one behind the other, of the groups and of the exponentials in 64 bits: 4 MB of logits are read in a
@@ -98,13 +100,17 @@ __device__ __forceinline__ bool select_by(const SelectArgs& a, V (&r)[NV], V* s_
       second = b2 > best ? (best > s2 ? best : s2) : (second > b2 ? second : b2);
       best = b2 > best ? b2 : best;
     }
-    if (a.top2 && gsz > 1) best += second;
+    V mag = size(best);                        // of what a group's score is the sum of
+    if (a.top2 && gsz > 1) {
+      mag += size(second);
+      best += second;
+    }
     if (!(best == best)) best = kLow;          // an infinite bias beside a score that ranks last
     int before = 0;
     for (int i = 0; i < a.n_group; ++i) {
       const V v = read_lane(best, i * L);
       before += v > best || (kExact && v == best && i < g);
-      if (!kExact) clear &= i == g || g >= a.n_group || size(v - best) > 2 * slack(best);
+      if (!kExact) clear &= i == g || g >= a.n_group || size(v - best) > slack(mag) + slack(read_lane(mag, i * L));
     }
     const unsigned long long keep = __ballot(g < a.n_group && part == 0 && before < a.topk_group);
     const float per = 1.f / static_cast<float>(gsz);

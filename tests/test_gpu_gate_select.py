@@ -154,3 +154,27 @@ def test_graph_replay_and_other_stream(device):
 def test_no_rows(device):
     topv, topi = ops.gate_select(torch.empty(0, 16, device=device), 4)
     assert topv.shape == (0, 4) and topi.shape == (0, 4)
+
+
+def test_group_sums_that_cancel(device):
+    """The two best of each group are large and of opposite sign, so that their sums differ by less than 32 bits hold of
+    the terms: the 64-bit sums decide (0.80088 against 0.80067: the first group)."""
+    logits = torch.tensor([[0.00351563, -0.84729785, 0.00429688, -0.84920335]])
+    bias = torch.tensor([16384.0, -16384.0, 16384.0, -16384.0])
+    for _ in range(2):
+        check(logits, 1, torch.float32, device, score="sigmoid", bias=bias, n_group=2, topk_group=1, group_score="top2")
+        logits, bias = logits.view(2, 2).flip(0).reshape(1, 4).contiguous(), bias.clone()
+
+
+@pytest.mark.parametrize("size", [1.0, 16.0, 128.0, 256.0, 1024.0, 16384.0, 1e5])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_large_biases_of_both_signs(device, score, size):
+    """Groups of two whose sums nearly tie beside biases of ``size`` and ``-size``."""
+    g = torch.Generator().manual_seed(int(size))
+    T = 3000
+    base = torch.randn(T, 1, 2, generator=g)
+    logits = (base + torch.randn(T, 4, 2, generator=g) * 2.0 ** -6).reshape(T, 8).contiguous()
+    bias = torch.tensor([size, -size]).repeat(4)
+    for topk_group in (1, 2):
+        check(logits, 1, torch.float32, device, score=score, bias=bias, n_group=4, topk_group=topk_group, group_score="top2")
+    check(logits, 2, torch.float32, device, score=score, bias=bias, n_group=4, topk_group=3, group_score="max")
