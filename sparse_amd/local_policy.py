@@ -170,14 +170,14 @@ def measure_costs(block: Any, batches: Sequence[int] = (1, 4, 8, 16, 32), repeat
                   expert_bytes: Optional[int] = None) -> Dict[str, float]:
     """Measure the cost fields on the running GPU with an all-resident block of the layer
     shape in question.  Copy rate and latency: a pinned-host to HBM copy of one expert's
-    bytes against a 4 KiB one.  Compute: the routed grouped-FFN launch timed at several
+    bytes (8-bit experts: those of a slot) against a 4 KiB one.  Compute: the routed grouped-FFN launch timed at several
     decode batch sizes, fitted by least squares to ``expert_ms * experts + item_ms * rows``
     (both clamped at zero).  ``next_attention_ms`` and ``split_overhead_ms`` are set to the
     smallest launch time seen: in an attention-free stack that is all a prefetch can hide
     behind besides the routed compute, and roughly what one more launch boundary costs."""
     import numpy as np
     import torch
-    from . import ops
+    from . import fp8, ops
     if getattr(block, "residency", None) is not None:
         raise ValueError("measure_costs needs a block with expert_offload='gpu'")
     stream = torch.cuda.current_stream().cuda_stream
@@ -193,8 +193,10 @@ def measure_costs(block: Any, batches: Sequence[int] = (1, 4, 8, 16, 32), repeat
         torch.cuda.synchronize()
         return start.elapsed_ms(end) / n
 
+    eight = block.weight_format == "fp8"
     elem = 4 if block.dtype == torch.float32 else 2
-    nbytes = int(expert_bytes) if expert_bytes else 3 * block.hidden_size * block.inter_size * elem
+    stored = block.slab.expert_bytes if eight else 3 * block.hidden_size * block.inter_size * elem
+    nbytes = int(expert_bytes) if expert_bytes else stored
     host = ops.host_alloc(nbytes)
     try:
         dev = torch.empty(nbytes, dtype=torch.uint8, device=block.device)
@@ -213,8 +215,14 @@ def measure_costs(block: Any, batches: Sequence[int] = (1, 4, 8, 16, 32), repeat
         block._route(x, ws)
         offsets = ws.perm.seg_offsets.cpu().tolist()
         experts = sum(1 for e in range(block.num_experts) if offsets[e + 1] > offsets[e])
-        t = timed(lambda: ops.grouped_swiglu(block._experts_desc, x, ws.topv, ws.perm, ws.segs_dev, ws.inter,
-                                             ws.parts), repeats)
+
+        def run_experts():
+            if eight:
+                fp8.moe_ffn(block.slab, x, ws.topv, ws.perm, segs=ws.segs_dev, parts=ws.parts, ws=ws.fp8_ws)
+            else:
+                ops.grouped_swiglu(block._experts_desc, x, ws.topv, ws.perm, ws.segs_dev, ws.inter, ws.parts)
+
+        t = timed(run_experts, repeats)
         rows_a.append((experts, T * block.top_k))
         rows_t.append(t)
     sol, *_ = np.linalg.lstsq(np.asarray(rows_a, dtype=np.float64), np.asarray(rows_t, dtype=np.float64), rcond=None)

@@ -199,3 +199,17 @@ def test_deepseek_v3_model_with_swapped_blocks(device):
         harness.begin_request()
         got_ids = harness.greedy_decode(model, ids, mask, 5).cpu()
     assert torch.equal(got_ids, want_ids)
+
+
+def test_costs_of_an_8_bit_block_are_measured(device, monkeypatch):
+    """Calibration runs the 8-bit experts and uploads the bytes of one of their slots."""
+    from sparse_amd import local_policy, ops
+    SparseContext.reset()
+    blk = block(make_mlp_block(QWEN, dtype=torch.bfloat16, seed=14, std=0.05), QWEN, device, weight_format="fp8")
+    sizes, upload = [], ops.expert_upload_async
+    monkeypatch.setattr(ops, "expert_upload_async", lambda d, h, n, s, e: (sizes.append(n), upload(d, h, n, s, e))[1])
+    costs = local_policy.measure_costs(blk, batches=(1, 4, 40), repeats=3)
+    assert all(v >= 0 for v in costs.values()) and costs["next_attention_ms"] > 0
+    assert max(sizes) == blk.slab.expert_bytes == fp8.slot_bytes(QWEN["hidden"], QWEN["inter"])
+    x = make_hidden(4, QWEN["hidden"], torch.bfloat16, seed=15)
+    run(blk, x, device)                       # and leaves the block as it was
