@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
       for (int it = 0; it < NMI; ++it) {
         const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + buf * kSlab + (wave * NMI + it) * 1024);
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(doff[it]), "s"(sb), "s"(dst)
-                     : "memory");
+                     : "memory", "m0");
       }
     };
     fill_scales();
