@@ -421,11 +421,8 @@ class DistributedSparseMoeBlock(nn.Module):
             self._backend = _HipBackend(self)
             self.residency = LayerResidency(self.layer_idx, E, self.top_k, cfg, self._backend, self.metrics,
                                             expert_bytes=self.arena.expert_bytes)
-            if eight:
-                self.slab = fp8.ExpertSlab(self.residency.num_slots, E, H, I, self.device)
-                self.slab.pow2 = self.arena.pow2
-            else:
-                self.slab = ExpertSlab(self.residency.num_slots, E, H, I, self.dtype, self.device)
+            self.slab = (fp8.ExpertSlab(self.residency.num_slots, E, H, I, self.device) if eight
+                         else ExpertSlab(self.residency.num_slots, E, H, I, self.dtype, self.device))
         self._experts_desc = None if eight else ops.make_experts(self.slab.data, self.slab.expert_slot, E, H, I)
         self._cache = self.residency.cache if self.residency is not None else None
         self._current_forward_batch_size = 0

@@ -174,7 +174,7 @@ struct F8Product {
   void* out_s;
   int32_t Ks, Ns, T;
   int32_t dtype;                                    // of topv, gate_s and outputs
-  int32_t pow2;                                     // every weight scale is a power of two
+  int32_t pow2;                                     // tiles may take scales that are powers of two as exponents
   sparse_hip_seglist segs;
 };
 

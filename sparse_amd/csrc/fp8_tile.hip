@@ -13,8 +13,10 @@
 //
 // Scales: the activations' E8M0 bytes of the whole tile are laid out in LDS once, the eight bytes that a
 // lane's eight row tiles need for a slab side by side, and enter the instruction as its own operand.  The
-// weights' fp32 scales multiply the slab's sum on its way into the accumulator, or, where all are powers of two,
-// enter the instruction as exponents (4096 rows of 2048 by 5632 weight rows: 65 -> 57 us).
+// weights' fp32 scales multiply the slab's sum on its way into the accumulator, or, where all those of the tile are
+// powers of two, enter the instruction as exponents (4096 rows of 2048 by 5632 weight rows: 65 -> 57 us).  A tile
+// looks at its scales and chooses by itself: what a row comes out as depends on its own weights' scales alone, as
+// they are at the time of the call, and not on the other matrices of the call.
 //
 // Gate/up ends in the quantiser: a tile's 128 neurons are one run of the intermediate, its largest magnitude is
 // found across the four wavefronts in LDS and 8-bit rows with their scales leave, a quarter of the bytes of fp32
@@ -64,6 +66,12 @@ __device__ __forceinline__ T* uniform_ptr(T* p) {
   return reinterpret_cast<T*>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
+// A power of two that is a normal fp32 number, 2^-126 to 2^127: its exponent is all there is to it.
+__device__ __forceinline__ bool tl_is_exponent(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return (b & 0x807fffffu) == 0 && b - 0x00800000u <= 0x7f000000u - 0x00800000u;
+}
+
 struct TileArgs {
   F8Product p;
   const PfTile* map;       // NULL: dense operands only, the tile comes from the block number
@@ -75,9 +83,8 @@ struct TileArgs {
 };
 
 // F: the 16-bit format of outputs, route weights and gate logits
-// kPow2: every weight scale is a power of two, and enters the instruction as its exponent
 // kNarrow: tiles of 32 rows by 128, three workgroups to a compute unit instead of two (not for gate/up)
-template <typename F, bool kGateUp, bool kPow2, bool kNarrow>
+template <typename F, bool kGateUp, bool kNarrow>
 __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(const TileArgs a) {
   constexpr int NG = kNarrow ? 2 : 4;                         // 16-row groups of weights per wavefront
   constexpr int kRows = kNarrow ? kTlNarrowRows : kPfBM;
@@ -177,7 +184,9 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
 
   // ---- scales to LDS, row factors ------------------------------------------------------
   // Bytes are fetched eight at a time before the first is stored: one by one, each would wait a memory latency.
+  // Every wavefront looks at all weight scales (and stores a quarter of them); returns whether all are exponents.
   auto fill_scales = [&]() __attribute__((always_inline)) {
+    bool odd = false;
     constexpr int kShare = kPfThreads / kRows;    // threads of a row
     const int m = tid / kShare, part = tid % kShare;
     const uint8_t* src = sbase + static_cast<size_t>(source_row(m)) * nk;
@@ -191,7 +200,11 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
       for (int i = 0; i < 8; ++i)
         if (kb0 + kShare * i < nk) dst[(kb0 + kShare * i) * kPfBM] = v[i];
     }
-    for (int i = tid; i < 2 * nk; i += kPfThreads) w[i] = ((i & 1) ? ws1 : ws0)[i >> 1];
+    for (int i = lane; i < 2 * nk; i += 64) {
+      const float v = ((i & 1) ? ws1 : ws0)[i >> 1];
+      if (((i >> 6) & 3) == wave) w[i] = v;
+      odd |= !(kNarrow && (i & 1)) && !tl_is_exponent(v);      // (a narrow tile lies in one 128-row block)
+    }
     // down: factor of each row, the route weight or the sigmoid of the shared expert's gate
     if (!kGateUp && tid < kPfBM) {
       float sc = 1.f;
@@ -202,31 +215,40 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
       }
       s_row[tid] = sc;
     }
+    return !__any(odd);
   };
 
+  // Byte offset of the lane's piece of each copy inside k slab 0: a wavefront copies a quarter of the tile's sub-tiles
+  // of 32 rows (past the last one the offsets repeat the tile's last row and go unused).
+  const int nmi = kNarrow ? 1 : (M + 31) >> 5;
+  uint32_t doff[kNarrow ? 1 : 4];
+#pragma unroll
+  for (int it = 0; it < (kNarrow ? 1 : 4); ++it)
+    doff[it] = source_row((wave * nmi + it) * 8 + l3) * ld + ((chunk0 ^ ((wave * nmi + it) & 1)) << 4);
+  const bool pow2 = fill_scales() && a.p.pow2 != 0;
+
   // The tile's rows are processed in sub-tiles of 32; a segment's last tile is specialised on how many of
-  // them hold rows.
-  auto body = [&](auto nmi_c) {
+  // them hold rows.  kPow2: every weight scale of the tile enters the instruction as its exponent.
+  auto body = [&](auto nmi_c, auto pow2_c) __attribute__((always_inline)) {
     constexpr int NMI = decltype(nmi_c)::value;
+    constexpr bool kPow2 = decltype(pow2_c)::value;
     constexpr int NMT = 2 * NMI;                  // 16-row tiles
     // While slab kt is multiplied, the rows of slab kt+S travel to the LDS buffer slab kt-1 has left and the
     // fragments of slab kt+S to the registers the last row pair has just finished with.  Vector memory retires
     // in order, so what has landed is known by counting.  Slabs past the end refetch the last one.
     constexpr int S = tl_depth(NMI, kNarrow), kSlab = 32 * NMI * kTlRowBytes, kWait = tl_wait(tl_younger(NMI, kNarrow));
-    uint32_t doff[NMI];   // byte offset of lane's piece of copy `it` inside k slab 0
+    uint32_t off[NMI];
 #pragma unroll
-    for (int it = 0; it < NMI; ++it)
-      doff[it] = source_row((wave * NMI + it) * 8 + l3) * ld + ((chunk0 ^ ((wave * NMI + it) & 1)) << 4);
+    for (int it = 0; it < NMI; ++it) off[it] = doff[it];
     auto stage_slab = [&](int slab, int buf) __attribute__((always_inline)) {
       const uint8_t* sb = abase + static_cast<size_t>(slab) * kF8Block;
 #pragma unroll
       for (int it = 0; it < NMI; ++it) {
         const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_base + buf * kSlab + (wave * NMI + it) * 1024);
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(doff[it]), "s"(sb), "s"(dst)
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[it]), "s"(sb), "s"(dst)
                      : "memory", "m0");
       }
     };
-    fill_scales();
     i32x4 wfrag[S][2][NG];   // [stage][k half][16-row group]
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -437,13 +459,17 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
       }
     }
   };
-  if constexpr (kNarrow) body(std::integral_constant<int, 1>{});
-  else switch ((M + 31) >> 5) {
-    case 1: body(std::integral_constant<int, 1>{}); break;
-    case 2: body(std::integral_constant<int, 2>{}); break;
-    case 3: body(std::integral_constant<int, 3>{}); break;
-    default: body(std::integral_constant<int, 4>{}); break;
-  }
+  auto bodies = [&](auto pow2_c) __attribute__((always_inline)) {
+    if constexpr (kNarrow) body(std::integral_constant<int, 1>{}, pow2_c);
+    else switch (nmi) {
+      case 1: body(std::integral_constant<int, 1>{}, pow2_c); break;
+      case 2: body(std::integral_constant<int, 2>{}, pow2_c); break;
+      case 3: body(std::integral_constant<int, 3>{}, pow2_c); break;
+      default: body(std::integral_constant<int, 4>{}, pow2_c); break;
+    }
+  };
+  if (pow2) bodies(std::true_type{});
+  else bodies(std::false_type{});
 }
 
 template <bool kGateUp, bool kNarrow>
@@ -451,14 +477,10 @@ static int launch_tile(const TileArgs& a, int64_t grid, hipStream_t st) {
   SP_REQUIRE(grid < (1ll << 31), "fp8 product: grid too large");
   const int Kmax = a.p.Ks > a.p.Kr ? a.p.Ks : a.p.Kr;
   const unsigned dyn = static_cast<unsigned>(f8_blocks(Kmax)) * kTlScaleBytes;
-#define SP_TILE_LAUNCH(F, P) \
-  hipLaunchKernelGGL((f8_tile_kernel<F, kGateUp, P, kNarrow>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a)
-  if (a.p.dtype == SPARSE_HIP_F16) {
-    if (a.p.pow2) SP_TILE_LAUNCH(Fp16, true); else SP_TILE_LAUNCH(Fp16, false);
-  } else {
-    if (a.p.pow2) SP_TILE_LAUNCH(Bf16, true); else SP_TILE_LAUNCH(Bf16, false);
-  }
-#undef SP_TILE_LAUNCH
+  if (a.p.dtype == SPARSE_HIP_F16)
+    hipLaunchKernelGGL((f8_tile_kernel<Fp16, kGateUp, kNarrow>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
+  else
+    hipLaunchKernelGGL((f8_tile_kernel<Bf16, kGateUp, kNarrow>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
   SP_LAUNCH_CHECK("f8_tile_kernel");
   return SPARSE_HIP_OK;
 }

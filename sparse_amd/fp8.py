@@ -133,8 +133,8 @@ def _check_quantized(values: torch.Tensor, scales: torch.Tensor, name: str = "we
 
 
 def are_pow2(scales: torch.Tensor) -> bool:
-    """Whether every scale is a power of two in fp32's normal range (8-bit products of many rows then take it
-    as an exponent)."""
+    """Whether every scale is a power of two in fp32's normal range.  (Products of many rows take such a scale as an
+    exponent, which they find out by themselves.)"""
     m, _ = torch.frexp(scales)
     return bool(((m == 0.5) & (scales >= 2.0 ** -126)).all())
 
@@ -142,17 +142,21 @@ def are_pow2(scales: torch.Tensor) -> bool:
 class Weight:
     """A matrix ``[rows, cols]`` laid out for the kernels, with its block scales."""
 
-    __slots__ = ("data", "scales", "rows", "cols", "pow2", "desc", "ref")
+    __slots__ = ("data", "scales", "rows", "cols", "desc", "ref")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> None:
         self.data, self.scales, self.rows, self.cols = data, scales, int(rows), int(cols)
-        self.pow2 = are_pow2(scales)
         self.desc = Fp8Matrix(data.data_ptr(), scales.data_ptr(), self.rows, self.cols)
         self.ref = C.byref(self.desc)
 
     @property
     def shape(self) -> Tuple[int, int]:
         return self.rows, self.cols
+
+    @property
+    def pow2(self) -> bool:
+        """Whether every scale is a power of two, as they are now (reads them back)."""
+        return are_pow2(self.scales)
 
     @classmethod
     def from_quantized(cls, values: torch.Tensor, scales: torch.Tensor) -> "Weight":
@@ -199,12 +203,12 @@ def linear(x: Union[torch.Tensor, Rows], weight: Weight, out: Optional[torch.Ten
     lib = _lib.load()
     if rows:
         rc = call_on(index, lib.sparse_hip_fp8_linear, None, src.data_ptr(), x.scales.data_ptr(), dtype_code(dtype), T,
-                     weight.ref, weight.pow2, out.data_ptr(), None)
+                     weight.ref, 1, out.data_ptr(), None)
     else:
         need = lib.sparse_hip_fp8_linear_ws_bytes(T, K)       # 0: the product quantises its rows itself
         ws = src.new_empty((need,), dtype=torch.uint8) if need else None
-        rc = call_on(index, lib.sparse_hip_fp8_linear, src.data_ptr(), None, None, dtype_code(dtype), T, weight.ref,
-                     weight.pow2, out.data_ptr(), _ptr(ws))
+        rc = call_on(index, lib.sparse_hip_fp8_linear, src.data_ptr(), None, None, dtype_code(dtype), T, weight.ref, 1,
+                     out.data_ptr(), _ptr(ws))
     _lib.check(rc, "sparse_hip_fp8_linear")
     return out
 
@@ -247,7 +251,6 @@ class ExpertSlab:
         self.expert_bytes = slot_bytes(hidden, inter)
         self.data = torch.empty((self.num_slots, self.expert_bytes), dtype=torch.uint8, device=device)
         self._refs: dict = {}
-        self.pow2 = False       # whether every scale of the slots in use is a power of two
 
     @classmethod
     def from_quantized(cls, experts: Sequence[Tuple[Quantized, Quantized, Quantized]], device=None) -> "ExpertSlab":
@@ -256,13 +259,19 @@ class ExpertSlab:
         slab = cls(len(experts), len(experts), gate.shape[1], gate.shape[0], device if device is not None else gate.device)
         for e, expert in enumerate(experts):
             pack_expert_into(slab.data[e], expert, slab.hidden, slab.inter)
-        slab.pow2 = are_pow2(torch.cat([s.reshape(-1) for expert in experts for _, s in expert]))
         return slab
 
     @classmethod
     def quantize(cls, experts: Sequence[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]], device=None) -> "ExpertSlab":
         """The same from 16- or 32-bit (gate, up, down) weights."""
         return cls.from_quantized([tuple(quantize_weight(w) for w in triple) for triple in experts], device)
+
+    @property
+    def pow2(self) -> bool:
+        """Whether every scale of every slot is a power of two, as they are now (reads them back)."""
+        at = 2 * self.inter * padded(self.hidden) + self.hidden * padded(self.inter)
+        size = 4 * 3 * blocks(self.hidden) * blocks(self.inter)
+        return are_pow2(self.data[:, at:at + size].contiguous().view(torch.float32))
 
     def slot_ptr(self, slot: int) -> int:
         return self.data.data_ptr() + int(slot) * self.expert_bytes
@@ -285,11 +294,8 @@ class HostExpertArena(weights.HostExpertArena):
                  pin: bool = True) -> None:
         self.hidden, self.inter, self.dtype = int(hidden), int(inter), torch.uint8
         self._allocate(len(experts), slot_bytes(hidden, inter), torch.uint8, pin)
-        pow2 = []
         for e, expert in enumerate(experts):
             pack_expert_into(self.rows[e], expert, hidden, inter)
-            pow2.append(all(are_pow2(s) for _, s in expert))
-        self.pow2 = all(pow2)
 
 
 def module_weight(linear_mod, device=None) -> Quantized:
@@ -345,14 +351,13 @@ def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Perm
     else:
         _need(parts, "parts", dtype, (T * K, H))
     gate = up = down = None
-    Is, pow2 = 0, experts.pow2
+    Is = 0
     if shared is not None:
         gate, up, down = shared
         Is = down.cols
         for m, want, name in ((gate, (Is, H), "gate_proj"), (up, (Is, H), "up_proj"), (down, (H, Is), "down_proj")):
             if (m.rows, m.cols) != want:
                 raise ValueError(f"shared {name} must be {want}, got {m.shape}")
-            pow2 = pow2 and m.pow2
         _same_device(index, gate.data, up.data, down.data)
         gate, up, down = gate.ref, up.ref, down.ref
         if shared_gate is not None:
@@ -376,6 +381,6 @@ def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Perm
     _same_device(index, topv, perm.perm, experts.data, parts, shared_gate, shared_out, ws)
     rc = call_on(index, lib.sparse_hip_fp8_moe_ffn, experts.descriptor(dtype), x.data_ptr(), topv.data_ptr(),
                  perm.perm.data_ptr(), perm.seg_offsets.data_ptr(), C.byref(segs), T, K, parts.data_ptr(), gate, up, down,
-                 _ptr(shared_gate), pow2, _ptr(shared_out), ws.data_ptr())
+                 _ptr(shared_gate), 1, _ptr(shared_out), ws.data_ptr())
     _lib.check(rc, "sparse_hip_fp8_moe_ffn")
     return parts, shared_out

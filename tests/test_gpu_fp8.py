@@ -477,3 +477,48 @@ def test_arguments_that_are_refused(device):
             fp8.linear(x, w, out)
     with pytest.raises(ValueError):
         fp8.quantize(x.t())
+
+
+@pytest.mark.parametrize("T", [4, 70])
+def test_replaced_expert_keeps_its_scales(path, device, T):
+    """An expert of arbitrary scales packed over one whose scales were powers of two."""
+    c = make_case(T, 192, 4, 128, 2, 0, False, torch.bfloat16, seed=31, pow2=True)
+    d = on_gpu(c, device)
+    new = make_case(T, 192, 4, 128, 2, 0, False, torch.bfloat16, seed=77)["ex"][2]
+    fp8.pack_expert_into(d["slab"].data[1], tuple((q.to(device), s.to(device)) for q, s in new), 192, 128)
+    c["ex"][1] = new
+    parts, _ = fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"])
+    want, bound, _, _ = oracle(c, path)
+    within(parts, want, bound, torch.bfloat16)
+    assert not d["slab"].pow2
+
+
+@pytest.mark.parametrize("T", [4, 70])
+def test_weight_with_changed_scales(path, device, T):
+    """Scales that are written over after the weight was made count as they are now."""
+    x, (q, s) = rand_rows(T, 300, torch.bfloat16), rand_weight(200, 300, pow2=True)
+    w = fp8.Weight.from_quantized(q.to(device), s.to(device))
+    s = s * (torch.rand(s.shape, generator=torch.Generator().manual_seed(2)) + 0.25)
+    w.scales.copy_(s)
+    want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s), grouped(T))
+    within(fp8.linear(x.to(device), w), want, bound, torch.bfloat16)
+    assert not w.pow2
+
+
+@pytest.mark.parametrize("T", [6, 70, 400])
+def test_routed_rows_do_not_depend_on_what_else_is_in_the_call(path, device, T):
+    """Experts with power-of-two scales beside others and beside a shared expert without, all in one call or each apart."""
+    case = (T, 1024, 4, 704, 2, 320, True, torch.float16)
+    c, odd = make_case(*case, seed=41, pow2=True), make_case(*case, seed=41)
+    c["sh"], c["ex"][3] = odd["sh"], odd["ex"][3]
+    c["x"] = (c["x"] * torch.exp(3 * torch.randn(1024, generator=torch.Generator().manual_seed(3))).clamp(max=200)).half()
+    d = on_gpu(c, device)
+    parts, shared = fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"], shared=d["sh"], shared_gate=d["sg"])
+    apart = torch.empty_like(parts)
+    for e in range(4):
+        fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"], segs=ops.seglist_host([e]), parts=apart)
+    assert torch.equal(apart, parts)
+    pure = dict(c, ex=[t if i < 3 else c["ex"][0] for i, t in enumerate(c["ex"])], sh=None)
+    alone, _ = fp8.moe_ffn(on_gpu(pure, device)["slab"], d["x"], d["topv"], d["perm"])
+    end = int(d["perm"].seg_offsets[3])
+    assert torch.equal(alone[:end], parts[:end])

@@ -201,6 +201,33 @@ def test_deepseek_v3_model_with_swapped_blocks(device):
     assert torch.equal(got_ids, want_ids)
 
 
+@pytest.mark.parametrize("T", [8, 120, 500])
+def test_offloaded_block_gives_the_resident_bits_beside_a_shared_expert_of_other_scales(device, T):
+    """Routed experts quantised at load (scales that are powers of two), a shared expert with a checkpoint's own ones:
+    the routed rows are the same whether they run in the shared expert's call or in their own."""
+    shape = dict(QWEN, hidden=1024, inter=704)
+    SparseContext.reset()
+    mlp = make_mlp_block(shape, dtype=torch.float16, seed=13, std=0.05)
+
+    def eight(m):
+        q, s = fp8.quantize_weight(m.weight.float())
+        return NS(weight=q, weight_scale_inv=s * (torch.rand(s.shape, generator=torch.Generator().manual_seed(s.numel())) + 0.5))
+
+    sh = mlp.shared_expert
+    mixed = NS(gate=mlp.gate, experts=mlp.experts, shared_expert_gate=mlp.shared_expert_gate,
+               shared_expert=NS(gate_proj=eight(sh.gate_proj), up_proj=eight(sh.up_proj), down_proj=eight(sh.down_proj)))
+    a = block(mixed, shape, device, torch.float16, weight_format="fp8")
+    b = block(mixed, shape, device, torch.float16, weight_format="fp8", expert_offload="cpu", expert_cache=3)
+    assert a.slab.pow2 and not a.shared_weights[0].pow2
+    for call in range(2):
+        x = make_hidden(T, shape["hidden"], torch.float16, seed=50 + call)
+        x = (x * torch.exp(3 * torch.randn(1024, generator=torch.Generator().manual_seed(3))).clamp(max=200)).half()
+        SparseContext.begin_runtime_call(call)
+        want, _ = run(a, x, device)
+        got, _ = run(b, x, device)
+        assert torch.equal(got, want)
+
+
 def test_costs_of_an_8_bit_block_are_measured(device, monkeypatch):
     """Calibration runs the 8-bit experts and uploads the bytes of one of their slots."""
     from sparse_amd import local_policy, ops
