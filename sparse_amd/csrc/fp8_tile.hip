@@ -49,8 +49,16 @@ constexpr int tl_younger(int nmi, bool narrow) {
   const int loads = narrow ? 4 : 8;
   return loads + (tl_depth(nmi, narrow) - 1) * (nmi + loads);
 }
+// The last slabs, those behind the loop, request nothing (nobody would use it, and the compiler drops a load without a
+// user, so that a count could not rely on it).  In number j of them the next slab's copies are followed by its own
+// fragment loads and by copies and loads of the S - 2 - j slabs behind it.
+constexpr int tl_younger_tail(int nmi, bool narrow, int j) {
+  const int loads = narrow ? 4 : 8, behind = tl_depth(nmi, narrow) - 2 - j;
+  return loads + behind * (nmi + loads);
+}
 constexpr int tl_wait(int vmcnt) { return 0x0F70 | (vmcnt & 15) | ((vmcnt >> 4) << 14); }
 static_assert(tl_younger(4, false) == 20 && tl_wait(20) == kWaitVmcnt20, "the count of the 16-bit kernels");
+static_assert(tl_younger_tail(2, false, -1) == tl_younger(2, false) && tl_younger_tail(1, true, 4) == 4, "one rule for both");
 static_assert(tl_younger(2, false) < 64 && tl_younger(1, false) < 64 && tl_younger(1, true) < 64, "six bits");
 static_assert((tl_depth(1, false) + 1) * 32 * kTlRowBytes <= kTlRing && (tl_depth(2, false) + 1) * 64 * kTlRowBytes <= kTlRing, "rings fit");
 constexpr int kTlNarrowRows = 32;
@@ -235,7 +243,8 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
     constexpr int NMT = 2 * NMI;                  // 16-row tiles
     // While slab kt is multiplied, the rows of slab kt+S travel to the LDS buffer slab kt-1 has left and the
     // fragments of slab kt+S to the registers the last row pair has just finished with.  Vector memory retires
-    // in order, so what has landed is known by counting.  Slabs past the end refetch the last one.
+    // in order, so what has landed is known by counting.  Slabs past the end refetch the last one; the up to S - 1
+    // slabs behind the loop find everything requested.
     constexpr int S = tl_depth(NMI, kNarrow), kSlab = 32 * NMI * kTlRowBytes, kWait = tl_wait(tl_younger(NMI, kNarrow));
     uint32_t off[NMI];
 #pragma unroll
@@ -274,8 +283,9 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
     const int fsw = ((fr >> 1) & 7) ^ ((fr & 1) << 2);
     const int a_row = fr * kTlRowBytes, a_x = (fq ^ fsw) << 4;
     int cur = 0, ahead = S;   // buffer of slab kt, buffer of slab kt+S
-    auto slab = [&](auto stage_c, int kt) {
-      constexpr int st = decltype(stage_c)::value;
+    // tail_c: -1 in the loop, else the number of the slab behind it (whose stage has the same number)
+    auto slab = [&](auto stage_c, auto tail_c, int kt) {
+      constexpr int st = decltype(stage_c)::value, kTail = decltype(tail_c)::value;
       constexpr int NP = NMT / 2;                 // pairs of 16-row tiles
       const int kts = min(kt + S, nk - 1);
       const uint8_t* la = lds + cur * kSlab + a_row;
@@ -283,7 +293,7 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
       const float2 sw = *reinterpret_cast<const float2*>(s_scales + nk * kPfBM + kt * 8);
       const float sw0 = kGateUp || kNarrow || wave < 2 ? sw.x : sw.y, sw1 = kGateUp ? sw.y : sw0;
       i32x4 fa[2][2][2];   // [parity][tile of the pair][half]
-      if (NP == 1) {       // the copies go first, so that every height issues vector memory in the counted order
+      if (NP == 1 && kTail < 0) {       // the copies go first, so that every height issues vector memory in the counted order
         stage_slab(kts, ahead);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -317,7 +327,7 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
             constexpr int g = decltype(g_c)::value;
             mul(std::integral_constant<int, 2 * pr>{}, g_c, fa[pr & 1][0]);
             mul(std::integral_constant<int, 2 * pr + 1>{}, g_c, fa[pr & 1][1]);
-            if constexpr (pr == NP - 1) {       // last user of group g's fragments: request those of slab kt+S
+            if constexpr (pr == NP - 1 && kTail < 0) {       // last user of group g's fragments: request those of slab kt+S
               __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
               for (int h = 0; h < 2; ++h) wfrag[st][h][g] = wload(g, kts, h);
@@ -331,7 +341,7 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
             group(std::integral_constant<int, 3>{});
           }
           __builtin_amdgcn_sched_barrier(0);
-          if (NP > 1 && pr == 0) {   // the copies of slab kt+S go out once the matrix pipe has work
+          if (NP > 1 && pr == 0 && kTail < 0) {   // the copies of slab kt+S go out once the matrix pipe has work
             stage_slab(kts, ahead);
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -341,28 +351,32 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
       pair(std::integral_constant<int, 1>{});
       pair(std::integral_constant<int, 2>{});
       pair(std::integral_constant<int, 3>{});
-      __builtin_amdgcn_s_waitcnt(kWait);
+      __builtin_amdgcn_s_waitcnt(kTail < 0 ? kWait : tl_wait(tl_younger_tail(NMI, kNarrow, kTail < 0 ? 0 : kTail)));
       __syncthreads();
       cur = (cur == S) ? 0 : cur + 1;
       ahead = (ahead == S) ? 0 : ahead + 1;
     };
     int kt = 0;
+    auto turn = [&](auto st_c) __attribute__((always_inline)) {
+      if constexpr (decltype(st_c)::value < S) slab(st_c, std::integral_constant<int, -1>{}, kt + decltype(st_c)::value);
+    };
     for (; kt + S <= nk; kt += S) {
-      slab(std::integral_constant<int, 0>{}, kt);
-      slab(std::integral_constant<int, 1>{}, kt + 1);
-      if constexpr (S > 2) slab(std::integral_constant<int, 2>{}, kt + 2);
-      if constexpr (S > 3) slab(std::integral_constant<int, 3>{}, kt + 3);
-      if constexpr (S > 4) slab(std::integral_constant<int, 4>{}, kt + 4);
-      if constexpr (S > 5) slab(std::integral_constant<int, 5>{}, kt + 5);
+      turn(std::integral_constant<int, 0>{});
+      turn(std::integral_constant<int, 1>{});
+      turn(std::integral_constant<int, 2>{});
+      turn(std::integral_constant<int, 3>{});
+      turn(std::integral_constant<int, 4>{});
+      turn(std::integral_constant<int, 5>{});
     }
-    if (kt < nk) slab(std::integral_constant<int, 0>{}, kt);
-    if (S > 2 && kt + 1 < nk) slab(std::integral_constant<int, 1>{}, kt + 1);
-    if constexpr (S > 3)
-      if (kt + 2 < nk) slab(std::integral_constant<int, 2>{}, kt + 2);
-    if constexpr (S > 4)
-      if (kt + 3 < nk) slab(std::integral_constant<int, 3>{}, kt + 3);
-    if constexpr (S > 5)
-      if (kt + 4 < nk) slab(std::integral_constant<int, 4>{}, kt + 4);
+    auto tail = [&](auto st_c) __attribute__((always_inline)) {
+      if constexpr (decltype(st_c)::value < S - 1)
+        if (kt + decltype(st_c)::value < nk) slab(st_c, st_c, kt + decltype(st_c)::value);
+    };
+    tail(std::integral_constant<int, 0>{});
+    tail(std::integral_constant<int, 1>{});
+    tail(std::integral_constant<int, 2>{});
+    tail(std::integral_constant<int, 3>{});
+    tail(std::integral_constant<int, 4>{});
     __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);  // no copy may land in LDS after the epilogue starts to reuse it
     __syncthreads();
 
