@@ -366,7 +366,7 @@ class DistributedSparseMoeBlock(nn.Module):
             if self.topk_group >= self.n_group:
                 self.n_group = self.topk_group = 1          # every group kept: plain top-k
         self.experts_kind, expert_weights = extract_experts(mlp_block.experts)
-        if self.weight_format != "fp8" and any(w.dtype == fp8.E4M3 for w in expert_weights[0]):
+        if self.weight_format != "fp8" and any(w.dtype == fp8.E4M3 for triple in expert_weights for w in triple):
             raise ValueError("8-bit expert weights need weight_format='fp8'")
         self.num_experts = int(num_experts) if num_experts is not None else len(expert_weights)
         if self.num_experts != len(expert_weights) or self.gate_weight.shape[0] != self.num_experts:

@@ -266,3 +266,18 @@ def test_native_block_refuses_an_8_bit_shared_expert():
     shared.down_proj.weight = torch.nn.Parameter(shared.down_proj.weight.detach().to(torch.float8_e4m3fn), requires_grad=False)
     with pytest.raises(ValueError, match="weight_format='fp8'"):
         DistributedSparseMoeBlock(0, mlp, None, DistEnv(0, 1, 0, torch.device("cpu")), num_experts=8, top_k=2, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("expert,matrix", [(0, "gate_proj"), (3, "up_proj"), (7, "down_proj")])
+def test_native_block_refuses_one_8_bit_expert_among_others(expert, matrix):
+    """8-bit values without their scales would be taken for the weights themselves."""
+    from sparse_amd.block import DistributedSparseMoeBlock
+    from sparse_amd.context import DistEnv, SparseContext
+    from sparse_amd.synthetic import make_mlp_block
+
+    SparseContext.reset()
+    mlp = make_mlp_block(dict(family="deepseek_shared", hidden=64, num_experts=8, inter=64, shared_inter=64), dtype=torch.bfloat16)
+    m = getattr(mlp.experts[expert], matrix)
+    m.weight = torch.nn.Parameter(m.weight.detach().to(torch.float8_e4m3fn), requires_grad=False)
+    with pytest.raises(ValueError, match="weight_format='fp8'"):
+        DistributedSparseMoeBlock(0, mlp, None, DistEnv(0, 1, 0, torch.device("cpu")), num_experts=8, top_k=2, dtype=torch.bfloat16)
