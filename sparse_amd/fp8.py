@@ -140,14 +140,32 @@ def are_pow2(scales: torch.Tensor) -> bool:
 
 
 class Weight:
-    """A matrix ``[rows, cols]`` laid out for the kernels, with its block scales."""
+    """A matrix ``[rows, cols]`` laid out for the kernels (``data``, bytes in ``tile_values``' order), with its block
+    ``scales``.  Both may be written into; they cannot be exchanged for other tensors, whose place the kernels would
+    not know: make another ``Weight``, on another device too."""
 
-    __slots__ = ("data", "scales", "rows", "cols", "desc", "ref")
+    __slots__ = ("_data", "_scales", "rows", "cols", "desc", "ref")
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> None:
-        self.data, self.scales, self.rows, self.cols = data, scales, int(rows), int(cols)
+        self._data, self._scales, self.rows, self.cols = data, scales, int(rows), int(cols)
+        size = -(-self.rows // 16) * 16 * padded(self.cols)
+        if data.dtype != torch.uint8 or data.numel() != size or not data.is_contiguous():
+            raise ValueError(f"a [{rows}, {cols}] weight is {size} contiguous bytes, got {tuple(data.shape)} {data.dtype}")
+        want = (blocks(self.rows), blocks(self.cols))
+        if scales.dtype != torch.float32 or tuple(scales.shape) != want or not scales.is_contiguous():
+            raise ValueError(f"weight scales must be {want} contiguous float32, got {tuple(scales.shape)} {scales.dtype}")
+        if data.device != scales.device:
+            raise ValueError("weight values and scales are on different devices")
         self.desc = Fp8Matrix(data.data_ptr(), scales.data_ptr(), self.rows, self.cols)
         self.ref = C.byref(self.desc)
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -199,7 +217,7 @@ def linear(x: Union[torch.Tensor, Rows], weight: Weight, out: Optional[torch.Ten
     else:
         _need(out, "out", dtype, (T, weight.rows))
         _same_device(index, out)
-    _same_device(index, weight.data)
+    _same_device(index, weight._data)
     lib = _lib.load()
     if rows:
         rc = call_on(index, lib.sparse_hip_fp8_linear, None, src.data_ptr(), x.scales.data_ptr(), dtype_code(dtype), T,
@@ -241,7 +259,7 @@ def pack_expert_into(dst: torch.Tensor, expert: Tuple[Quantized, Quantized, Quan
 
 class ExpertSlab:
     """8-bit experts of one layer in HBM, one slot each.  Host segment lists name the slots of their experts;
-    with a device list expert e is in slot e."""
+    with a device list expert e is in slot e.  ``data`` may be written into, not exchanged for another tensor."""
 
     def __init__(self, num_slots: int, num_experts: int, hidden: int, inter: int, device) -> None:
         if hidden % 64 or inter % 64 or hidden <= 0 or inter <= 0:
@@ -249,7 +267,7 @@ class ExpertSlab:
         self.hidden, self.inter = int(hidden), int(inter)
         self.num_slots, self.num_experts = int(num_slots), int(num_experts)
         self.expert_bytes = slot_bytes(hidden, inter)
-        self.data = torch.empty((self.num_slots, self.expert_bytes), dtype=torch.uint8, device=device)
+        self._data = torch.empty((self.num_slots, self.expert_bytes), dtype=torch.uint8, device=device)
         self._refs: dict = {}
 
     @classmethod
@@ -265,6 +283,10 @@ class ExpertSlab:
     def quantize(cls, experts: Sequence[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]], device=None) -> "ExpertSlab":
         """The same from 16- or 32-bit (gate, up, down) weights."""
         return cls.from_quantized([tuple(quantize_weight(w) for w in triple) for triple in experts], device)
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
 
     @property
     def pow2(self) -> bool:

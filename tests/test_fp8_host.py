@@ -281,3 +281,25 @@ def test_native_block_refuses_one_8_bit_expert_among_others(expert, matrix):
     m.weight = torch.nn.Parameter(m.weight.detach().to(torch.float8_e4m3fn), requires_grad=False)
     with pytest.raises(ValueError, match="weight_format='fp8'"):
         DistributedSparseMoeBlock(0, mlp, None, DistEnv(0, 1, 0, torch.device("cpu")), num_experts=8, top_k=2, dtype=torch.bfloat16)
+
+
+def test_weights_and_slabs_stay_where_their_descriptors_say():
+    """The kernels go by addresses taken when a weight or slab was made: its tensors cannot be exchanged afterwards."""
+    w = fp8.Weight.quantize(torch.randn(130, 257))
+    assert w.desc.values_dev == w.data.data_ptr() and w.desc.scales_dev == w.scales.data_ptr()
+    for name in ("data", "scales"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, getattr(w, name).clone())
+    slab = fp8.ExpertSlab(2, 2, 128, 64, "cpu")
+    with pytest.raises(AttributeError):
+        slab.data = slab.data.clone()
+
+
+def test_weights_are_made_of_what_their_shape_needs():
+    w = fp8.Weight.quantize(torch.randn(130, 257))
+    fp8.Weight(w.data, w.scales, 130, 257)
+    for data, scales, rows, cols in ((w.data[:-1], w.scales, 130, 257), (w.data, w.scales[:1], 130, 257),
+                                     (w.data, w.scales.double(), 130, 257), (w.data.view(fp8.E4M3), w.scales, 130, 257),
+                                     (w.data, w.scales, 145, 257), (w.data, w.scales, 130, 385), (w.data, w.scales.t(), 130, 257)):
+        with pytest.raises(ValueError):
+            fp8.Weight(data, scales, rows, cols)
