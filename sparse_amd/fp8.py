@@ -193,6 +193,12 @@ class Weight:
         return (q * s).to(dtype)
 
 
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    p, q = a.data_ptr(), b.data_ptr()
+    return p < q + b.numel() * b.element_size() and q < p + a.numel() * a.element_size()
+
+
 def linear(x: Union[torch.Tensor, Rows], weight: Weight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x W^T`` with ``x [T, K]`` (bf16 or fp16) quantised inside the call, or given as ``Rows`` of such an x:
     ``[T, N]`` in x's dtype, accumulated in fp32 and rounded once."""
@@ -217,7 +223,9 @@ def linear(x: Union[torch.Tensor, Rows], weight: Weight, out: Optional[torch.Ten
     else:
         _need(out, "out", dtype, (T, weight.rows))
         _same_device(index, out)
-    _same_device(index, weight._data)
+        if overlap(out, src):
+            raise ValueError("out overlaps x, which is read while out is written")
+    _same_device(index, weight._data, x.scales if rows else None)
     lib = _lib.load()
     if rows:
         rc = call_on(index, lib.sparse_hip_fp8_linear, None, src.data_ptr(), x.scales.data_ptr(), dtype_code(dtype), T,

@@ -303,3 +303,10 @@ def test_weights_are_made_of_what_their_shape_needs():
                                      (w.data, w.scales, 145, 257), (w.data, w.scales, 130, 385), (w.data, w.scales.t(), 130, 257)):
         with pytest.raises(ValueError):
             fp8.Weight(data, scales, rows, cols)
+
+
+def test_overlap_is_what_shares_bytes():
+    t = torch.zeros(64, dtype=torch.bfloat16)
+    assert fp8.overlap(t, t) and fp8.overlap(t[:32], t[31:]) and fp8.overlap(t[31:], t[:32]) and fp8.overlap(t[4:8], t)
+    assert not fp8.overlap(t[:32], t[32:]) and not fp8.overlap(t[32:], t[:32]) and not fp8.overlap(t[:0], t[:0])
+    assert not fp8.overlap(t, t.clone())

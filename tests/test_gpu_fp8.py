@@ -522,3 +522,16 @@ def test_routed_rows_do_not_depend_on_what_else_is_in_the_call(path, device, T):
     alone, _ = fp8.moe_ffn(on_gpu(pure, device)["slab"], d["x"], d["topv"], d["perm"])
     end = int(d["perm"].seg_offsets[3])
     assert torch.equal(alone[:end], parts[:end])
+
+
+@pytest.mark.parametrize("T", [1, 2, 5])
+def test_linear_into_its_own_rows_is_refused(device, T):
+    """Workgroups read all of a row while others already write theirs."""
+    q, s = rand_weight(256, 256)
+    w = fp8.Weight.from_quantized(q.to(device), s.to(device))
+    buf = torch.zeros(2 * T, 256, dtype=torch.bfloat16, device=device)
+    buf[:T] = rand_rows(T, 256, torch.bfloat16).to(device)
+    for out in (buf[:T], buf.view(-1)[128:128 + T * 256].view(T, 256), buf.view(-1)[T * 256 - 1:2 * T * 256 - 1].view(T, 256)):
+        with pytest.raises(ValueError, match="overlaps"):
+            fp8.linear(buf[:T], w, out)
+    assert torch.equal(fp8.linear(buf[:T], w, buf[T:]), fp8.linear(buf[:T].clone(), w))
