@@ -433,11 +433,11 @@ int sparse_hip_combine_split(const void* parts_dev, const int32_t* inv_perm_dev,
  *           two largest; the topk_group best stay (ties to the lower group), the others are never chosen
  *   topi = the K largest r of the groups that stay, descending, ties to the lower id
  *   topv = p[topi], divided by max(their sum, 1e-20) if renorm, times `scale`
- * Scores and ranking are computed in 64 bits, topv is rounded once to `out_dtype`.  A row of logits that
+ * Scores and ranking are those of 64 bits, topv is rounded to fp32 and from there to `out_dtype`.  A row of logits that
  * are all -inf scores 0 throughout; NaN scores rank last and come out as NaN weights, ids are always
  * distinct and in range.  logits [T,E] in `logits_dtype`, bias [E] fp32, topv [T,K], topi [T,K].
  * E <= SPARSE_HIP_MAX_EXPERTS, K <= SPARSE_HIP_MAX_TOPK, n_group <= 64 divides E,
- * K <= topk_group * E / n_group.  T == 0 does nothing.
+ * K <= topk_group * E / n_group, T <= 2^28.  T == 0 does nothing.
  */
 int sparse_hip_gate_select(const void* logits_dev, int logits_dtype, const float* bias_dev, int T, int E,
                            int K, int score, int n_group, int topk_group, int group_score, int renorm,

@@ -165,7 +165,7 @@ int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_
              "fp8_linear: weight is [%d,%d], must be in [1,%d] x [1,%d]", weight->rows, weight->cols, kF8MaxOut, kF8MaxDim);
   int rc = check_matrix("fp8_linear", "weight", weight, weight->rows, weight->cols);
   if (rc != SPARSE_HIP_OK) return rc;
-  SP_REQUIRE(T >= 0, "fp8_linear: T=%d", T);
+  SP_REQUIRE(T >= 0 && T <= kF8MaxRows, "fp8_linear: T=%d outside [0,%d]", T, static_cast<int>(kF8MaxRows));
   if (T == 0) return SPARSE_HIP_OK;
   SP_REQUIRE((x_dev != nullptr) != (xq_dev != nullptr), "fp8_linear: give x or its 8-bit rows");
   SP_REQUIRE(out_dev != nullptr, "fp8_linear: NULL output");

@@ -23,6 +23,7 @@ namespace sparse {
 constexpr int kSelWaves = 4;
 static_assert(SPARSE_HIP_MAX_EXPERTS <= 256, "four experts per lane at most");
 constexpr int kSelMaxGroups = 64;
+constexpr int kSelMaxTokens = 1 << 28;       // token numbers of the last workgroup stay within 32 bits
 
 struct SelectArgs {
   const void* logits;
@@ -277,7 +278,7 @@ extern "C" int sparse_hip_gate_select(const void* logits_dev, int logits_dtype, 
   SP_REQUIRE(topk_group >= 1 && topk_group <= n_group, "gate_select: topk_group=%d outside [1,%d]", topk_group, n_group);
   SP_REQUIRE(K <= topk_group * (E / n_group), "gate_select: K=%d exceeds the %d experts of %d groups", K,
              topk_group * (E / n_group), topk_group);
-  SP_REQUIRE(T >= 0, "gate_select: T=%d", T);
+  SP_REQUIRE(T >= 0 && T <= kSelMaxTokens, "gate_select: T=%d outside [0,%d]", T, kSelMaxTokens);
   if (T == 0) return SPARSE_HIP_OK;
   SP_REQUIRE(logits_dev && topv_dev && topi_dev, "gate_select: NULL pointer");
   const SelectArgs a = {logits_dev, bias_dev, topv_dev, topi_dev, T, E, K, score == SPARSE_HIP_SCORE_SIGMOID,

@@ -156,6 +156,8 @@ def gate_select(logits: torch.Tensor, k: int, score: str = "softmax", bias: Opti
     k = int(k)
     if k < 1:
         raise ValueError(f"k must be at least 1, got {k}")
+    if T > 1 << 28:
+        raise ValueError(f"at most 2^28 tokens are routed in a call, got {T}")
     odt = out_dtype or logits.dtype
     index = logits.get_device()
     if bias is not None:

@@ -310,3 +310,12 @@ def test_overlap_is_what_shares_bytes():
     assert fp8.overlap(t, t) and fp8.overlap(t[:32], t[31:]) and fp8.overlap(t[31:], t[:32]) and fp8.overlap(t[4:8], t)
     assert not fp8.overlap(t[:32], t[32:]) and not fp8.overlap(t[32:], t[:32]) and not fp8.overlap(t[:0], t[:0])
     assert not fp8.overlap(t, t.clone())
+
+
+def test_sizes_that_32_bit_row_numbers_do_not_reach_are_refused():
+    lib = _lib.load()
+    P = 4096
+    m = _lib.Fp8Matrix(P, P, 32, 64)
+    for T in ((1 << 28) + 1, (1 << 31) - 1):
+        refused(lib.sparse_hip_fp8_linear(None, P, P, 1, T, C.byref(m), 0, P, None, None), f"T={T}")
+        refused(lib.sparse_hip_gate_select(P, 0, None, T, 1, 1, 0, 1, 1, 0, 0, 1.0, 0, P, P, None), f"T={T}")
