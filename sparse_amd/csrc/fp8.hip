@@ -241,6 +241,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
     SP_REQUIRE(aligned16(parts_dev), "%s: parts must be 16-byte aligned", fn);
     if (segs->eids_dev != nullptr) {
       SP_REQUIRE(segs->count_dev != nullptr, "%s: a device segment list needs a count", fn);
+      SP_REQUIRE(segs->n <= E, "%s: a device segment list of up to %d, there are %d experts", fn, segs->n, E);
     } else {
       bool seen[SPARSE_HIP_MAX_EXPERTS] = {};     // (the workspace has room for each segment's tiles once)
       for (int i = 0; i < segs->n; ++i) {

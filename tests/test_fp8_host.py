@@ -319,3 +319,12 @@ def test_sizes_that_32_bit_row_numbers_do_not_reach_are_refused():
     for T in ((1 << 28) + 1, (1 << 31) - 1):
         refused(lib.sparse_hip_fp8_linear(None, P, P, 1, T, C.byref(m), 0, P, None, None), f"T={T}")
         refused(lib.sparse_hip_gate_select(P, 0, None, T, 1, 1, 0, 1, 1, 0, 0, 1.0, 0, P, P, None), f"T={T}")
+
+
+def test_device_list_longer_than_the_experts_is_refused():
+    """The kernels read as many entries as it says before they know how many count."""
+    s = _lib.SegList()
+    s.n, s.eids_dev, s.count_dev = 5, 4096, 4096
+    ex = _lib.Experts(4096, fp8.slot_bytes(128, 64), None, 4, 128, 64, 1)
+    refused(_lib.load().sparse_hip_fp8_moe_ffn(C.byref(ex), 4096, 4096, 4096, 4096, C.byref(s), 3, 2, 4096, None, None, None, None, 0,
+                                               None, 4096, None), "4 experts")
