@@ -112,13 +112,15 @@ def product(x, w, grouped):
 
 def swiglu(x, gate, up, down, grouped, grouped_down):
     """SwiGLU of (already quantised) rows on (values, scales) weights, with the bound of an fp32 implementation.
+    Gate and up are products added in fp32 whatever ``grouped`` says: the result is rounded to 8 bits next, and no kernel
+    may let the matrix instruction's cut-off decide on which side of a border it falls.
 
     An error of h moves a quantised value only where a rounding border lies within it; how far is found by
     rounding both ends of the interval.  SiLU's slope is at most 1.1; a hardware exp2 and reciprocal are
     good to 2^-20 here.  What a moved value does to the products beside it in its group of eight is at most
     one unit of the cut-off for each of the eight."""
-    g, eg = product(x, gate, grouped)
-    u, eu = product(x, up, grouped)
+    g, eg = product(x, gate, False)
+    u, eu = product(x, up, False)
     sg = g * torch.sigmoid(g)
     h = sg * u
     d = 1.1 * eg * u.abs() + sg.abs() * eu + 1.1 * eg * eu + 2.0 ** -20 * h.abs()
@@ -226,12 +228,11 @@ def cut_bound(v, w):
 
 
 def swiglu_formula(x, gate, up, down):
-    """SwiGLU of (already quantised) rows as it is defined, its sums exact, and how far the tile kernels may be from
-    that: their fp32 steps, the cut-off in every product, and 8-bit roundings of the intermediate that fall to the
-    other side of a border because of both."""
+    """SwiGLU of (already quantised) rows as it is defined, its sums exact, and how far the kernels may be from that:
+    their fp32 steps, 8-bit roundings of the intermediate that fall to the other side of a border because of them, and
+    the cut-off in the down projection."""
     g, eg = product(x, gate, False)
     u, eu = product(x, up, False)
-    eg, eu = eg + cut_bound(x, gate), eu + cut_bound(x, up)
     sg = g * torch.sigmoid(g)
     h = sg * u
     d = 1.1 * eg * u.abs() + sg.abs() * eu + 1.1 * eg * eu + 2.0 ** -20 * h.abs()

@@ -35,6 +35,7 @@ SOURCES = [
     "fp8_quantize.hip",
     "fp8_few.hip",
     "fp8_rows.hip",
+    "fp8_gateup.hip",
     "fp8_tile.hip",
     "rs_predict.hip",
     "layout.hip",
@@ -58,6 +59,7 @@ HIP_FLAGS = [
 # uses scratch memory is refused.
 NO_SCRATCH = {"swiglu_prefill.hip": ("prefill_ffn_kernel",),
               "swiglu_prefill_merged.hip": ("prefill_merged_kernel",),
+              "fp8_gateup.hip": ("f8_gateup_kernel",),
               "fp8_tile.hip": ("f8_tile_kernel",)}
 RESOURCE_REMARKS = "-Rpass-analysis=kernel-resource-usage"
 

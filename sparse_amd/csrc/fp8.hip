@@ -21,10 +21,10 @@ constexpr int kF8StreamRows = 1 << 20;      // the streaming kernel's grid has a
 //   linear  2048 x 5632: 32 rows 10.4 / 11.2 us, 64 rows 13.3 / 11.5;  4096 x 4096: 48 rows 14.8 / 15.4, 64 rows 17.1 / 15.4
 //           1000 x 1418: 192 rows 9.2 / 9.7, 333 rows 11.9 / 10.2;  512 x 1024: 192 rows 7.3 / 7.6, 333 rows 8.6 / 7.7
 //           5632 x 2048: 64 rows 12.3 / 18.4, 192 rows 26.7 / 19.7;  256 x 256: 512 rows 6.3 / 7.0, 1024 rows 7.5 / 7.1
-//   experts 60 of 1408 x 2048, 4 a token, shared 5632: 32 tokens 81.8 / 96.2 us, 64 tokens 113 / 102
-//           16 of 704 x 1024, 3 a token: 48 tokens 19.5 / 20.5, 96 tokens 23.5 / 21.4
-//           8 of 704 x 2048, 2 a token, shared 1408: 48 tokens 22.8 / 23.3, 64 tokens 25.8 / 23.4
-//           64 of 256 x 512, 6 a token: 16 tokens 15.2 / 17.5, 48 tokens 20.4 / 18.0
+//   experts 60 of 1408 x 2048, 4 a token, shared 5632: 32 tokens 80.8 / 99.6 us, 48 tokens 104 / 104, 64 tokens 113 / 107
+//           16 of 704 x 1024, 3 a token: 64 tokens 20.8 / 24.8, 96 tokens 23.4 / 25.0, 128 tokens 25.9 / 25.3
+//           8 of 704 x 2048, 2 a token, shared 1408: 64 tokens 25.8 / 27.5, 96 tokens 34.3 / 28.1
+//           64 of 256 x 512, 6 a token: 32 tokens 18.7 / 20.2, 48 tokens 20.4 / 20.1, 64 tokens 21.3 / 20.3
 static bool linear_tiles(int T, int N) {
   const int path = g_path.load(std::memory_order_relaxed);
   if (T <= kF8FewRows || path == 1) return false;
@@ -37,7 +37,7 @@ static bool ffn_tiles(int T, int K, int E, int H, int I) {
   if (T <= kF8FewRows || path == 1) return false;
   // work of the rows against a fixed cost and one for the weights
   const double size = static_cast<double>(H) * I;
-  return path == 2 || T > kF8StreamRows || static_cast<double>(T) * K * (size + 1.0e6) > 2.2e8 + 3.6 * size * E;
+  return path == 2 || T > kF8StreamRows || static_cast<double>(T) * K * (size + 1.0e6) > 3.6e8 + 2.5 * size * E;
 }
 
 // Rows per tile: the fewest of 32, 64, 128 with which the call's tiles (of 256 columns) still fit on the device
@@ -56,7 +56,7 @@ static int ffn_tile_rows(int T, int K, int E, int H, int I) {
 }
 
 // Rows of the shared expert's gate/up tiles: higher ones, beside routed tiles that leave less room.  128 tokens, 4 of 60
-// experts of 1408 x 2048 and a shared one of 5632: 176 tiles of 32 rows behind 600 routed ones 122 us, 88 of 64 109.
+// experts of 1408 x 2048 and a shared one of 5632: 176 tiles of 32 rows behind 600 routed ones 128 us, 88 of 64 116.
 static int ffn_shared_rows(int T, int K, int E, int I, int Is, int rows) {
   const int64_t routed = (static_cast<int64_t>(T) * K / rows + E / 2) * ((I + kPfBR / 2 - 1) / (kPfBR / 2));
   while (rows < kPfBM && routed + static_cast<int64_t>((T + rows - 1) / rows) * ((Is + kPfBR / 2 - 1) / (kPfBR / 2)) > 512) rows *= 2;
@@ -108,12 +108,14 @@ static FfnWs ffn_ws(void* ws, int T, int K, int E, int nseg, int H, int I, int I
   Carve c{static_cast<uint8_t*>(ws)};
   FfnWs w = {};
   const int64_t rows = nseg > 0 ? static_cast<int64_t>(T) * K : 0;
+  const bool tiles = ffn_tiles(T, K, E, H, I);
   if (T > kF8FewRows) {
-    w.x = take_rows(c, T, H);
+    if (tiles) w.x.values = static_cast<uint8_t*>(c.take(static_cast<size_t>(T) * f8_padded(H) * sizeof(uint16_t)));
+    else w.x = take_rows(c, T, H);
     w.h = take_rows(c, rows, I);
     if (Is > 0) w.sh = take_rows(c, T, Is);
   }
-  if (ffn_tiles(T, K, E, H, I)) {
+  if (tiles) {
     const int rows_per_tile = ffn_tile_rows(T, K, E, H, I);
     w.tiles = c.take(prefill_queue_ws_bytes(T, K, nseg, H, I, Is, rows_per_tile, f8_tile_columns(rows_per_tile),
                                             ffn_shared_rows(T, K, E, I, Is, rows_per_tile)));
@@ -269,7 +271,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
   const FfnWs w = ffn_ws(ws_dev, T, K, E, segs->n, H, I, Is);
 
   // One or two tokens: rows are quantised inside the products.  More: in launches of their own, beside products
-  // that stream weights; beside the tile kernel x only, which quantises the intermediate in its epilogue.
+  // that stream weights; beside the tiles x only, as gate/up quantises the intermediate in its epilogue.
   const bool few = T <= kF8FewRows, tiles = ffn_tiles(T, K, E, H, I);
   const int rows_per_tile = tiles ? ffn_tile_rows(T, K, E, H, I) : 0;
   int rc = SPARSE_HIP_OK;
@@ -279,7 +281,7 @@ int sparse_hip_fp8_moe_ffn(const sparse_hip_experts* experts, const void* x_dev,
     queues = prefill_queue_args(experts->expert_slot_dev, seg_offsets_dev, *segs, T, K, H, I, Is, w.tiles, &queue_args,
                                 rows_per_tile, f8_tile_columns(rows_per_tile),
                                 ffn_shared_rows(T, K, E, I, Is, rows_per_tile));
-    rc = f8_quantize_and_queue({x_dev, T, H, w.x.values, w.x.scales}, dtype, queue_args, st);
+    rc = f8_quantize_and_queue({x_dev, T, H, w.x.values, nullptr}, dtype, queue_args, st);
   } else if (!few) {
     rc = f8_quantize({x_dev, T, H, w.x.values, w.x.scales}, {}, dtype, st);
   }

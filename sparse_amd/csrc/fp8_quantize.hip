@@ -24,7 +24,9 @@ struct QuantizeArgs {
 };
 
 // kVec: rows start on 16-byte boundaries and K is a multiple of 8
-template <typename T, bool kVec>
+// kWide: what has been rounded to 8 bits leaves in bf16, times half its scale, and no scales (for kernels that multiply
+// in bf16: 2^-121 to 2^119 times an e4m3 value is a bf16 value)
+template <typename T, bool kVec, bool kWide>
 __device__ __forceinline__ void quantize_block(const QuantizeArgs& a, uint32_t block) {
   const int which = block >= a.first_blocks;
   if (which) block -= a.first_blocks;
@@ -61,13 +63,22 @@ __device__ __forceinline__ void quantize_block(const QuantizeArgs& a, uint32_t b
   uint32_t q[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) q[j] = f8_pack4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
-  *reinterpret_cast<uint4*>(a.values[which] + t * nb * kF8Block + k) = make_uint4(q[0], q[1], q[2], q[3]);
+  const int64_t at = t * nb * kF8Block + k;
+  if constexpr (kWide) {
+    const float half = __uint_as_float(static_cast<uint32_t>(s - 1 + kF8Bias) << 23);
+    uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.values[which]) + at);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      out[j] = __builtin_bit_cast(uint4, f8_widen8(q[2 * j], q[2 * j + 1], half));
+    return;
+  }
+  *reinterpret_cast<uint4*>(a.values[which] + at) = make_uint4(q[0], q[1], q[2], q[3]);
   if (threadIdx.x % kQzLanes == 0) a.scales[which][run] = static_cast<uint8_t>(s + kF8Bias);
 }
 
 template <typename T, bool kVec>
 __global__ __launch_bounds__(kQzThreads) void f8_quantize_kernel(const QuantizeArgs a) {
-  quantize_block<T, kVec>(a, blockIdx.x);
+  quantize_block<T, kVec, false>(a, blockIdx.x);
 }
 // The queue build is 20 workgroups that wait for memory most of their 5 to 10 us; beside the quantiser they cost
 // nothing.  They go first.
@@ -75,7 +86,7 @@ static_assert(kQzThreads == 256, "the queue build counts on 256 threads");
 template <typename T, bool kVec>
 __global__ __launch_bounds__(kQzThreads) void f8_quantize_queue_kernel(const QuantizeArgs a, const PfxMapArgs queue, uint32_t queue_blocks) {
   if (blockIdx.x < queue_blocks) prefill_queue_block(queue, blockIdx.x);
-  else quantize_block<T, kVec>(a, blockIdx.x - queue_blocks);
+  else quantize_block<T, kVec, true>(a, blockIdx.x - queue_blocks);
 }
 
 template <typename T>

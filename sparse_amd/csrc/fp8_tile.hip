@@ -1,37 +1,30 @@
-// Block-scaled 8-bit matrix products of many rows: the tile kernel.
+// Block-scaled 8-bit matrix products of many rows whose results are rounded to 16 bits (linear, down): the tile kernel.
 //
 //   y[m, n] = sum over blocks b of 2^e(m, b) s(n, b) sum over k in b of x[m, k] w[n, k]
 //
-// A workgroup of four wavefronts computes up to 128 rows x 256 weight rows (gate/up: 128 gate rows and the 128 up
-// rows of the same neurons) over 128-wide k slabs.  An 8-bit slab row is 128 bytes, as a 64-wide slab row of
-// the 16-bit kernels is, so the movement of data is theirs: activation rows, gathered through the
-// permutation, go to an LDS ring by direct global -> LDS copies with 16-byte chunks swizzled by row; weight
-// fragments come straight from the tiled layout into alternating register sets; everything is requested two
-// to four slabs ahead (tl_depth) and vector memory is awaited by count.  A slab is one 16x16x128 matrix
-// instruction per 16 x 16 tile where the 16-bit kernels have two of half the rate: the same bytes feed
-// twice the arithmetic.
+// A workgroup of four wavefronts computes up to 128 rows x 256 weight rows over 128-wide k slabs.  An 8-bit slab row is
+// 128 bytes, as a 64-wide slab row of the 16-bit kernels is, so the movement of data is theirs: activation rows go to an
+// LDS ring by direct global -> LDS copies with 16-byte chunks swizzled by row; weight fragments come straight from the
+// tiled layout into alternating register sets; everything is requested two to six slabs ahead (tl_depth) and vector
+// memory is awaited by count.  A slab is one 16x16x128 matrix instruction per 16 x 16 tile where the 16-bit kernels have
+// two of half the rate: the same bytes feed twice the arithmetic.
 //
 // Scales: the activations' E8M0 bytes of the whole tile are laid out in LDS once, the eight bytes that a
 // lane's eight row tiles need for a slab side by side, and enter the instruction as its own operand.  The
 // weights' fp32 scales multiply the slab's sum on its way into the accumulator, or, where all those of the tile are
 // powers of two, enter the instruction as exponents (4096 rows of 2048 by 5632 weight rows: 65 -> 57 us).  A tile
 // looks at its scales and chooses by itself: what a row comes out as depends on its own weights' scales alone, as
-// they are at the time of the call, and not on the other matrices of the call.
+// they are at the time of the call, and not on the other matrices of the call.  (The branch waits for the scales: 0.7 us
+// of such a call.  Behind the first copies instead, registers spill.)
 //
-// Gate/up ends in the quantiser: a tile's 128 neurons are one run of the intermediate, its largest magnitude is
-// found across the four wavefronts in LDS and 8-bit rows with their scales leave, a quarter of the bytes of fp32
-// ones and a launch less.
-//
-// What bounds it: two workgroups share a compute unit; in the steady loop their matrix instructions fill half of
-// the cycles (16 slabs of 128 rows: 27 us of both, 13.7 at the instruction's peak), and the 4.5 us before a
-// tile's first slab and 4 us behind its last are covered by the other workgroup only.  4096 rows of 2048 by 5632
-// weight rows: 51 us, 1.86 PFLOP/s (a library 8-bit product of that size: 51 us).  4096 tokens, 6 of 64 experts
-// of 1408 x 2048, shared 2816: gate/up 378 GFLOP in 194 to 221 us, down 189 GFLOP in 123 to 136.  Lower tiles for
-// a fuller last round lose: 96 rows 54 us, 64 rows 63.
+// What bounds it: two workgroups share a compute unit, whose matrix pipes are busy for 52 % of the cycles in which it has
+// work (linear; down 39 %); the 4.5 us before a tile's first slab and 4 us behind its last are covered by the other
+// workgroup only.  4096 rows of 2048 by 5632 weight rows: 51 us, 1.85 PFLOP/s (a library 8-bit product of that size:
+// 51 us).  Down of 4096 tokens, 6 of 64 experts of 1408 x 2048, shared 2816: 189 GFLOP in 124 us.  Lower tiles for a
+// fuller last round lose: 96 rows 54 us, 64 rows 63.
 #include <type_traits>
 
-#include "fp8.h"
-#include "prefill_tiles.h"
+#include "fp8_tile.h"
 
 namespace sparse {
 
@@ -56,8 +49,7 @@ constexpr int tl_younger_tail(int nmi, bool narrow, int j) {
   const int loads = narrow ? 4 : 8, behind = tl_depth(nmi, narrow) - 2 - j;
   return loads + behind * (nmi + loads);
 }
-constexpr int tl_wait(int vmcnt) { return 0x0F70 | (vmcnt & 15) | ((vmcnt >> 4) << 14); }
-static_assert(tl_younger(4, false) == 20 && tl_wait(20) == kWaitVmcnt20, "the count of the 16-bit kernels");
+static_assert(tl_younger(4, false) == 20, "the count of the 16-bit kernels");
 static_assert(tl_younger_tail(2, false, -1) == tl_younger(2, false) && tl_younger_tail(1, true, 4) == 4, "one rule for both");
 static_assert(tl_younger(2, false) < 64 && tl_younger(1, false) < 64 && tl_younger(1, true) < 64, "six bits");
 static_assert((tl_depth(1, false) + 1) * 32 * kTlRowBytes <= kTlRing && (tl_depth(2, false) + 1) * 64 * kTlRowBytes <= kTlRing, "rings fit");
@@ -66,40 +58,14 @@ constexpr int kTlNarrowRing = (tl_depth(1, true) + 1) * kTlNarrowRows * kTlRowBy
 constexpr int kTlScaleBytes = kPfBM + 2 * sizeof(float);   // per slab: activation bytes, two weight scales
 static_assert(kTlSlab == kPfLdsA, "the slab geometry is that of the 16-bit kernels");
 
-template <typename T>
-__device__ __forceinline__ T* uniform_ptr(T* p) {
-  const uint64_t v = reinterpret_cast<uint64_t>(p);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
-  return reinterpret_cast<T*>((static_cast<uint64_t>(hi) << 32) | lo);
-}
-
-// A power of two that is a normal fp32 number, 2^-126 to 2^127: its exponent is all there is to it.
-__device__ __forceinline__ bool tl_is_exponent(float v) {
-  const uint32_t b = __float_as_uint(v);
-  return (b & 0x807fffffu) == 0 && b - 0x00800000u <= 0x7f000000u - 0x00800000u;
-}
-
-struct TileArgs {
-  F8Product p;
-  const PfTile* map;       // NULL: dense operands only, the tile comes from the block number
-  const int32_t* qhdr;
-  uint32_t topk_magic;     // ceil(2^32 / topk); 0 for topk == 1
-  int32_t mt, nt, rows;    // row and column tiles when map is NULL, rows per tile
-  // gate/up: where the quantised rows go
-  uint8_t *q_r, *qs_r, *q_s, *qs_s;
-};
-
 // F: the 16-bit format of outputs, route weights and gate logits
-// kNarrow: tiles of 32 rows by 128, three workgroups to a compute unit instead of two (not for gate/up)
-template <typename F, bool kGateUp, bool kNarrow>
+// kNarrow: tiles of 32 rows by 128, three workgroups to a compute unit instead of two
+template <typename F, bool kNarrow>
 __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(const TileArgs a) {
   constexpr int NG = kNarrow ? 2 : 4;                         // 16-row groups of weights per wavefront
   constexpr int kRows = kNarrow ? kTlNarrowRows : kPfBM;
-  static_assert(!(kNarrow && kGateUp), "gate/up tiles are wide: their 128 neurons are one run of the quantiser");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kNarrow ? kTlNarrowRing : kTlRing];
-  __shared__ float s_row[kPfBM];          // factor of a row (down), exponent of a row's scale (gate/up)
-  __shared__ float s_amax[kGateUp ? 4 : 1][kPfBM];
+  __shared__ float s_row[kPfBM];          // factor of a row
   extern __shared__ __attribute__((aligned(16))) uint8_t s_scales[];   // [nk][128] bytes, then [nk][2] floats
 
   const int tid = threadIdx.x;
@@ -111,13 +77,7 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
   // ---- which tile (wavefront-uniform) ------------------------------------------------
   int slot, r0, M, bn;
   if (a.map != nullptr) {
-    const int xcd = blockIdx.x % kPfXcds, rank = blockIdx.x / kPfXcds;
-    if (rank >= a.qhdr[kPfXcds + xcd]) return;   // the grid is sized for the longest possible queue
-    const PfTile tile = a.map[a.qhdr[xcd] + rank];
-    slot = __builtin_amdgcn_readfirstlane(tile.slot);
-    r0 = __builtin_amdgcn_readfirstlane(tile.r0);
-    M = __builtin_amdgcn_readfirstlane(tile.rows);
-    bn = __builtin_amdgcn_readfirstlane(tile.bn);
+    if (!tl_queued(a, slot, r0, M, bn)) return;
   } else {
     // block b runs on XCD b % 8; an XCD takes a contiguous share of the (column tile, row tile) order
     const int total = a.mt * a.nt, xcd = blockIdx.x % kPfXcds, rank = blockIdx.x / kPfXcds;
@@ -134,7 +94,7 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
   const int Kdim = dense ? a.p.Ks : a.p.Kr, N = dense ? a.p.Ns : a.p.Nr;
   const int nk = (Kdim + kF8Block - 1) / kF8Block;
   const uint32_t ld = static_cast<uint32_t>(nk) * kF8Block;
-  const int n0 = bn * (kGateUp ? kPfBR / 2 : 64 * NG);   // first output column of this tile
+  const int n0 = bn * 64 * NG;   // first output column of this tile
 
   // ---- operand addresses ------------------------------------------------------------
   // Row r keeps chunk 2q + h at position (q + 4h) ^ f(r), f(r) = ((r >> 1) & 7) ^ ((r & 1) << 2); of eight rows
@@ -142,47 +102,31 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
   const int l3 = lane >> 3;
   const int pos0 = (lane & 7) ^ ((l3 >> 1) ^ ((l3 & 1) << 2));
   const uint32_t chunk0 = ((pos0 & 3) << 1) | (pos0 >> 2);
-  const bool gather = !dense && a.p.gather != 0;
-  // rows that are not gathered are addressed from the tile's first one, so that 32-bit offsets always reach
-  const size_t row_base = gather ? 0 : static_cast<size_t>(r0);
-  const uint8_t* abase = uniform_ptr((dense ? a.p.act_s : a.p.act_r) + row_base * ld);
-  const uint8_t* sbase = (dense ? a.p.act_ss : a.p.act_rs) + row_base * nk;
-  auto source_row = [&](int m) -> uint32_t {
-    const int mm = min(m, M - 1);
-    if (!gather) return static_cast<uint32_t>(mm);
-    uint32_t g = static_cast<uint32_t>(a.p.perm[r0 + mm]);
-    return a.topk_magic != 0 ? __umulhi(g, a.topk_magic) : g;
-  };
-  // The wavefront's 64 weight rows are four 16-row groups (gate/up: groups 0, 1 gate rows of 32 neurons,
-  // groups 2, 3 the up rows of the same neurons); a group's slab is 2 KB, its two halves 1 KB each in lane order.
+  // rows are addressed from the tile's first one, so that 32-bit offsets always reach
+  const uint8_t* abase = uniform_ptr((dense ? a.p.act_s : a.p.act_r) + static_cast<size_t>(r0) * ld);
+  const uint8_t* sbase = (dense ? a.p.act_ss : a.p.act_rs) + static_cast<size_t>(r0) * nk;
+  auto source_row = [&](int m) { return static_cast<uint32_t>(min(m, M - 1)); };
+  // The wavefront's 64 weight rows are four 16-row groups; a group's slab is 2 KB, its two halves 1 KB each in lane order.
   const uint8_t* wbase[NG];
-  const float *ws0, *ws1;      // the scales of the tile's two 128-row blocks (gate/up: of gate and of up)
+  const float *ws0, *ws1;      // the scales of the tile's two 128-row blocks
   const uint32_t woff = lane * 16;
   {
-    const uint8_t *w0, *w1;
-    const float *s0, *s1;
-    if (dense) {
-      w0 = a.p.w0;
-      w1 = a.p.w1;
-      s0 = a.p.s0;
-      s1 = a.p.s1;
-    } else {
+    const uint8_t* w0 = a.p.w0;
+    const float* s0 = a.p.s0;
+    if (!dense) {
       const uint8_t* base = a.p.slab + static_cast<uint64_t>(slot) * a.p.slot_stride;
       w0 = base + a.p.off0;
-      w1 = base + a.p.off1;
       s0 = reinterpret_cast<const float*>(base + a.p.soff0);
-      s1 = reinterpret_cast<const float*>(base + a.p.soff1);
     }
     const int last16 = ((N + 15) & ~15) - 16;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const uint8_t* base = (kGateUp && g >= 2) ? w1 : w0;
-      const int n = min(kGateUp ? (n0 + wave * 32 + (g & 1) * 16) : (n0 + wave * 16 * NG + g * 16), last16);
-      wbase[g] = uniform_ptr(base + static_cast<size_t>(n >> 4) * nk * kF8TileBytes);
+      const int n = min(n0 + wave * 16 * NG + g * 16, last16);
+      wbase[g] = uniform_ptr(w0 + static_cast<size_t>(n >> 4) * nk * kF8TileBytes);
     }
     const int nblk = (N + kF8Block - 1) / kF8Block, b0 = n0 / kF8Block;
     ws0 = s0 + static_cast<size_t>(b0) * nk;
-    ws1 = kGateUp ? s1 + static_cast<size_t>(b0) * nk : s0 + static_cast<size_t>(min(b0 + 1, nblk - 1)) * nk;
+    ws1 = s0 + static_cast<size_t>(min(b0 + 1, nblk - 1)) * nk;
   }
   typedef const __attribute__((address_space(1))) char* gptr_t;
   auto wload = [&](int g, int slab, int h) __attribute__((always_inline)) {
@@ -211,10 +155,10 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
     for (int i = lane; i < 2 * nk; i += 64) {
       const float v = ((i & 1) ? ws1 : ws0)[i >> 1];
       if (((i >> 6) & 3) == wave) w[i] = v;
-      odd |= !(kNarrow && (i & 1)) && !tl_is_exponent(v);      // (a narrow tile lies in one 128-row block)
+      odd |= !(kNarrow && (i & 1)) && !tl_is_exponent<-126, 127>(v);      // (a narrow tile lies in one 128-row block)
     }
-    // down: factor of each row, the route weight or the sigmoid of the shared expert's gate
-    if (!kGateUp && tid < kPfBM) {
+    // factor of each row, the route weight or the sigmoid of the shared expert's gate
+    if (tid < kPfBM) {
       float sc = 1.f;
       if (tid < M) {
         const int p = r0 + tid;
@@ -291,7 +235,7 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
       const uint8_t* la = lds + cur * kSlab + a_row;
       const uint2 sb = *reinterpret_cast<const uint2*>(s_scales + kt * kPfBM + fr * 8);
       const float2 sw = *reinterpret_cast<const float2*>(s_scales + nk * kPfBM + kt * 8);
-      const float sw0 = kGateUp || kNarrow || wave < 2 ? sw.x : sw.y, sw1 = kGateUp ? sw.y : sw0;
+      const float w = kNarrow || wave < 2 ? sw.x : sw.y;
       i32x4 fa[2][2][2];   // [parity][tile of the pair][half]
       if (NP == 1 && kTail < 0) {       // the copies go first, so that every height issues vector memory in the counted order
         stage_slab(kts, ahead);
@@ -307,7 +251,6 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
       auto mul = [&](auto mt_c, auto g_c, const i32x4 (&f)[2]) __attribute__((always_inline)) {
         constexpr int mt = decltype(mt_c)::value, g = decltype(g_c)::value;
         const int sbv = static_cast<int>(mt < 4 ? sb.x : sb.y);
-        const float w = g < 2 ? sw0 : sw1;
         const i32x8 wf = f8_join(wfrag[st][0][g], wfrag[st][1][g]), xf = f8_join(f[0], f[1]);
         if constexpr (kPow2) {
           acc[mt][g] = f8_mfma<0, mt & 3>(wf, xf, acc[mt][g], static_cast<int>(__float_as_uint(w) >> 23), sbv);
@@ -383,92 +326,44 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
     // ---- epilogue ----------------------------------------------------------------
     // The product was formed as W * X^T: a lane holds row m = 16*mt + fr and, per 16-row weight group, four
     // consecutive output columns 4*fq + j.
-    if constexpr (kGateUp) {
-      // SwiGLU, then the row's largest magnitude over the tile's 128 neurons (which are one run of the
-      // quantiser): over a lane's values, its row's four lanes, the four wavefronts.
+    // 16-bit rows times their factor, staged per wavefront in two 32-column passes into 16-byte stores
+    uint8_t* st = lds + wave * (kRows * 64);
+    uint16_t* out = static_cast<uint16_t*>(dense ? a.p.out_s : a.p.out_r);
+    // whole 16-byte stores need rows that start on 16-byte boundaries
+    const bool whole = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
-      for (int mt = 0; mt < NMT; ++mt) {
-        float m = 0.f;
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float h = silu_f32(acc[mt][p][j]) * acc[mt][2 + p][j];
-            acc[mt][p][j] = n0 + wave * 32 + p * 16 < N ? h : 0.f;   // columns behind the matrix's end (a multiple of 16)
-            m = fmaxf(m, f8_magnitude(acc[mt][p][j]));
-          }
-        m = fmaxf(m, __shfl_xor(m, 16));
-        m = fmaxf(m, __shfl_xor(m, 32));
-        if (fq == 0) s_amax[wave][mt * 16 + fr] = m;
-      }
-      __syncthreads();
-      uint8_t* st = lds;             // 128 rows x 128 bytes, 16-byte chunks swizzled by row
+    for (int pass = 0; pass < NG / 2; ++pass) {
+      if (pass) __syncthreads();  // staging rows are reused
 #pragma unroll
       for (int mt = 0; mt < NMT; ++mt) {
         const int m = mt * 16 + fr;
-        const float top = fmaxf(fmaxf(s_amax[0][m], s_amax[1][m]), fmaxf(s_amax[2][m], s_amax[3][m]));
-        const float inv = f8_inverse(f8_exponent(top));
+        const float sc = s_row[m];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const int chunk = (wave * 2 + p) ^ (m & 7);
-          *reinterpret_cast<uint32_t*>(st + m * 128 + chunk * 16 + fq * 4) =
-              f8_pack4(acc[mt][p][0] * inv, acc[mt][p][1] * inv, acc[mt][p][2] * inv, acc[mt][p][3] * inv);
+          const vf32x4 v = acc[mt][2 * pass + p];
+          uint2 pk;
+          pk.x = F::pack2(v[0] * sc, v[1] * sc);
+          pk.y = F::pack2(v[2] * sc, v[3] * sc);
+          const int chunk = (2 * p + (fq >> 1)) ^ ((m >> 1) & 3);
+          *reinterpret_cast<uint2*>(st + m * 64 + chunk * 16 + (fq & 1) * 8) = pk;
         }
       }
       __syncthreads();
-      const int nb = (N + kF8Block - 1) / kF8Block;
-      uint8_t* out = dense ? a.q_s : a.q_r;
-      uint8_t* outs = dense ? a.qs_s : a.qs_r;
+      const int ncol0 = n0 + wave * 16 * NG + pass * 32;
 #pragma unroll
-      for (int it = 0; it < NMI; ++it) {
-        const int m = it * 32 + (tid >> 3), c = tid & 7;
-        const i32x4 v = *reinterpret_cast<const i32x4*>(st + m * 128 + (c ^ (m & 7)) * 16);
-        if (m < M) *reinterpret_cast<i32x4*>(out + (static_cast<size_t>(r0 + m) * nb + bn) * kF8Block + c * 16) = v;
-      }
-      if (tid < M) {
-        const float top = fmaxf(fmaxf(s_amax[0][tid], s_amax[1][tid]), fmaxf(s_amax[2][tid], s_amax[3][tid]));
-        outs[static_cast<size_t>(r0 + tid) * nb + bn] = static_cast<uint8_t>(f8_exponent(top) + kF8Bias);
-      }
-    } else {
-      // 16-bit rows times their factor, staged per wavefront in two 32-column passes into 16-byte stores
-      uint8_t* st = lds + wave * (kRows * 64);
-      uint16_t* out = static_cast<uint16_t*>(dense ? a.p.out_s : a.p.out_r);
-      // whole 16-byte stores need rows that start on 16-byte boundaries
-      const bool whole = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+      for (int it = 0; it < 2 * NMI; ++it) {
+        const int m = it * 16 + (lane >> 2), q = lane & 3;
+        const uint4 val = *reinterpret_cast<const uint4*>(st + m * 64 + (q ^ ((m >> 1) & 3)) * 16);
+        const int n = ncol0 + q * 8;
+        if (m >= M || n >= N) continue;
+        uint16_t* o = out + static_cast<size_t>(r0 + m) * N + n;
+        if (whole) {
+          *reinterpret_cast<uint4*>(o) = val;
+        } else {
+          const uint32_t v[4] = {val.x, val.y, val.z, val.w};
 #pragma unroll
-      for (int pass = 0; pass < NG / 2; ++pass) {
-        if (pass) __syncthreads();  // staging rows are reused
-#pragma unroll
-        for (int mt = 0; mt < NMT; ++mt) {
-          const int m = mt * 16 + fr;
-          const float sc = s_row[m];
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const vf32x4 v = acc[mt][2 * pass + p];
-            uint2 pk;
-            pk.x = F::pack2(v[0] * sc, v[1] * sc);
-            pk.y = F::pack2(v[2] * sc, v[3] * sc);
-            const int chunk = (2 * p + (fq >> 1)) ^ ((m >> 1) & 3);
-            *reinterpret_cast<uint2*>(st + m * 64 + chunk * 16 + (fq & 1) * 8) = pk;
-          }
-        }
-        __syncthreads();
-        const int ncol0 = n0 + wave * 16 * NG + pass * 32;
-#pragma unroll
-        for (int it = 0; it < 2 * NMI; ++it) {
-          const int m = it * 16 + (lane >> 2), q = lane & 3;
-          const uint4 val = *reinterpret_cast<const uint4*>(st + m * 64 + (q ^ ((m >> 1) & 3)) * 16);
-          const int n = ncol0 + q * 8;
-          if (m >= M || n >= N) continue;
-          uint16_t* o = out + static_cast<size_t>(r0 + m) * N + n;
-          if (whole) {
-            *reinterpret_cast<uint4*>(o) = val;
-          } else {
-            const uint32_t v[4] = {val.x, val.y, val.z, val.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (n + j < N) o[j] = static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1)));
-          }
+          for (int j = 0; j < 8; ++j)
+            if (n + j < N) o[j] = static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1)));
         }
       }
     }
@@ -486,33 +381,17 @@ __global__ __launch_bounds__(kPfThreads, kNarrow ? 3 : 2) void f8_tile_kernel(co
   else bodies(std::false_type{});
 }
 
-template <bool kGateUp, bool kNarrow>
+template <bool kNarrow>
 static int launch_tile(const TileArgs& a, int64_t grid, hipStream_t st) {
   SP_REQUIRE(grid < (1ll << 31), "fp8 product: grid too large");
   const int Kmax = a.p.Ks > a.p.Kr ? a.p.Ks : a.p.Kr;
   const unsigned dyn = static_cast<unsigned>(f8_blocks(Kmax)) * kTlScaleBytes;
   if (a.p.dtype == SPARSE_HIP_F16)
-    hipLaunchKernelGGL((f8_tile_kernel<Fp16, kGateUp, kNarrow>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
+    hipLaunchKernelGGL((f8_tile_kernel<Fp16, kNarrow>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
   else
-    hipLaunchKernelGGL((f8_tile_kernel<Bf16, kGateUp, kNarrow>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
+    hipLaunchKernelGGL((f8_tile_kernel<Bf16, kNarrow>), dim3(static_cast<unsigned>(grid)), dim3(kPfThreads), dyn, st, a);
   SP_LAUNCH_CHECK("f8_tile_kernel");
   return SPARSE_HIP_OK;
-}
-
-static inline int64_t queue_grid(int cap) { return (static_cast<int64_t>(cap - 1) / kPfXcds + 2) * kPfXcds; }
-static inline uint32_t magic(int topk) { return topk == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + topk - 1) / topk); }
-
-int f8_tile_gateup(const F8Product& p, const PfQueues& q, void* h, void* hs, void* sh, void* shs, hipStream_t st) {
-  TileArgs a = {};
-  a.p = p;
-  a.map = q.map_gu;
-  a.qhdr = q.hdr;
-  a.topk_magic = magic(p.topk);
-  a.q_r = static_cast<uint8_t*>(h);
-  a.qs_r = static_cast<uint8_t*>(hs);
-  a.q_s = static_cast<uint8_t*>(sh);
-  a.qs_s = static_cast<uint8_t*>(shs);
-  return launch_tile<true, false>(a, queue_grid(q.cap_gu), st);
 }
 
 int f8_tile_columns(int tile_rows) { return tile_rows <= kTlNarrowRows ? kPfBR / 2 : kPfBR; }
@@ -522,8 +401,8 @@ int f8_tile_down(const F8Product& p, const PfQueues& q, int tile_rows, hipStream
   a.p = p;
   a.map = q.map_dn;
   a.qhdr = q.hdr + 16;
-  return tile_rows <= kTlNarrowRows ? launch_tile<false, true>(a, queue_grid(q.cap_dn), st)
-                                    : launch_tile<false, false>(a, queue_grid(q.cap_dn), st);
+  return tile_rows <= kTlNarrowRows ? launch_tile<true>(a, tl_queue_grid(q.cap_dn), st)
+                                    : launch_tile<false>(a, tl_queue_grid(q.cap_dn), st);
 }
 
 int f8_tile_linear(const F8Product& p, int tile_rows, hipStream_t st) {
@@ -536,7 +415,7 @@ int f8_tile_linear(const F8Product& p, int tile_rows, hipStream_t st) {
   const int64_t total = static_cast<int64_t>(a.mt) * a.nt;
   SP_REQUIRE(total < (1ll << 30), "fp8_linear: too many tiles");
   const int64_t grid = (total + kPfXcds - 1) / kPfXcds * kPfXcds;
-  return tile_rows <= kTlNarrowRows ? launch_tile<false, true>(a, grid, st) : launch_tile<false, false>(a, grid, st);
+  return tile_rows <= kTlNarrowRows ? launch_tile<true>(a, grid, st) : launch_tile<false>(a, grid, st);
 }
 
 }  // namespace sparse

@@ -37,7 +37,8 @@ def heights(T, Is):
     before = lib.sparse_hip_fp8_path(2)
     total = lib.sparse_hip_fp8_moe_ffn_ws_bytes(T, K, E, E, H, I, Is)
     lib.sparse_hip_fp8_path(before)
-    for rows, k in ((T, H), (T * K, I)) + (((T, Is),) if Is else ()):
+    total -= up(2 * T * fp8.padded(H), 256) * 256                 # x in bf16
+    for rows, k in ((T * K, I),) + (((T, Is),) if Is else ()):
         total -= up(rows * fp8.padded(k), 256) * 256 + up(rows * fp8.blocks(k), 256) * 256
     fits = [(r, s) for r in (32, 64, 128) for s in (32, 64, 128) if s >= r and queue_bytes(T, Is, r, s) == total]
     assert fits, total
