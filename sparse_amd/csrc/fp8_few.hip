@@ -20,7 +20,7 @@
 // and the weights' fp32 scale on its way into the accumulator.
 //
 // One token of 4 among 60 experts of 1408 x 2048 and a shared one of 5632: gate/up 46 MB in 9 to 11 us, down 23 MB in
-// 8.2 to 9.2; a single 5632 x 2048 matrix, 11.5 MB, 5.3 us (from the last-level cache).  At the 7 TB/s of longer
+// 7.9 to 9.2; a single 5632 x 2048 matrix, 11.5 MB, 5.3 us (from the last-level cache).  At the 7 TB/s of longer
 // streams that would be 6.6 and 3.3 us: the rest is the start of a launch (2.5 us until the first weights arrive, by
 // time stamps in the kernel) and its end (1.5 us of sums and stores), and in down the shared expert's six chunks.
 #include "fp8.h"

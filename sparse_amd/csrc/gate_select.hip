@@ -13,7 +13,7 @@
 // A group's sum of two is as far off as its two terms together, however small it is itself: where large biases
 // of both signs cancel in it, the 32-bit sum may be rounding alone.
 // 32-bit maxima cross the lanes in one instruction a step where 64-bit ones take a dozen: one token of 256
-// experts in 8 groups 8.7 -> 5.4 us, 4096 tokens 17.1 -> 12.5 us.  What is left is the latency of the K + 1
+// experts in 8 groups 8.7 -> 5.8 us, 4096 tokens 17.1 -> 13.6 us.  What is left is the latency of the K + 1
 // maxima, one behind the other, of the groups and of the exponentials in 64 bits: 4 MB of logits are read in a
 // microsecond.
 #include "common.h"

@@ -201,7 +201,9 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def linear(x: Union[torch.Tensor, Rows], weight: Weight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x W^T`` with ``x [T, K]`` (bf16 or fp16) quantised inside the call, or given as ``Rows`` of such an x:
-    ``[T, N]`` in x's dtype, accumulated in fp32 and rounded once."""
+    ``[T, N]`` in x's dtype, accumulated in fp32 and rounded once.  (From three rows on the matrix instruction forms
+    sums of eight products with 13 bits below the largest: some ``2**-15`` of a usual result.)  ``out`` must not share
+    memory with x."""
     dtype = x.dtype
     if dtype not in HALF_DTYPES:
         raise ValueError(f"x must be bfloat16 or float16, got {dtype}")
@@ -356,7 +358,8 @@ def moe_ffn(experts: ExpertSlab, x: torch.Tensor, topv: torch.Tensor, perm: Perm
     """Routed experts (over ``segs``, by default every active one) and the shared expert of one call of any
     size on 8-bit weights: returns ``(parts [T*K, H]`` in permuted order, each row times its route weight,
     ``shared [T, H]`` or None``)`` for ``ops.combine``.  ``x [T, H]`` bf16 or fp16, ``topv [T, K]`` of the same
-    dtype; ``shared_gate [T]``: logits whose sigmoid multiplies the shared rows.  ``ws``: a byte tensor of
+    dtype; ``shared_gate [T]``: logits whose sigmoid multiplies the shared rows.  Gate and up, which are rounded to 8
+    bits next, are products added in fp32 at every size; the down projection is summed as in ``linear``.  ``ws``: a byte tensor of
     ``moe_ffn_ws_bytes`` for callers that keep one."""
     _need_half(x, "x")
     if x.dim() != 2 or topv.dim() != 2:
