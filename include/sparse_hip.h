@@ -478,7 +478,8 @@ int sparse_hip_fp8_quantize(const void* x_dev, int dtype, int T, int K, void* va
  * or x_dev is NULL and xq_dev / xs_dev hold the rows' values and scales (no workspace).  `pow2_scales`: not 0 lets
  * a call of many rows hand scales to the matrix instruction as exponents, which is faster, in each tile whose
  * scales the kernel finds to be powers of two (2^-126 to 2^127); 0 has all of them multiplied in fp32.  Both are
- * right for any scales.  Up to 2^28 rows and 2^16 columns.
+ * right for any scales.  (A block's sum is formed before the weight's scale is applied: x times 8-bit weight
+ * values, summed over a block, has to stay within fp32.)  Up to 2^28 rows and 2^16 columns.
  */
 size_t sparse_hip_fp8_linear_ws_bytes(int T, int K);
 int sparse_hip_fp8_linear(const void* x_dev, const void* xq_dev, const void* xs_dev, int dtype, int T,

@@ -535,3 +535,53 @@ def test_linear_into_its_own_rows_is_refused(device, T):
         with pytest.raises(ValueError, match="overlaps"):
             fp8.linear(buf[:T], w, out)
     assert torch.equal(fp8.linear(buf[:T], w, buf[T:]), fp8.linear(buf[:T].clone(), w))
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("T", [1, 7, 40])
+def test_experts_far_from_one(path, device, T, pow2):
+    """Rows near both ends of the range beside weights whose scales bring gate and up back: runs of the lowest scale,
+    scales that bf16 takes in and scales that it does not."""
+    for lo, hi in ((2.0 ** -124, 2.0 ** 116), (2.0 ** -110, 2.0 ** 108), (2.0 ** 96, 2.0 ** -99), (2.0 ** 60, 2.0 ** -62)):
+        c = make_case(T, 192, 3, 128, 2, 192, False, torch.bfloat16, seed=61, pow2=pow2)
+        c["x"] = (c["x"].float() * lo).to(torch.bfloat16)
+
+        def far(t):
+            return (t[0][0], t[0][1] * hi), (t[1][0], t[1][1] * hi), t[2]
+
+        c["ex"], c["sh"] = [far(t) for t in c["ex"]], far(c["sh"])
+        d = on_gpu(c, device)
+        parts, shared = fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"], shared=d["sh"])
+        want, bound, wsh, bsh = oracle(c, path)
+        within(parts, want, bound, torch.bfloat16)
+        within(shared, wsh, bsh, torch.bfloat16)
+
+
+@pytest.mark.parametrize("T", [2, 6, 150])
+def test_experts_nan_stays_in_its_row(path, device, T):
+    c = make_case(T, 256, 4, 192, 2, 128, True, torch.bfloat16, seed=71)
+    d = on_gpu(c, device)
+    clean, clean_sh = fp8.moe_ffn(d["slab"], d["x"], d["topv"], d["perm"], shared=d["sh"], shared_gate=d["sg"])
+    x = d["x"].clone()
+    x[0, 7], x[T - 1, 200] = math.nan, math.inf
+    parts, shared = fp8.moe_ffn(d["slab"], x, d["topv"], d["perm"], shared=d["sh"], shared_gate=d["sg"])
+    token = d["perm"].perm.long() // 2
+    hit = (token == 0) | (token == T - 1)
+    assert bool(torch.isnan(parts[hit]).all()) and torch.equal(parts[~hit], clean[~hit])
+    rest = [t for t in range(T) if t not in (0, T - 1)]
+    assert bool(torch.isnan(shared[0]).all()) and bool(torch.isnan(shared[T - 1]).all()) and torch.equal(shared[rest], clean_sh[rest])
+
+
+def test_scales_multiplied_in_fp32_on_request(device):
+    """The C entry's switch: scales that are powers of two multiplied like any others."""
+    T, K, N = 300, 384, 256
+    x, (q, s) = rand_rows(T, K, torch.bfloat16), rand_weight(N, K, pow2=True)
+    w = fp8.Weight.from_quantized(q.to(device), s.to(device))
+    rows = fp8.quantize(x.to(device))
+    want, bound = ref_fp8.product(ref_fp8.rows(x), (q, s), True)
+    for flag in (0, 1):
+        out = torch.empty(T, N, dtype=torch.bfloat16, device=device)
+        rc = ops.call_on(0, _lib.load().sparse_hip_fp8_linear, None, rows.data.data_ptr(), rows.scales.data_ptr(), 1, T, w.ref, flag,
+                         out.data_ptr(), None)
+        assert rc == 0
+        within(out, want, bound, torch.bfloat16)
